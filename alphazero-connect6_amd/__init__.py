@@ -51,7 +51,9 @@ ENGINE_SYMBOLS = ["c6_last_error", "c6_version", "c6_rng_spec", "c6_device_count
                   "c6_group_create", "c6_group_destroy", "c6_group_size", "c6_group_engine", "c6_group_member_info", "c6_group_uses_rccl",
                   "c6_group_load_weights", "c6_group_set_callback", "c6_group_step", "c6_group_run", "c6_group_sync", "c6_group_stats",
                   "c6_group_fetch_games", "c6_group_enable_tuples", "c6_group_pool_begin", "c6_group_pool_end", "c6_group_pool_tuples",
-                  "c6_group_pooled", "c6_group_fetch_pooled", "c6_group_push_pooled"]
+                  "c6_group_pooled", "c6_group_fetch_pooled", "c6_group_push_pooled",
+                  "c6_logits_process", "c6_policy_loss_workspace", "c6_policy_loss", "c6_policy_loss_grad", "c6_clip_create", "c6_clip_destroy",
+                  "c6_clip_workspace", "c6_clip_norm", "c6_clip_apply"]
 
 
 class C6Error(RuntimeError):
@@ -91,6 +93,11 @@ class Profile(C.Structure):
 
 class RolloutInfo(C.Structure):
     _fields_ = [("nodes", C.c_uint32), ("edges", C.c_uint32), ("searches", C.c_uint32), ("uid", C.c_uint32)]
+
+
+class Logits(C.Structure):  # c6_logits
+    _fields_ = [("rows", C.c_int), ("width", C.c_int), ("type", C.c_int), ("device", C.c_int), ("x", C.c_void_p), ("x_stride", C.c_int64),
+                ("mask", C.c_void_p), ("mask_row", C.c_int64), ("mask_byte", C.c_int64)]
 
 
 class Path(C.Structure):  # cppbind/.../rawobj/mod.rs:29-36
@@ -236,6 +243,19 @@ def lib():
         L.c6_group_pooled.restype = C.c_void_p
         L.c6_group_fetch_pooled.argtypes = [C.c_void_p, C.c_int, C.c_size_t, C.POINTER(C.c_size_t), C.c_void_p]
         L.c6_group_push_pooled.argtypes = [C.c_void_p, C.c_int, C.c_void_p]
+    if hasattr(L, "c6_logits_process"):      # (absent from A/B libraries built from earlier sources)
+        vp, i64 = C.c_void_p, C.c_int64
+        L.c6_logits_process.argtypes = [C.POINTER(Logits), vp, i64, vp, C.c_int, vp, i64, vp, i64, vp, i64, vp]
+        L.c6_policy_loss_workspace.argtypes = [C.c_int, C.c_int]
+        L.c6_policy_loss_workspace.restype = C.c_size_t
+        L.c6_policy_loss.argtypes = [C.POINTER(Logits), vp, C.c_int, i64, vp, vp, vp, vp, i64, C.c_float, vp, C.c_size_t, vp]
+        L.c6_policy_loss_grad.argtypes = [C.POINTER(Logits), vp, C.c_int, i64, vp, vp, vp, i64, vp, i64, vp]
+        L.c6_clip_create.argtypes = [C.c_int, C.POINTER(vp), C.POINTER(vp), C.POINTER(C.c_size_t), C.POINTER(C.c_int), C.c_int, C.POINTER(vp)]
+        L.c6_clip_destroy.argtypes = [vp]
+        L.c6_clip_workspace.argtypes = [vp]
+        L.c6_clip_workspace.restype = C.c_size_t
+        L.c6_clip_norm.argtypes = [vp, vp, vp, C.c_size_t, vp]
+        L.c6_clip_apply.argtypes = [vp, C.c_float, vp, vp, C.c_size_t, vp]
     L.cpp_self_play.restype = Vec
     L.cpp_self_play.argtypes = [CALLBACK, ALLOC_PATH, ALLOC_RESULT, C.c_int, C.c_float, C.c_double, C.c_float, C.c_bool, C.c_int]
     L.cpp_play.restype = Vec

@@ -1,0 +1,173 @@
+// grad_clip.hip -- global gradient norm over many tensors and clipping (include/connect6_amd.h part 7, c6_clip_*).
+#include "c6_ops.h"
+
+#include <algorithm>
+#include <vector>
+
+namespace {
+
+struct Chunk {                    // a piece of one tensor, the work of one workgroup at a time
+    const void *src;
+    void *dst;
+    uint32_t n, type;
+};
+constexpr uint32_t CHUNK = 32768;         // elements
+constexpr int MAXPART = 2048;             // partial sums: workgroups of the norm's pass
+
+__device__ double block_sum(double v, double *red) {
+    v = c6_wave_all(v, [](double a, double b) { return a + b; });
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// Squares are taken and summed in 64 bits: 1e30^2 does not overflow and 1e-30^2 does not vanish.
+template <typename T>
+__device__ double chunk_squares(const T *x, uint32_t n) {
+    double s = 0;
+    for (uint32_t i = threadIdx.x; i < n; i += 256) {
+        const double g = (double)c6_get(x[i]);
+        s = __builtin_fma(g, g, s);
+    }
+    return s;
+}
+
+__global__ __launch_bounds__(256) void c6_clip_norm_kernel(const Chunk *table, int chunks, double *partial) {
+    __shared__ double red[4];
+    double s = 0;
+    for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+        const Chunk k = table[c];
+        C6_BY_TYPE(k.type, T, s += chunk_squares((const T *)k.src, k.n));
+    }
+    s = block_sum(s, red);
+    if (threadIdx.x == 0) partial[blockIdx.x] = s;
+}
+
+__device__ double total_norm(const double *partial, int parts, double *red) {
+    double s = 0;
+    for (int i = threadIdx.x; i < parts; i += 256) s += partial[i];
+    return sqrt(block_sum(s, red));
+}
+
+__global__ __launch_bounds__(256) void c6_clip_finish_kernel(const double *partial, int parts, float *norm) {
+    __shared__ double red[4];
+    const double n = total_norm(partial, parts, red);
+    if (threadIdx.x == 0) *norm = (float)n;
+}
+
+__global__ __launch_bounds__(256) void c6_clip_apply_kernel(const Chunk *table, int chunks, const double *partial, int parts, float max_norm, float *norm) {
+    __shared__ double red[4];
+    const double n = total_norm(partial, parts, red);
+    if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
+    const double q = (double)max_norm / (n + 1e-6);
+    const float f = q > 1.0 ? 1.f : (float)q;       // a NaN norm makes f NaN
+    for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+        const Chunk k = table[c];
+        if (f == 1.f && k.src == k.dst) continue;   // g * 1 is g
+        C6_BY_TYPE(k.type, T, for (uint32_t i = threadIdx.x; i < k.n; i += 256) ((T *)k.dst)[i] = c6_put<T>(c6_get(((const T *)k.src)[i]) * f));
+    }
+}
+
+int bad(const char *msg) { return c6_set_error(C6_ERR_BAD_ARG, msg); }
+
+}   // namespace
+
+struct c6_clip {
+    int device = 0, chunks = 0, parts = 0;
+    Chunk *table = nullptr;
+};
+
+static int clip_create(int count, const void *const *grads, void *const *outs, const size_t *sizes, const int *types, int device, c6_clip **out) {
+    struct Span { uintptr_t a, b; bool written; };
+    std::vector<Chunk> table;
+    std::vector<Span> spans;
+    for (int i = 0; i < count; i++) {
+        if (!c6_type_ok(types[i])) return bad("c6_clip_create: types must be C6_TYPE_F32, C6_TYPE_F16 or C6_TYPE_BF16");
+        if (!sizes[i]) continue;
+        const size_t es = c6_type_bytes(types[i]);
+        const char *src = (const char *)grads[i];
+        char *dst = outs ? (char *)outs[i] : (char *)grads[i];
+        if (!src || !dst) return bad("c6_clip_create: a tensor is NULL");
+        if (!c6_aligned(src, es) || !c6_aligned(dst, es)) return bad("c6_clip_create: a tensor is not aligned to its type");
+        if (sizes[i] > ((size_t)1 << 46)) return bad("c6_clip_create: a tensor exceeds the address space");
+        const size_t bytes = sizes[i] * es;
+        if (src != dst) spans.push_back(Span{(uintptr_t)src, (uintptr_t)src + bytes, false});
+        spans.push_back(Span{(uintptr_t)dst, (uintptr_t)dst + bytes, true});
+        for (size_t at = 0; at < sizes[i]; at += CHUNK)
+            table.push_back(Chunk{src + at * es, dst + at * es, (uint32_t)std::min<size_t>(CHUNK, sizes[i] - at), (uint32_t)types[i]});
+    }
+    if (table.size() > (size_t)1 << 30) return bad("c6_clip_create: too many elements");
+    // sorted by address: an overlap shows against the furthest end so far, of anything and of what is written
+    std::sort(spans.begin(), spans.end(), [](const Span &p, const Span &q) { return p.a < q.a; });
+    uintptr_t end = 0, written_end = 0;
+    for (const Span &s : spans) {
+        if (s.a < (s.written ? end : written_end)) return bad("c6_clip_create: written memory overlaps other memory of the table");
+        end = std::max(end, s.b);
+        if (s.written) written_end = std::max(written_end, s.b);
+    }
+    if (int rc = c6_check_device(device)) return rc;
+    C6DeviceScope scope(device);
+    if (!scope.ok) return c6_set_error(C6_ERR_HIP, "c6_clip_create: hipSetDevice");
+    c6_clip *c = new c6_clip();
+    c->device = device;
+    c->chunks = (int)table.size();
+    c->parts = std::min(c->chunks, MAXPART);
+    if (c->chunks && (hipMalloc(&c->table, table.size() * sizeof(Chunk)) != hipSuccess ||
+                      hipMemcpy(c->table, table.data(), table.size() * sizeof(Chunk), hipMemcpyHostToDevice) != hipSuccess)) {
+        hipFree(c->table);
+        delete c;
+        return c6_set_error(C6_ERR_HIP, "c6_clip_create: no memory for the table");
+    }
+    *out = c;
+    return C6_OK;
+}
+
+extern "C" int c6_clip_create(int count, const void *const *grads, void *const *outs, const size_t *sizes, const int *types, int device, c6_clip **out) {
+    if (!out) return bad("c6_clip_create: out is NULL");
+    *out = nullptr;
+    if (count < 0 || (count && (!grads || !sizes || !types))) return bad("c6_clip_create: bad argument");
+    try {
+        return clip_create(count, grads, outs, sizes, types, device, out);
+    } catch (...) {      // (the host vectors' only failure)
+        return c6_set_error(C6_ERR_OVERFLOW, "c6_clip_create: out of host memory");
+    }
+}
+
+extern "C" void c6_clip_destroy(c6_clip *c) {
+    if (!c) return;
+    C6DeviceScope scope(c->device);
+    hipFree(c->table);
+    delete c;
+}
+
+extern "C" size_t c6_clip_workspace(const c6_clip *c) { return c ? std::max(c->parts, 1) * sizeof(double) : 0; }
+
+static int check_call(c6_clip *c, const float *norm, bool norm_needed, const void *workspace, size_t workspace_bytes) {
+    if (!c) return bad("c6_clip: NULL handle");
+    if ((norm_needed && !norm) || !c6_aligned(norm, 4)) return bad("c6_clip: norm is NULL or not aligned to 4 bytes");
+    if (!workspace || workspace_bytes < c6_clip_workspace(c) || !c6_aligned(workspace, 8)) return bad("c6_clip: the workspace is NULL, too small or not aligned to 8 bytes");
+    return C6_OK;
+}
+
+static int enqueue(c6_clip *c, bool apply, float max_norm, float *norm, double *partial, hipStream_t s) {
+    C6DeviceScope scope(c->device);
+    if (!scope.ok) return c6_set_error(C6_ERR_HIP, "c6_clip: hipSetDevice");
+    if (c->chunks) hipLaunchKernelGGL(c6_clip_norm_kernel, dim3(c->parts), dim3(256), 0, s, c->table, c->chunks, partial);
+    if (apply)
+        hipLaunchKernelGGL(c6_clip_apply_kernel, dim3(std::max(c->parts, 1)), dim3(256), 0, s, c->table, c->chunks, partial, c->parts, max_norm, norm);
+    else
+        hipLaunchKernelGGL(c6_clip_finish_kernel, dim3(1), dim3(256), 0, s, partial, c->parts, norm);
+    return hipGetLastError() == hipSuccess ? C6_OK : c6_set_error(C6_ERR_HIP, "c6_clip: launch failed");
+}
+
+extern "C" int c6_clip_norm(c6_clip *c, float *norm, void *workspace, size_t workspace_bytes, void *stream) {
+    if (int rc = check_call(c, norm, true, workspace, workspace_bytes)) return rc;
+    return enqueue(c, false, 0.f, norm, (double *)workspace, (hipStream_t)stream);
+}
+
+extern "C" int c6_clip_apply(c6_clip *c, float max_norm, float *norm, void *workspace, size_t workspace_bytes, void *stream) {
+    if (int rc = check_call(c, norm, false, workspace, workspace_bytes)) return rc;
+    if (!(max_norm >= 0.f) || max_norm > 3.402823466e38f) return bad("c6_clip_apply: max_norm must be finite and >= 0");
+    return enqueue(c, true, max_norm, norm, (double *)workspace, (hipStream_t)stream);
+}

@@ -1,0 +1,262 @@
+// policy_ops.hip -- what a policy's logits go through before a move is chosen, and the loss they are trained on
+// (include/connect6_amd.h part 7): penalties / biases / masks, cross entropy over the legal entries, and its gradient.
+#include "c6_ops.h"
+
+#include <algorithm>
+
+namespace {
+
+struct Rows {                     // the device's view of a c6_logits
+    const void *x;
+    const uint8_t *mask;
+    int64_t x_stride, mask_row, mask_byte;
+    int rows, width;
+};
+
+__device__ __forceinline__ bool legal(const Rows &l, int64_t r, int v) {
+    return !l.mask || (l.mask[r * l.mask_row + (int64_t)(v >> 3) * l.mask_byte] >> (v & 7) & 1);
+}
+
+// ---- penalties, biases, masks -------------------------------------------------------------------------------------------
+constexpr int PCHUNK = 8192;      // columns of one workgroup: their counters are 32 KB of LDS
+
+struct Repeats {
+    const int32_t *history, *len;
+    const float *penalties;
+    int64_t history_stride, penalties_stride;
+    int cap;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void c6_logits_process_kernel(Rows l, Repeats h, const float *bias, int64_t bias_stride, T *out, int64_t out_stride) {
+    __shared__ uint32_t count[PCHUNK];
+    const int chunks = (l.width + PCHUNK - 1) / PCHUNK;
+    const int64_t items = (int64_t)l.rows * chunks;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int64_t r = item / chunks;
+        const int v0 = (int)(item % chunks) * PCHUNK, nv = min(PCHUNK, l.width - v0);
+        float rep = 1.f, freq = 0.f, pres = 0.f;
+        if (h.history) {
+            for (int v = threadIdx.x; v < nv; v += 256) count[v] = 0;
+            __syncthreads();
+            int n = h.len ? h.len[r] : h.cap;
+            n = min(n, h.cap);
+            for (int i = threadIdx.x; i < n; i += 256) {
+                const int64_t at = (int64_t)h.history[r * h.history_stride + i] - v0;
+                if (at >= 0 && at < nv) atomicAdd(&count[at], 1u);
+            }
+            __syncthreads();
+            const float *p = h.penalties + r * h.penalties_stride;
+            rep = p[0]; freq = p[1]; pres = p[2];
+        }
+        const T *x = (const T *)l.x + r * l.x_stride;
+        for (int v = threadIdx.x; v < nv; v += 256) {
+            float y = c6_get(x[v0 + v]);
+            if (h.history && count[v]) y = (y > 0.f ? y / rep : y * rep) - (freq * (float)count[v] + pres);
+            if (bias) y += bias[r * bias_stride + v0 + v];
+            out[r * out_stride + v0 + v] = c6_put<T>(legal(l, r, v0 + v) ? y : -INFINITY);
+        }
+        __syncthreads();
+    }
+}
+
+// ---- cross entropy over the legal entries -------------------------------------------------------------------------------
+struct Target {
+    const void *p;
+    int64_t stride;
+    int kind;
+};
+__device__ __forceinline__ int target_index(const Target &t, int64_t r, int width) {      // -1: none
+    if (t.kind == C6_TARGET_WEIGHTS) return -1;
+    const int64_t i = t.kind == C6_TARGET_INDEX64 ? ((const int64_t *)t.p)[r] : ((const int32_t *)t.p)[r];
+    return i >= 0 && i < width ? (int)i : -1;
+}
+__device__ __forceinline__ float target_weight(const Target &t, int64_t r, int v, int index) {
+    return t.kind == C6_TARGET_WEIGHTS ? ((const float *)t.p)[r * t.stride + v] : (v == index ? 1.f : 0.f);
+}
+
+template <typename F>
+__device__ __forceinline__ float block_all(float v, F f, float *red) {
+    v = c6_wave_all(v, f);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return f(f(red[0], red[1]), f(red[2], red[3]));
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void c6_policy_loss_kernel(Rows l, Target t, float *loss, float *lse, float *total, T *grad, int64_t grad_stride, float scale) {
+    __shared__ float red[4];
+    const auto add = [](float a, float b) { return a + b; };
+    for (int64_t r = blockIdx.x; r < l.rows; r += gridDim.x) {
+        const T *x = (const T *)l.x + r * l.x_stride;
+        const int index = target_index(t, r, l.width);
+        float m = -INFINITY;
+        for (int v = threadIdx.x; v < l.width; v += 256)
+            if (legal(l, r, v)) m = fmaxf(m, c6_get(x[v]));
+        m = block_all(m, [](float a, float b) { return fmaxf(a, b); }, red);
+        if (m == -INFINITY) m = 0.f;
+        // NaN is not seen by the maximum but is by the sum; the terms t (m - x) are all >= 0: nothing cancels
+        float s = 0.f, w = 0.f, d = 0.f;
+        for (int v = threadIdx.x; v < l.width; v += 256)
+            if (legal(l, r, v)) {
+                const float y = c6_get(x[v]), q = target_weight(t, r, v, index);
+                s += expf(y - m);
+                w += q;
+                if (q != 0.f) d += q * (m - y);
+            }
+        s = block_all(s, add, red);
+        w = block_all(w, add, red);
+        d = block_all(d, add, red);
+        const bool some = s != 0.f;
+        if (threadIdx.x == 0) {
+            loss[r] = some ? w * logf(s) + d : 0.f;
+            lse[r] = some ? m + logf(s) : -INFINITY;
+            total[r] = some ? w : 0.f;
+        }
+        if (grad) {
+            const float inv = w / s;
+            for (int v = threadIdx.x; v < l.width; v += 256) {
+                float g = 0.f;
+                if (some && legal(l, r, v)) g = scale * (expf(c6_get(x[v]) - m) * inv - target_weight(t, r, v, index));
+                grad[r * grad_stride + v] = c6_put<T>(g);
+            }
+        }
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void c6_policy_loss_grad_kernel(Rows l, Target t, const float *lse, const float *total, const float *dloss, int64_t dloss_stride,
+                                                                  T *grad, int64_t grad_stride) {
+    for (int64_t r = blockIdx.x; r < l.rows; r += gridDim.x) {
+        const T *x = (const T *)l.x + r * l.x_stride;
+        const int index = target_index(t, r, l.width);
+        const float z = lse[r], w = total[r], scale = dloss[r * dloss_stride];
+        for (int v = threadIdx.x; v < l.width; v += 256) {
+            float g = 0.f;
+            if (z != -INFINITY && legal(l, r, v)) g = scale * (w * expf(c6_get(x[v]) - z) - target_weight(t, r, v, index));
+            grad[r * grad_stride + v] = c6_put<T>(g);
+        }
+    }
+}
+
+// ---- host side ----------------------------------------------------------------------------------------------------------
+int bad(const char *msg) { return c6_set_error(C6_ERR_BAD_ARG, msg); }
+
+// the last element a strided matrix touches stays addressable
+bool fits(int64_t rows, int64_t stride, int64_t width, int64_t bytes) {
+    int64_t last;
+    return !__builtin_mul_overflow(rows > 0 ? rows - 1 : 0, stride, &last) && !__builtin_add_overflow(last, width, &last) &&
+           !__builtin_mul_overflow(last, bytes, &last);
+}
+
+int check_logits(const c6_logits *l) {
+    if (!l) return bad("logits: NULL argument");
+    if (l->rows < 0 || l->width < 0) return bad("logits: negative size");
+    if (!c6_type_ok(l->type)) return bad("logits: type must be C6_TYPE_F32, C6_TYPE_F16 or C6_TYPE_BF16");
+    if (l->x_stride < 0 || l->mask_row < 0 || l->mask_byte < 0) return bad("logits: negative stride");
+    const int64_t es = (int64_t)c6_type_bytes(l->type);
+    if (!fits(l->rows, l->x_stride, l->width, es)) return bad("logits: the matrix exceeds the address space");
+    if (l->rows && l->width) {
+        if (!l->x) return bad("logits: x is NULL");
+        if (!c6_aligned(l->x, es)) return bad("logits: x is not aligned to its type");
+    }
+    return C6_OK;
+}
+
+// a written matrix: its rows do not overlap one another, and it is x itself or leaves x alone (rows of both may interleave in one buffer)
+int check_written(const c6_logits *l, const void *out, int64_t stride, const char *null_msg) {
+    const int64_t es = (int64_t)c6_type_bytes(l->type);
+    if (!l->rows || !l->width) return C6_OK;
+    if (!out) return bad(null_msg);
+    if (!c6_aligned(out, es)) return bad("logits: the output is not aligned to its type");
+    if (stride < 0 || (l->rows > 1 && stride < l->width)) return bad("logits: rows of the output overlap");
+    if (!fits(l->rows, stride, l->width, es)) return bad("logits: the output exceeds the address space");
+    if (l->rows > 1 && out == l->x && stride != l->x_stride) return bad("logits: in place needs the same stride");
+    if (out == l->x) return C6_OK;
+    const int64_t a = (int64_t)(uintptr_t)l->x, b = (int64_t)(uintptr_t)out;
+    const int64_t a1 = a + ((l->rows - 1) * l->x_stride + l->width) * es, b1 = b + ((l->rows - 1) * stride + l->width) * es;
+    if (a1 <= b || b1 <= a) return C6_OK;
+    if (l->rows > 1 && stride == l->x_stride) {      // interleaved: row r of the output lies between rows of x
+        int64_t off = (b - a) % (stride * es);
+        if (off < 0) off += stride * es;
+        if (off >= l->width * es && stride * es - off >= l->width * es) return C6_OK;
+    }
+    return bad("logits: the output overlaps x without being x");
+}
+
+int check_target(const c6_logits *l, const void *target, int kind, int64_t stride) {
+    if (kind != C6_TARGET_INDEX32 && kind != C6_TARGET_INDEX64 && kind != C6_TARGET_WEIGHTS) return bad("policy loss: unknown kind of target");
+    if (!l->rows || (kind == C6_TARGET_WEIGHTS && !l->width)) return C6_OK;
+    if (!target) return bad("policy loss: target is NULL");
+    if (!c6_aligned(target, kind == C6_TARGET_INDEX64 ? 8 : 4)) return bad("policy loss: target is not aligned to its type");
+    if (kind == C6_TARGET_WEIGHTS && (stride < 0 || !fits(l->rows, stride, l->width, 4))) return bad("policy loss: bad stride of the weights");
+    return C6_OK;
+}
+
+Rows rows_of(const c6_logits *l) { return Rows{l->x, l->mask, l->x_stride, l->mask_row, l->mask_byte, l->rows, l->width}; }
+
+int launched() { return hipGetLastError() == hipSuccess ? C6_OK : c6_set_error(C6_ERR_HIP, "logits: launch failed"); }
+
+}   // namespace
+
+extern "C" int c6_logits_process(const c6_logits *l, const int32_t *history, int64_t history_stride, const int32_t *history_len, int history_cap,
+                                 const float *penalties, int64_t penalties_stride, const float *bias, int64_t bias_stride, void *out, int64_t out_stride,
+                                 void *stream) {
+    if (int rc = check_logits(l)) return rc;
+    if (int rc = check_written(l, out, out_stride, "c6_logits_process: out is NULL")) return rc;
+    if (history) {
+        if (history_cap < 0 || history_stride < 0 || penalties_stride < 0) return bad("c6_logits_process: negative size or stride of the history");
+        if (!penalties) return bad("c6_logits_process: a history needs penalties");
+        if (!c6_aligned(history, 4) || !c6_aligned(penalties, 4) || !c6_aligned(history_len, 4)) return bad("c6_logits_process: a history, its lengths and penalties are aligned to 4 bytes");
+        if (!fits(l->rows, history_stride, history_cap, 4) || !fits(l->rows, penalties_stride, 3, 4)) return bad("c6_logits_process: the history exceeds the address space");
+    }
+    if (bias && (bias_stride < 0 || !c6_aligned(bias, 4) || !fits(l->rows, bias_stride, l->width, 4))) return bad("c6_logits_process: bad bias");
+    if (int rc = c6_check_device(l->device)) return rc;
+    if (!l->rows || !l->width) return C6_OK;
+    C6DeviceScope scope(l->device);
+    if (!scope.ok) return c6_set_error(C6_ERR_HIP, "c6_logits_process: hipSetDevice");
+    const int64_t items = (int64_t)l->rows * ((l->width + PCHUNK - 1) / PCHUNK);
+    const Repeats h{history, history_len, penalties, history_stride, penalties_stride, history_cap};
+    C6_BY_TYPE(l->type, T, hipLaunchKernelGGL((c6_logits_process_kernel<T>), dim3((unsigned)std::min<int64_t>(items, 1 << 20)), dim3(256), 0, (hipStream_t)stream,
+                                              rows_of(l), h, bias, bias_stride, (T *)out, out_stride));
+    return launched();
+}
+
+extern "C" size_t c6_policy_loss_workspace(int rows, int width) { return 0; }
+
+extern "C" int c6_policy_loss(const c6_logits *l, const void *target, int target_kind, int64_t target_stride, float *loss, float *lse, float *total, void *grad,
+                              int64_t grad_stride, float grad_scale, void *workspace, size_t workspace_bytes, void *stream) {
+    if (int rc = check_logits(l)) return rc;
+    if (int rc = check_target(l, target, target_kind, target_stride)) return rc;
+    if (grad)
+        if (int rc = check_written(l, grad, grad_stride, "")) return rc;
+    if (l->rows && (!loss || !lse || !total)) return bad("c6_policy_loss: loss, lse or total is NULL");
+    if (!c6_aligned(loss, 4) || !c6_aligned(lse, 4) || !c6_aligned(total, 4)) return bad("c6_policy_loss: loss, lse and total are aligned to 4 bytes");
+    if (int rc = c6_check_device(l->device)) return rc;
+    if (!l->rows) return C6_OK;
+    C6DeviceScope scope(l->device);
+    if (!scope.ok) return c6_set_error(C6_ERR_HIP, "c6_policy_loss: hipSetDevice");
+    const Target t{target, target_stride, target_kind};
+    C6_BY_TYPE(l->type, T, hipLaunchKernelGGL((c6_policy_loss_kernel<T>), dim3((unsigned)std::min(l->rows, 1 << 20)), dim3(256), 0, (hipStream_t)stream, rows_of(l), t,
+                                              loss, lse, total, (T *)grad, grad_stride, grad_scale));
+    return launched();
+}
+
+extern "C" int c6_policy_loss_grad(const c6_logits *l, const void *target, int target_kind, int64_t target_stride, const float *lse, const float *total,
+                                   const float *dloss, int64_t dloss_stride, void *grad, int64_t grad_stride, void *stream) {
+    if (int rc = check_logits(l)) return rc;
+    if (int rc = check_target(l, target, target_kind, target_stride)) return rc;
+    if (int rc = check_written(l, grad, grad_stride, "c6_policy_loss_grad: grad is NULL")) return rc;
+    if (l->rows && (!lse || !total || !dloss)) return bad("c6_policy_loss_grad: lse, total or dloss is NULL");
+    if (!c6_aligned(lse, 4) || !c6_aligned(total, 4) || !c6_aligned(dloss, 4)) return bad("c6_policy_loss_grad: lse, total and dloss are aligned to 4 bytes");
+    if (dloss_stride < 0) return bad("c6_policy_loss_grad: negative stride");
+    if (int rc = c6_check_device(l->device)) return rc;
+    if (!l->rows || !l->width) return C6_OK;
+    C6DeviceScope scope(l->device);
+    if (!scope.ok) return c6_set_error(C6_ERR_HIP, "c6_policy_loss_grad: hipSetDevice");
+    const Target t{target, target_stride, target_kind};
+    C6_BY_TYPE(l->type, T, hipLaunchKernelGGL((c6_policy_loss_grad_kernel<T>), dim3((unsigned)std::min(l->rows, 1 << 20)), dim3(256), 0, (hipStream_t)stream, rows_of(l), t,
+                                              lse, total, dloss, dloss_stride, (T *)grad, grad_stride));
+    return launched();
+}

@@ -553,6 +553,73 @@ int c6_group_fetch_pooled(c6_group *g, int member, size_t cap, size_t *count, vo
 /* ... and device to device into a replay buffer living on member r's device (ReplayBuffer::push_game for every record) */
 int c6_group_push_pooled(c6_group *g, int member, c6_replay *r);
 
+/* =====================================================================================================================
+ * Part 7 -- operators on a policy's logits and on gradients.  Everything they read and write is DEVICE memory on `device`, and they run on
+ * the caller's HIP stream (hipStream_t as void*; NULL: the default stream) without allocating, copying or synchronising: they can be
+ * captured into a graph, and the calling thread's current device is left as it was.  A workspace belongs to one call at a time: two calls
+ * (or two captured graphs) that may run at once need one each.
+ * ===================================================================================================================== */
+enum { C6_TYPE_F32 = 0, C6_TYPE_F16 = 1, C6_TYPE_BF16 = 2 };
+
+/* rows of logits, and which of their entries are legal */
+typedef struct c6_logits {
+    int rows, width;         /* >= 0 */
+    int type;                /* C6_TYPE_* of x, and of what is computed for every entry */
+    int device;              /* HIP ordinal */
+    const void *x;           /* entry v of row r: x[r * x_stride + v]; aligned to its type */
+    int64_t x_stride;        /* elements from row to row, >= 0 (0: every row is the same one) */
+    const uint8_t *mask;     /* NULL: every entry is legal; else entry v of row r is legal iff bit (v & 7) of the byte
+                                mask[r * mask_row + (v >> 3) * mask_byte] is set.  (bytes_per_row, 1): a packed row after the other;
+                                (1, boards): the layout that c6_legal_mask writes; mask_row 0: one mask shared by the rows */
+    int64_t mask_row, mask_byte; /* bytes, >= 0 */
+} c6_logits;
+
+/* Penalties for repeated moves (or tokens), biases and masks.  With c = how often v occurs among the first min(history_len[r],
+ * history_cap) ids of row r's history (ids outside [0, width), such as the -1 of "no move", count for nothing) and
+ * (repetition, frequency, presence) = penalties[r * penalties_stride + 0 .. 2], in 32 bits:
+ *     y = x;   if c > 0:  y = (x > 0 ? x / repetition : x * repetition) - (frequency * c + presence);
+ *     y += bias[r * bias_stride + v];      an entry that is not legal: y = -infinity, whatever x is
+ * and out = y rounded once to the type.  history (int32) NULL: no penalties; history_len NULL: every row has history_cap ids; bias NULL:
+ * none.  Strides in elements, >= 0 (0: shared by the rows).  out may be x itself (same pointer and stride) and overlaps nothing else. */
+int c6_logits_process(const c6_logits *l, const int32_t *history, int64_t history_stride, const int32_t *history_len, int history_cap,
+                      const float *penalties, int64_t penalties_stride, const float *bias, int64_t bias_stride, void *out, int64_t out_stride,
+                      void *stream);
+
+/* Cross entropy over the legal entries.  With target weights t >= 0 over the entries (those of illegal entries count for nothing):
+ *     lse = log sum exp(x),   total = sum t,   loss = sum t (lse - x),   gradient = scale * (total * exp(x - lse) - t)
+ * over the legal entries; the gradient of the others is 0.  A row without a legal entry above -infinity: loss = total = 0,
+ * lse = -infinity, gradient 0.  NaN or +infinity at a legal entry makes the row NaN.  Statistics are held in 32 bits. */
+enum {
+    C6_TARGET_INDEX32 = 0,   /* target: int32 [rows], t = 1 at that entry; an index outside [0, width) or at an illegal entry: t = 0 everywhere */
+    C6_TARGET_INDEX64 = 1,   /* ... int64 */
+    C6_TARGET_WEIGHTS = 2    /* target: float, weight v of row r at target[r * target_stride + v]: visit counts, a teacher's distribution */
+};
+/* bytes of workspace that c6_policy_loss needs for so many rows and entries (may be 0) */
+size_t c6_policy_loss_workspace(int rows, int width);
+/* loss, lse, total: float [rows], written.  grad (type of x, stride in elements) may be NULL: no gradient; else the gradient at
+ * scale = grad_scale for every row (1 / rows: the mean's).  grad may be x itself (same pointer and stride) and overlaps nothing else. */
+int c6_policy_loss(const c6_logits *l, const void *target, int target_kind, int64_t target_stride, float *loss, float *lse, float *total, void *grad,
+                   int64_t grad_stride, float grad_scale, void *workspace, size_t workspace_bytes, void *stream);
+/* the gradient alone, from the lse and total that c6_policy_loss left: scale = dloss[r * dloss_stride] (dloss_stride 0: one for all rows) */
+int c6_policy_loss_grad(const c6_logits *l, const void *target, int target_kind, int64_t target_stride, const float *lse, const float *total,
+                        const float *dloss, int64_t dloss_stride, void *grad, int64_t grad_stride, void *stream);
+
+/* Global gradient norm over many tensors, and clipping:
+ *     norm = sqrt(sum of g^2 over every element of every tensor),   out = g * min(1, max_norm / (norm + 1e-6))
+ * The sum is held in 64 bits (no overflow, nothing lost among many elements) in a fixed order: the same gradients give the same bits.
+ * A c6_clip is the device-side table of the tensors' addresses, made once for buffers that stay where they are; it is only read
+ * afterwards. */
+typedef struct c6_clip c6_clip;
+/* grads[i] / outs[i]: sizes[i] contiguous elements of types[i] (C6_TYPE_*), aligned to their type; a size may be 0.  outs NULL, or
+ * outs[i] == grads[i]: in place.  Written memory may not overlap other memory of the table.  count 0: norm 0. */
+int c6_clip_create(int count, const void *const *grads, void *const *outs, const size_t *sizes, const int *types, int device, c6_clip **out);
+void c6_clip_destroy(c6_clip *c);      /* no call on it may still be running */
+size_t c6_clip_workspace(const c6_clip *c);
+/* *norm (device float, written; may be NULL in c6_clip_apply): the norm of the gradients as they come in */
+int c6_clip_norm(c6_clip *c, float *norm, void *workspace, size_t workspace_bytes, void *stream);
+/* max_norm: finite, >= 0.  A norm that is NaN makes every output NaN.  In place and nothing to clip: nothing is written. */
+int c6_clip_apply(c6_clip *c, float max_norm, float *norm, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
