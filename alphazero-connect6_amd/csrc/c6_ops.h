@@ -15,6 +15,58 @@ __device__ __forceinline__ float c6_get(T v) { return (float)v; }
 template <typename T>
 __device__ __forceinline__ T c6_put(float v) { return (T)v; }
 
+// 16 bytes at a time: N elements at an address aligned to ONE element (the memory pipeline takes such addresses; a wave's 1024 bytes then touch nine
+// lines of 128 bytes instead of eight), in registers as they lie in memory
+typedef uint32_t c6_u32x4 __attribute__((ext_vector_type(4)));
+template <typename T>
+struct C6Vec {
+    static constexpr int N = 16 / sizeof(T);
+    struct __attribute__((packed, aligned(sizeof(T)))) Raw { c6_u32x4 u; };
+    static __device__ __forceinline__ c6_u32x4 load(const T *p) { return reinterpret_cast<const Raw *>(p)->u; }
+    static __device__ __forceinline__ void store(T *p, c6_u32x4 u) { reinterpret_cast<Raw *>(p)->u = u; }
+    static __device__ __forceinline__ void get(c6_u32x4 u, float (&f)[N]) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t w = u[i];      // (a bit cast of the vector's element itself takes element 0)
+            if constexpr (sizeof(T) == 4) {
+                f[i] = __builtin_bit_cast(float, w);
+            } else if constexpr (__is_same(T, __bf16)) {
+                f[2 * i] = __builtin_bit_cast(float, w << 16);
+                f[2 * i + 1] = __builtin_bit_cast(float, w & 0xffff0000u);
+            } else {
+                typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+                const h2 h = __builtin_bit_cast(h2, w);
+                f[2 * i] = (float)h[0];
+                f[2 * i + 1] = (float)h[1];
+            }
+        }
+    }
+    static __device__ __forceinline__ c6_u32x4 put(const float (&f)[N]) {
+        c6_u32x4 u;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if constexpr (sizeof(T) == 4) {
+                u[i] = __builtin_bit_cast(uint32_t, f[i]);
+            } else {
+                typedef T t2 __attribute__((ext_vector_type(2)));
+                typedef float f2 __attribute__((ext_vector_type(2)));
+                u[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{f[2 * i], f[2 * i + 1]}), t2));
+            }
+        }
+        return u;
+    }
+    // the first n of N elements (the end of a row); the rest reads as `fill`
+    static __device__ __forceinline__ void get_some(const T *p, int n, float fill, float (&f)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; i++) f[i] = i < n ? c6_get(p[i]) : fill;
+    }
+    static __device__ __forceinline__ void put_some(T *p, int n, const float (&f)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (i < n) p[i] = c6_put<T>(f[i]);
+    }
+};
+
 template <typename V, typename F>
 __device__ __forceinline__ V c6_wave_all(V v, F f) {
 #pragma unroll

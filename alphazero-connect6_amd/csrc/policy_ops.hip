@@ -17,46 +17,102 @@ __device__ __forceinline__ bool legal(const Rows &l, int64_t r, int v) {
     return !l.mask || (l.mask[r * l.mask_row + (int64_t)(v >> 3) * l.mask_byte] >> (v & 7) & 1);
 }
 
-// ---- penalties, biases, masks -------------------------------------------------------------------------------------------
-constexpr int PCHUNK = 8192;      // columns of one workgroup: their counters are 32 KB of LDS
+// the legal bits of the N entries from column c (a multiple of N) on
+template <int N>
+__device__ __forceinline__ uint32_t legal_bits(const Rows &l, const uint8_t *mask_row, int c) {
+    return (uint32_t)mask_row[(int64_t)(c >> 3) * l.mask_byte] >> (N == 4 ? c & 4 : 0);
+}
 
+// ---- penalties, biases, masks -------------------------------------------------------------------------------------------
+// A row is cut into chunks; LANES threads take one chunk: a wave for rows of up to 1024 entries (four rows a workgroup), else a workgroup per 8192.
+// The chunk's logits are requested first, 16 bytes a lane and all in flight, and wait in registers while the row's history is counted in LDS:
+// each chunk reads the whole history and counts the ids that fall into it (integer adds: the order does not matter).
 struct Repeats {
     const int32_t *history, *len;
     const float *penalties;
     int64_t history_stride, penalties_stride;
     int cap;
 };
+constexpr int PROCESS_WAVE = 1024, PROCESS_BLOCK = 8192;
 
-template <typename T>
+template <typename T, int LANES, bool HIST>
 __global__ __launch_bounds__(256) void c6_logits_process_kernel(Rows l, Repeats h, const float *bias, int64_t bias_stride, T *out, int64_t out_stride) {
-    __shared__ uint32_t count[PCHUNK];
-    const int chunks = (l.width + PCHUNK - 1) / PCHUNK;
+    typedef C6Vec<T> V;
+    constexpr int CHUNK = LANES == 64 ? PROCESS_WAVE : PROCESS_BLOCK, U = CHUNK / (LANES * V::N), PER = 256 / LANES;
+    __shared__ uint32_t counters[HIST ? PER * CHUNK : 1];
+    const int lane = threadIdx.x % LANES, part = threadIdx.x / LANES;
+    uint32_t *count = counters + (HIST ? part * CHUNK : 0);
+    const auto meet = [] {      // one wave's LDS operations are performed in order: only the compiler has to keep them so
+        if (LANES == 64) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        else __syncthreads();
+    };
+    const int chunks = (l.width + CHUNK - 1) / CHUNK;
     const int64_t items = (int64_t)l.rows * chunks;
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    for (int64_t item = (int64_t)blockIdx.x * PER + part; item < items; item += (int64_t)gridDim.x * PER) {
         const int64_t r = item / chunks;
-        const int v0 = (int)(item % chunks) * PCHUNK, nv = min(PCHUNK, l.width - v0);
+        const int v0 = (int)(item % chunks) * CHUNK, nv = min(CHUNK, l.width - v0);
+        const T *x = (const T *)l.x + r * l.x_stride + v0;
+        T *o = out + r * out_stride + v0;
+        const uint8_t *mask = l.mask ? l.mask + r * l.mask_row : nullptr;
+        c6_u32x4 raw[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int c = (u * LANES + lane) * V::N;
+            if (c + V::N <= nv) raw[u] = V::load(x + c);
+        }
         float rep = 1.f, freq = 0.f, pres = 0.f;
-        if (h.history) {
-            for (int v = threadIdx.x; v < nv; v += 256) count[v] = 0;
-            __syncthreads();
-            int n = h.len ? h.len[r] : h.cap;
-            n = min(n, h.cap);
-            for (int i = threadIdx.x; i < n; i += 256) {
-                const int64_t at = (int64_t)h.history[r * h.history_stride + i] - v0;
-                if (at >= 0 && at < nv) atomicAdd(&count[at], 1u);
+        if (HIST) {
+            for (int c = lane * 4; c < nv; c += LANES * 4) *reinterpret_cast<uint4 *>(count + c) = uint4{0, 0, 0, 0};
+            meet();
+            const int32_t *ids = h.history + r * h.history_stride;
+            const int n = min(h.len ? h.len[r] : h.cap, h.cap);
+            for (int i = lane; i < n; i += LANES) {
+                const uint32_t at = (uint32_t)ids[i] - (uint32_t)v0;      // (an id below v0, or below 0, wraps to far beyond nv)
+                if (at < (uint32_t)nv) atomicAdd(&count[at], 1u);
             }
-            __syncthreads();
             const float *p = h.penalties + r * h.penalties_stride;
             rep = p[0]; freq = p[1]; pres = p[2];
+            meet();
         }
-        const T *x = (const T *)l.x + r * l.x_stride;
-        for (int v = threadIdx.x; v < nv; v += 256) {
-            float y = c6_get(x[v0 + v]);
-            if (h.history && count[v]) y = (y > 0.f ? y / rep : y * rep) - (freq * (float)count[v] + pres);
-            if (bias) y += bias[r * bias_stride + v0 + v];
-            out[r * out_stride + v0 + v] = c6_put<T>(legal(l, r, v0 + v) ? y : -INFINITY);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int c = (u * LANES + lane) * V::N;
+            if (c >= nv) continue;
+            const bool whole = c + V::N <= nv;
+            float y[V::N];
+            if (whole) V::get(raw[u], y);
+            else V::get_some(x + c, nv - c, 0.f, y);
+            if (HIST) {
+                uint32_t k[V::N];
+#pragma unroll
+                for (int i = 0; i < V::N; i += 4) *reinterpret_cast<uint4 *>(k + i) = *reinterpret_cast<const uint4 *>(count + c + i);
+#pragma unroll
+                for (int i = 0; i < V::N; i++)
+                    if (k[i]) y[i] = (y[i] > 0.f ? y[i] / rep : y[i] * rep) - (freq * (float)k[i] + pres);
+            }
+            if (bias) {
+                const float *b = bias + r * bias_stride + v0 + c;
+                float f[V::N];
+#pragma unroll
+                for (int i = 0; i < V::N; i += 4) {
+                    float q[4];
+                    if (whole) C6Vec<float>::get(C6Vec<float>::load(b + i), q);
+                    else C6Vec<float>::get_some(b + i, nv - c - i, 0.f, q);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) f[i + j] = q[j];
+                }
+#pragma unroll
+                for (int i = 0; i < V::N; i++) y[i] += f[i];
+            }
+            if (mask) {
+                const uint32_t ok = legal_bits<V::N>(l, mask, v0 + c);
+#pragma unroll
+                for (int i = 0; i < V::N; i++) y[i] = ok >> i & 1 ? y[i] : -INFINITY;
+            }
+            if (whole) V::store(o + c, V::put(y));
+            else V::put_some(o + c, nv - c, y);
         }
-        __syncthreads();
+        if (HIST) meet();      // the counters are read before the next item clears them
     }
 }
 
@@ -73,6 +129,24 @@ __device__ __forceinline__ int target_index(const Target &t, int64_t r, int widt
 }
 __device__ __forceinline__ float target_weight(const Target &t, int64_t r, int v, int index) {
     return t.kind == C6_TARGET_WEIGHTS ? ((const float *)t.p)[r * t.stride + v] : (v == index ? 1.f : 0.f);
+}
+
+// target weights of the N entries from column c on, of nv columns; `index`: the column of an index target
+template <int N, bool WEIGHTS>
+__device__ __forceinline__ void get_weights(const float *weights, int c, int nv, int index, float (&q)[N]) {
+    if (!WEIGHTS) {
+#pragma unroll
+        for (int i = 0; i < N; i++) q[i] = c + i == index ? 1.f : 0.f;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        float f[4];
+        if (c + N <= nv) C6Vec<float>::get(C6Vec<float>::load(weights + c + i), f);
+        else C6Vec<float>::get_some(weights + c + i, nv - c - i, 0.f, f);
+#pragma unroll
+        for (int j = 0; j < 4; j++) q[i + j] = f[j];
+    }
 }
 
 template <typename F>
@@ -125,17 +199,48 @@ __global__ __launch_bounds__(256) void c6_policy_loss_kernel(Rows l, Target t, f
     }
 }
 
-template <typename T>
+// The gradient from what the forward pass saved: elementwise, in chunks like those of c6_logits_process_kernel.
+constexpr int GRAD_WAVE = 1024, GRAD_BLOCK = 4096;
+
+template <typename T, int LANES, bool WEIGHTS>
 __global__ __launch_bounds__(256) void c6_policy_loss_grad_kernel(Rows l, Target t, const float *lse, const float *total, const float *dloss, int64_t dloss_stride,
                                                                   T *grad, int64_t grad_stride) {
-    for (int64_t r = blockIdx.x; r < l.rows; r += gridDim.x) {
-        const T *x = (const T *)l.x + r * l.x_stride;
-        const int index = target_index(t, r, l.width);
-        const float z = lse[r], w = total[r], scale = dloss[r * dloss_stride];
-        for (int v = threadIdx.x; v < l.width; v += 256) {
-            float g = 0.f;
-            if (z != -INFINITY && legal(l, r, v)) g = scale * (w * expf(c6_get(x[v]) - z) - target_weight(t, r, v, index));
-            grad[r * grad_stride + v] = c6_put<T>(g);
+    typedef C6Vec<T> V;
+    constexpr int CHUNK = LANES == 64 ? GRAD_WAVE : GRAD_BLOCK, U = CHUNK / (LANES * V::N), PER = 256 / LANES;
+    const int lane = threadIdx.x % LANES, part = threadIdx.x / LANES;
+    const int chunks = (l.width + CHUNK - 1) / CHUNK;
+    const int64_t items = (int64_t)l.rows * chunks;
+    for (int64_t item = (int64_t)blockIdx.x * PER + part; item < items; item += (int64_t)gridDim.x * PER) {
+        const int64_t r = item / chunks;
+        const int v0 = (int)(item % chunks) * CHUNK, nv = min(CHUNK, l.width - v0);
+        const T *x = (const T *)l.x + r * l.x_stride + v0;
+        T *g = grad + r * grad_stride + v0;
+        const float *weights = WEIGHTS ? (const float *)t.p + r * t.stride + v0 : nullptr;
+        const uint8_t *mask = l.mask ? l.mask + r * l.mask_row : nullptr;
+        c6_u32x4 raw[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int c = (u * LANES + lane) * V::N;
+            if (c + V::N <= nv) raw[u] = V::load(x + c);
+        }
+        const int index = target_index(t, r, l.width) - v0;      // of this chunk; elsewhere or none: outside it
+        const float z = lse[r], scale = dloss[r * dloss_stride], w = total[r];
+        const bool some = z != -INFINITY;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int c = (u * LANES + lane) * V::N;
+            if (c >= nv) continue;
+            const bool whole = c + V::N <= nv;
+            float y[V::N], q[V::N];
+            if (whole) V::get(raw[u], y);
+            else V::get_some(x + c, nv - c, 0.f, y);
+            get_weights<V::N, WEIGHTS>(weights, c, nv, index, q);
+            uint32_t ok = some ? ~0u : 0u;
+            if (mask) ok &= legal_bits<V::N>(l, mask, v0 + c);
+#pragma unroll
+            for (int i = 0; i < V::N; i++) y[i] = ok >> i & 1 ? scale * (w * expf(y[i] - z) - q[i]) : 0.f;
+            if (whole) V::store(g + c, V::put(y));
+            else V::put_some(g + c, nv - c, y);
         }
     }
 }
@@ -194,6 +299,12 @@ int check_target(const c6_logits *l, const void *target, int kind, int64_t strid
     return C6_OK;
 }
 
+// workgroups for all chunks of all rows, `per` chunks a workgroup (what exceeds the grid's limit is looped over)
+unsigned grid_of(const c6_logits *l, int chunk, int per) {
+    const int64_t items = (int64_t)l->rows * ((l->width + chunk - 1) / chunk);
+    return (unsigned)std::min<int64_t>((items + per - 1) / per, 1 << 22);
+}
+
 Rows rows_of(const c6_logits *l) { return Rows{l->x, l->mask, l->x_stride, l->mask_row, l->mask_byte, l->rows, l->width}; }
 
 int launched() { return hipGetLastError() == hipSuccess ? C6_OK : c6_set_error(C6_ERR_HIP, "logits: launch failed"); }
@@ -216,10 +327,17 @@ extern "C" int c6_logits_process(const c6_logits *l, const int32_t *history, int
     if (!l->rows || !l->width) return C6_OK;
     C6DeviceScope scope(l->device);
     if (!scope.ok) return c6_set_error(C6_ERR_HIP, "c6_logits_process: hipSetDevice");
-    const int64_t items = (int64_t)l->rows * ((l->width + PCHUNK - 1) / PCHUNK);
     const Repeats h{history, history_len, penalties, history_stride, penalties_stride, history_cap};
-    C6_BY_TYPE(l->type, T, hipLaunchKernelGGL((c6_logits_process_kernel<T>), dim3((unsigned)std::min<int64_t>(items, 1 << 20)), dim3(256), 0, (hipStream_t)stream,
-                                              rows_of(l), h, bias, bias_stride, (T *)out, out_stride));
+    const bool wave = l->width <= PROCESS_WAVE;
+    const unsigned grid = grid_of(l, wave ? PROCESS_WAVE : PROCESS_BLOCK, wave ? 4 : 1);
+#define C6_LAUNCH(LANES, HIST)                                                                                                                        \
+    C6_BY_TYPE(l->type, T, hipLaunchKernelGGL((c6_logits_process_kernel<T, LANES, HIST>), dim3(grid), dim3(256), 0, (hipStream_t)stream, rows_of(l), \
+                                              h, bias, bias_stride, (T *)out, out_stride))
+    if (wave && history) C6_LAUNCH(64, true);
+    else if (wave) C6_LAUNCH(64, false);
+    else if (history) C6_LAUNCH(256, true);
+    else C6_LAUNCH(256, false);
+#undef C6_LAUNCH
     return launched();
 }
 
@@ -256,7 +374,16 @@ extern "C" int c6_policy_loss_grad(const c6_logits *l, const void *target, int t
     C6DeviceScope scope(l->device);
     if (!scope.ok) return c6_set_error(C6_ERR_HIP, "c6_policy_loss_grad: hipSetDevice");
     const Target t{target, target_stride, target_kind};
-    C6_BY_TYPE(l->type, T, hipLaunchKernelGGL((c6_policy_loss_grad_kernel<T>), dim3((unsigned)std::min(l->rows, 1 << 20)), dim3(256), 0, (hipStream_t)stream, rows_of(l), t,
-                                              lse, total, dloss, dloss_stride, (T *)grad, grad_stride));
+    const bool wave = l->width <= GRAD_WAVE;
+    const unsigned grid = grid_of(l, wave ? GRAD_WAVE : GRAD_BLOCK, wave ? 4 : 1);
+#define C6_LAUNCH(LANES, WEIGHTS)                                                                                                                          \
+    C6_BY_TYPE(l->type, T, hipLaunchKernelGGL((c6_policy_loss_grad_kernel<T, LANES, WEIGHTS>), dim3(grid), dim3(256), 0, (hipStream_t)stream, rows_of(l), t, \
+                                              lse, total, dloss, dloss_stride, (T *)grad, grad_stride))
+    const bool weights = target_kind == C6_TARGET_WEIGHTS;
+    if (wave && weights) C6_LAUNCH(64, true);
+    else if (wave) C6_LAUNCH(64, false);
+    else if (weights) C6_LAUNCH(256, true);
+    else C6_LAUNCH(256, false);
+#undef C6_LAUNCH
     return launched();
 }
