@@ -33,9 +33,9 @@ struct Repeats {
     int64_t history_stride, penalties_stride;
     int cap;
 };
-constexpr int PROCESS_WAVE = 1024, PROCESS_BLOCK = 8192;
+constexpr int PROCESS_WAVE = 1024, PROCESS_BLOCK = 4096;
 
-template <typename T, int LANES, bool HIST>
+template <typename T, int LANES, bool HIST, bool BIAS>
 __global__ __launch_bounds__(256) void c6_logits_process_kernel(Rows l, Repeats h, const float *bias, int64_t bias_stride, T *out, int64_t out_stride) {
     typedef C6Vec<T> V;
     constexpr int CHUNK = LANES == 64 ? PROCESS_WAVE : PROCESS_BLOCK, U = CHUNK / (LANES * V::N), PER = 256 / LANES;
@@ -54,24 +54,50 @@ __global__ __launch_bounds__(256) void c6_logits_process_kernel(Rows l, Repeats 
         const T *x = (const T *)l.x + r * l.x_stride + v0;
         T *o = out + r * out_stride + v0;
         const uint8_t *mask = l.mask ? l.mask + r * l.mask_row : nullptr;
-        c6_u32x4 raw[U];
+        const float *b = BIAS ? bias + r * bias_stride + v0 : nullptr;
+        c6_u32x4 raw[U], add[BIAS ? U : 1][V::N / 4];
+        uint32_t ok[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int c = (u * LANES + lane) * V::N;
+            ok[u] = ~0u;
             if (c + V::N <= nv) raw[u] = V::load(x + c);
+            if (mask && c < nv) ok[u] = legal_bits<V::N>(l, mask, v0 + c);
+            if constexpr (BIAS)
+                if (c + V::N <= nv)
+#pragma unroll
+                    for (int i = 0; i < V::N / 4; i++) add[u][i] = C6Vec<float>::load(b + c + 4 * i);
         }
         float rep = 1.f, freq = 0.f, pres = 0.f;
         if (HIST) {
+            const float *p = h.penalties + r * h.penalties_stride;
+            rep = p[0]; freq = p[1]; pres = p[2];
             for (int c = lane * 4; c < nv; c += LANES * 4) *reinterpret_cast<uint4 *>(count + c) = uint4{0, 0, 0, 0};
             meet();
             const int32_t *ids = h.history + r * h.history_stride;
             const int n = min(h.len ? h.len[r] : h.cap, h.cap);
-            for (int i = lane; i < n; i += LANES) {
-                const uint32_t at = (uint32_t)ids[i] - (uint32_t)v0;      // (an id below v0, or below 0, wraps to far beyond nv)
+            const auto seen = [&](int32_t id) {
+                const uint32_t at = (uint32_t)id - (uint32_t)v0;      // (an id below v0, or below 0, wraps to far beyond nv)
                 if (at < (uint32_t)nv) atomicAdd(&count[at], 1u);
+            };
+            constexpr int FLIGHT = 4;      // 16 ids of a lane in flight: the loop is bound by the latency of its loads
+            int i = lane * 4;
+            for (; i + 4 + (FLIGHT - 1) * LANES * 4 <= n; i += FLIGHT * LANES * 4) {
+                c6_u32x4 q[FLIGHT];
+#pragma unroll
+                for (int k = 0; k < FLIGHT; k++) q[k] = C6Vec<float>::load((const float *)ids + i + k * LANES * 4);
+#pragma unroll
+                for (int k = 0; k < FLIGHT; k++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) seen((int32_t)q[k][j]);
             }
-            const float *p = h.penalties + r * h.penalties_stride;
-            rep = p[0]; freq = p[1]; pres = p[2];
+            for (; i < n; i += LANES * 4) {
+                int32_t q[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) q[j] = i + j < n ? ids[i + j] : -1;
+#pragma unroll
+                for (int j = 0; j < 4; j++) seen(q[j]);
+            }
             meet();
         }
 #pragma unroll
@@ -86,29 +112,26 @@ __global__ __launch_bounds__(256) void c6_logits_process_kernel(Rows l, Repeats 
                 uint32_t k[V::N];
 #pragma unroll
                 for (int i = 0; i < V::N; i += 4) *reinterpret_cast<uint4 *>(k + i) = *reinterpret_cast<const uint4 *>(count + c + i);
+                uint32_t any = 0;
 #pragma unroll
-                for (int i = 0; i < V::N; i++)
-                    if (k[i]) y[i] = (y[i] > 0.f ? y[i] / rep : y[i] * rep) - (freq * (float)k[i] + pres);
+                for (int i = 0; i < V::N; i++) any |= k[i];
+                if (any)
+#pragma unroll
+                    for (int i = 0; i < V::N; i++)
+                        if (k[i]) y[i] = (y[i] > 0.f ? y[i] / rep : y[i] * rep) - (freq * (float)k[i] + pres);
             }
-            if (bias) {
-                const float *b = bias + r * bias_stride + v0 + c;
-                float f[V::N];
+            if constexpr (BIAS) {
 #pragma unroll
                 for (int i = 0; i < V::N; i += 4) {
                     float q[4];
-                    if (whole) C6Vec<float>::get(C6Vec<float>::load(b + i), q);
-                    else C6Vec<float>::get_some(b + i, nv - c - i, 0.f, q);
+                    if (whole) C6Vec<float>::get(add[u][i / 4], q);
+                    else C6Vec<float>::get_some(b + c + i, nv - c - i, 0.f, q);
 #pragma unroll
-                    for (int j = 0; j < 4; j++) f[i + j] = q[j];
+                    for (int j = 0; j < 4; j++) y[i + j] += q[j];
                 }
-#pragma unroll
-                for (int i = 0; i < V::N; i++) y[i] += f[i];
             }
-            if (mask) {
-                const uint32_t ok = legal_bits<V::N>(l, mask, v0 + c);
 #pragma unroll
-                for (int i = 0; i < V::N; i++) y[i] = ok >> i & 1 ? y[i] : -INFINITY;
-            }
+            for (int i = 0; i < V::N; i++) y[i] = ok[u] >> i & 1 ? y[i] : -INFINITY;
             if (whole) V::store(o + c, V::put(y));
             else V::put_some(o + c, nv - c, y);
         }
@@ -330,13 +353,17 @@ extern "C" int c6_logits_process(const c6_logits *l, const int32_t *history, int
     const Repeats h{history, history_len, penalties, history_stride, penalties_stride, history_cap};
     const bool wave = l->width <= PROCESS_WAVE;
     const unsigned grid = grid_of(l, wave ? PROCESS_WAVE : PROCESS_BLOCK, wave ? 4 : 1);
-#define C6_LAUNCH(LANES, HIST)                                                                                                                        \
-    C6_BY_TYPE(l->type, T, hipLaunchKernelGGL((c6_logits_process_kernel<T, LANES, HIST>), dim3(grid), dim3(256), 0, (hipStream_t)stream, rows_of(l), \
+#define C6_LAUNCH(LANES, HIST, BIAS)                                                                                                                        \
+    C6_BY_TYPE(l->type, T, hipLaunchKernelGGL((c6_logits_process_kernel<T, LANES, HIST, BIAS>), dim3(grid), dim3(256), 0, (hipStream_t)stream, rows_of(l), \
                                               h, bias, bias_stride, (T *)out, out_stride))
-    if (wave && history) C6_LAUNCH(64, true);
-    else if (wave) C6_LAUNCH(64, false);
-    else if (history) C6_LAUNCH(256, true);
-    else C6_LAUNCH(256, false);
+#define C6_LAUNCH_LANES(LANES)                         \
+    if (history && bias) C6_LAUNCH(LANES, true, true); \
+    else if (history) C6_LAUNCH(LANES, true, false);   \
+    else if (bias) C6_LAUNCH(LANES, false, true);      \
+    else C6_LAUNCH(LANES, false, false)
+    if (wave) { C6_LAUNCH_LANES(64); }
+    else { C6_LAUNCH_LANES(256); }
+#undef C6_LAUNCH_LANES
 #undef C6_LAUNCH
     return launched();
 }
