@@ -60,6 +60,11 @@ struct C6Vec {
 #pragma unroll
         for (int i = 0; i < N; i++) f[i] = i < n ? c6_get(p[i]) : fill;
     }
+    static __device__ __forceinline__ c6_u32x4 load_some(const T *p, int n, float fill) {
+        float f[N];
+        get_some(p, n, fill, f);
+        return put(f);
+    }
     static __device__ __forceinline__ void put_some(T *p, int n, const float (&f)[N]) {
 #pragma unroll
         for (int i = 0; i < N; i++)
@@ -67,10 +72,29 @@ struct C6Vec {
     }
 };
 
-template <typename V, typename F>
-__device__ __forceinline__ V c6_wave_all(V v, F f) {
+// f over each row of 16 lanes, by DPP: xor 1, xor 2, mirror 8, mirror 16
+template <typename F>
+__device__ __forceinline__ float c6_row_all(float v, F f) {
+#define C6_DPP(ctrl) v = f(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, 0xf, 0xf, true)))
+    C6_DPP(0xb1);
+    C6_DPP(0x4e);
+    C6_DPP(0x141);
+    C6_DPP(0x140);
+#undef C6_DPP
+    return v;
+}
+// ... and over all 64, the four rows through scalar registers: the same in every lane
+template <typename F>
+__device__ __forceinline__ float c6_wave_all(float v, F f) {
+    const int bits = __builtin_bit_cast(int, c6_row_all(v, f));
+    const auto row = [&](int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(bits, lane)); };
+    return f(f(row(0), row(16)), f(row(32), row(48)));
+}
+__device__ __forceinline__ float c6_wave_sum(float v) { return c6_wave_all(v, [](float a, float b) { return a + b; }); }
+__device__ __forceinline__ float c6_wave_max(float v) { return c6_wave_all(v, [](float a, float b) { return fmaxf(a, b); }); }
+__device__ __forceinline__ double c6_wave_sum(double v) {
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v = f(v, __shfl_xor(v, off, 64));
+    for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
     return v;
 }
 

@@ -15,7 +15,7 @@ constexpr uint32_t CHUNK = 32768;         // elements
 constexpr int MAXPART = 2048;             // partial sums: workgroups of the norm's pass
 
 __device__ double block_sum(double v, double *red) {
-    v = c6_wave_all(v, [](double a, double b) { return a + b; });
+    v = c6_wave_sum(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();

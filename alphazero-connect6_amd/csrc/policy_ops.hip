@@ -172,53 +172,327 @@ __device__ __forceinline__ void get_weights(const float *weights, int c, int nv,
     }
 }
 
-template <typename F>
-__device__ __forceinline__ float block_all(float v, F f, float *red) {
-    v = c6_wave_all(v, f);
+// What is known of some legal entries of a row: their maximum m, s = sum exp(x - m), w = sum t, d = sum t (m - x).  All terms of s, w and d are
+// >= 0: nothing cancels, whatever the size of the logits.  Nothing above -infinity: m = -infinity, s = 0.  The maximum does not see NaN, s does.
+struct alignas(16) Part {
+    float m, s, w, d;
+};
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+// exp(a) as 2^(a log2 e): half steps of |a| in the argument and of the result, where expf costs three times as many instructions
+__device__ __forceinline__ float exp_of(float a) { return __builtin_amdgcn_exp2f(a * LOG2E); }
+__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
+
+// p seen from a maximum M >= p.m
+__device__ __forceinline__ Part from(const Part &p, float M) {
+    Part q;
+    q.m = M;
+    q.s = p.s * exp_of(p.m - base_of(M));
+    q.w = p.w;
+    q.d = p.d + (p.w != 0.f && p.m != -INFINITY ? p.w * (M - p.m) : 0.f);      // (m = -infinity and w > 0: d is infinite already)
+    return q;
+}
+__device__ __forceinline__ Part wave_part(const Part &p, bool weights) {
+    Part q = from(p, c6_wave_max(p.m));
+    q.s = c6_wave_sum(q.s);
+    if (weights) {
+        q.w = c6_wave_sum(q.w);
+        q.d = c6_wave_sum(q.d);
+    }
+    return q;
+}
+// over the waves of a workgroup, the same in every thread; `space`: one Part a wave, not in use by an earlier call that some wave may still read
+template <int LANES>
+__device__ __forceinline__ Part block_part(const Part &p, bool weights, Part *space) {
+    Part q = wave_part(p, weights);
+    if (LANES == 64) return q;
+    if ((threadIdx.x & 63) == 0) space[threadIdx.x >> 6] = q;
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return f(f(red[0], red[1]), f(red[2], red[3]));
+    // every row of 16 lanes takes all the waves' Parts, one a lane
+    const int i = threadIdx.x & 15;
+    static_assert(LANES / 64 <= 16, "one lane of a row for each wave");
+    q = i < LANES / 64 ? space[i] : Part{-INFINITY, 0.f, 0.f, 0.f};
+    const auto add = [](float a, float b) { return a + b; };
+    q = from(q, c6_row_all(q.m, [](float a, float b) { return fmaxf(a, b); }));
+    q.s = c6_row_all(q.s, add);
+    if (weights) {
+        q.w = c6_row_all(q.w, add);
+        q.d = c6_row_all(q.d, add);
+    }
+    return q;
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void c6_policy_loss_kernel(Rows l, Target t, float *loss, float *lse, float *total, T *grad, int64_t grad_stride, float scale) {
-    __shared__ float red[4];
-    const auto add = [](float a, float b) { return a + b; };
-    for (int64_t r = blockIdx.x; r < l.rows; r += gridDim.x) {
+// A row (or a chunk of one) in the registers of LANES lanes, in pieces of N entries (16 bytes): lane i holds the pieces i, i + LANES, ...; the entries behind
+// the last whole piece are one more piece of the last lane.  What is not there, or not legal, is -infinity.
+template <typename T, int LANES, int NV>
+struct Held {
+    typedef C6Vec<T> V;
+    c6_u32x4 raw[NV], tail;
+    int whole, rest;       // whole pieces, entries behind them
+
+    __device__ __forceinline__ Held(int width) : whole(width / V::N), rest(width % V::N) {
+        float f[V::N];
+#pragma unroll
+        for (int i = 0; i < V::N; i++) f[i] = -INFINITY;
+        tail = V::put(f);
+#pragma unroll
+        for (int u = 0; u < NV; u++) raw[u] = tail;
+    }
+    __device__ __forceinline__ bool has(int u, int lane) const { return lane < whole - u * LANES; }
+    __device__ __forceinline__ bool has_tail(int lane) const { return rest && lane == LANES - 1; }
+    __device__ __forceinline__ void request(int u, const T *x, int lane) {
+        if (has(u, lane)) raw[u] = V::load(x + u * LANES * V::N + lane * V::N);
+    }
+    __device__ __forceinline__ void request_tail(const T *x, int lane) {
+        if (has_tail(lane)) {
+            float f[V::N];
+            V::get_some(x + whole * V::N, rest, -INFINITY, f);
+            tail = V::put(f);
+        }
+    }
+    __device__ __forceinline__ void request(const T *x, int lane) {
+#pragma unroll
+        for (int u = 0; u < NV; u++) request(u, x, lane);
+        request_tail(x, lane);
+    }
+};
+// what was unpacked from u before is not kept for later: unpacking again is cheaper than two or four registers a word
+__device__ __forceinline__ void unpack_again(c6_u32x4 &u) { asm volatile("" : "+v"(u)); }
+
+// weights and mask of the row (or chunk), whose first column is a multiple of 8
+struct Beside {
+    const float *weights;
+    const uint8_t *mask;
+    int64_t byte;
+    template <int N>
+    __device__ __forceinline__ uint32_t bits(int c) const { return mask ? (uint32_t)mask[(int64_t)(c >> 3) * byte] >> (N == 4 ? c & 4 : 0) : ~0u; }
+    // weights of n entries from column c on, 0 where illegal
+    template <int N>
+    __device__ __forceinline__ void get(int c, int n, float (&q)[N]) const {
+        const uint32_t ok = bits<N>(c);
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            float f[4];
+            if (n >= N) C6Vec<float>::get(C6Vec<float>::load(weights + c + i), f);
+            else C6Vec<float>::get_some(weights + c + i, n - i, 0.f, f);
+#pragma unroll
+            for (int j = 0; j < 4; j++) q[i + j] = ok >> (i + j) & 1 ? f[j] : 0.f;
+        }
+    }
+};
+
+template <bool WEIGHTS>
+__device__ __forceinline__ Beside beside(const Rows &l, const Target &t, int64_t r, int v0) {
+    return Beside{WEIGHTS ? (const float *)t.p + r * t.stride + v0 : nullptr, l.mask ? l.mask + r * l.mask_row + (int64_t)(v0 >> 3) * l.mask_byte : nullptr, l.mask_byte};
+}
+
+template <typename T, int LANES, int NV, bool WEIGHTS>
+__device__ __forceinline__ Part part_of(Held<T, LANES, NV> &h, const Beside &at, int lane) {
+    typedef C6Vec<T> V;
+    Part p{-INFINITY, 0.f, 0.f, 0.f};
+    if (at.mask) {
+        const auto keep = [&](c6_u32x4 &u, int c) {
+            const uint32_t ok = at.bits<V::N>(c);
+            float f[V::N];
+            V::get(u, f);
+#pragma unroll
+            for (int i = 0; i < V::N; i++) f[i] = ok >> i & 1 ? f[i] : -INFINITY;
+            u = V::put(f);
+        };
+#pragma unroll
+        for (int u = 0; u < NV; u++) {
+            if (h.has(u, lane)) keep(h.raw[u], u * LANES * V::N + lane * V::N);
+            unpack_again(h.raw[u]);
+        }
+        if (h.has_tail(lane)) keep(h.tail, h.whole * V::N);
+    }
+    const auto top = [&](c6_u32x4 &u) {
+        float f[V::N];
+        V::get(u, f);
+#pragma unroll
+        for (int i = 0; i < V::N; i++) p.m = fmaxf(p.m, f[i]);
+        unpack_again(u);
+    };
+#pragma unroll
+    for (int u = 0; u < NV; u++) top(h.raw[u]);
+    top(h.tail);
+    const float base = base_of(p.m);
+    const auto sum = [&](c6_u32x4 &u, bool there, int c, int n) {
+        float f[V::N];
+        V::get(u, f);
+#pragma unroll
+        for (int i = 0; i < V::N; i++) p.s += exp_of(f[i] - base);
+        if (WEIGHTS && there) {
+            float q[V::N];
+            at.get<V::N>(c, n, q);
+#pragma unroll
+            for (int i = 0; i < V::N; i++) {
+                p.w += q[i];
+                if (q[i] != 0.f) p.d += q[i] * (base - f[i]);
+            }
+        }
+        unpack_again(u);
+    };
+#pragma unroll
+    for (int u = 0; u < NV; u++) sum(h.raw[u], h.has(u, lane), u * LANES * V::N + lane * V::N, V::N);
+    sum(h.tail, h.has_tail(lane), h.whole * V::N, h.rest);
+    return p;
+}
+// what a row's Part says of it, and how its gradient goes: factor * exp(x - base) - scale * t
+struct Done {
+    float loss, lse, total, factor, base;
+    bool some;
+};
+__device__ __forceinline__ Done done(const Part &p, float scale) {
+    Done k;
+    const float log_s = LN2 * __builtin_amdgcn_logf(p.s);
+    k.some = p.s != 0.f;
+    k.base = base_of(p.m);
+    k.loss = k.some ? p.w * log_s + p.d : 0.f;
+    k.lse = k.some ? p.m + log_s : -INFINITY;
+    k.total = k.some ? p.w : 0.f;
+    k.factor = scale * (p.w / p.s);
+    return k;
+}
+template <typename T, bool WEIGHTS>
+__device__ __forceinline__ void gradient(const c6_u32x4 &u, const Beside &at, const Done &k, float scale, int index, int c, int n, T *g) {
+    typedef C6Vec<T> V;
+    float f[V::N];
+    V::get(u, f);
+#pragma unroll
+    for (int i = 0; i < V::N; i++) f[i] = k.some ? k.factor * exp_of(f[i] - k.base) : 0.f;
+    if (WEIGHTS && k.some) {
+        float q[V::N];
+        at.get<V::N>(c, n, q);
+#pragma unroll
+        for (int i = 0; i < V::N; i++) f[i] -= scale * q[i];
+    }
+    if (!WEIGHTS && k.some && (unsigned)(index - c) < (unsigned)V::N) {
+#pragma unroll
+        for (int i = 0; i < V::N; i++) f[i] -= c + i == index ? scale : 0.f;
+    }
+    if (n >= V::N) V::store(g + c, V::put(f));
+    else V::put_some(g + c, n, f);
+}
+
+// One pass over rows that fit the registers of LANES lanes: read once, the gradient written once.  A lane takes the maximum of its own entries, the sums
+// relative to that, and one reduction over the lanes joins them.  As a piece's gradient leaves, the same piece of the workgroup's next row is requested
+// into its registers: loads and stores overlap, and the sums of a row begin as its first pieces arrive.
+template <typename T, int LANES, int NV, bool WEIGHTS>
+__global__ __launch_bounds__(LANES == 64 ? 256 : LANES) void c6_policy_loss_kernel(Rows l, Target t, float *loss, float *lse, float *total, T *grad, int64_t grad_stride, float scale) {
+    typedef C6Vec<T> V;
+    constexpr int PER = LANES == 64 ? 4 : 1;
+    __shared__ Part space[2][LANES / 64];
+    const int64_t step = (int64_t)gridDim.x * PER;
+    int64_t r = (int64_t)blockIdx.x * PER + (LANES == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
+    Held<T, LANES, NV> h(l.width);
+    if (r < l.rows) h.request((const T *)l.x + r * l.x_stride, threadIdx.x % LANES);
+    for (int turn = 0; r < l.rows; r += step, turn ^= 1) {
+        int lane = threadIdx.x % LANES;
+        asm volatile("" : "+v"(lane));      // (what follows from it is computed in every turn, not kept in registers across them)
         const T *x = (const T *)l.x + r * l.x_stride;
-        const int index = target_index(t, r, l.width);
-        float m = -INFINITY;
-        for (int v = threadIdx.x; v < l.width; v += 256)
-            if (legal(l, r, v)) m = fmaxf(m, c6_get(x[v]));
-        m = block_all(m, [](float a, float b) { return fmaxf(a, b); }, red);
-        if (m == -INFINITY) m = 0.f;
-        // NaN is not seen by the maximum but is by the sum; the terms t (m - x) are all >= 0: nothing cancels
-        float s = 0.f, w = 0.f, d = 0.f;
-        for (int v = threadIdx.x; v < l.width; v += 256)
-            if (legal(l, r, v)) {
-                const float y = c6_get(x[v]), q = target_weight(t, r, v, index);
-                s += expf(y - m);
-                w += q;
-                if (q != 0.f) d += q * (m - y);
-            }
-        s = block_all(s, add, red);
-        w = block_all(w, add, red);
-        d = block_all(d, add, red);
-        const bool some = s != 0.f;
-        if (threadIdx.x == 0) {
-            loss[r] = some ? w * logf(s) + d : 0.f;
-            lse[r] = some ? m + logf(s) : -INFINITY;
-            total[r] = some ? w : 0.f;
+        const Beside at = beside<WEIGHTS>(l, t, r, 0);
+        int index = -1;
+        float played = 0.f;
+        if (!WEIGHTS) {
+            index = target_index(t, r, l.width);
+            if (index >= 0 && !legal(l, r, index)) index = -1;
+            if (index >= 0) played = c6_get(x[index]);
         }
+        Part p = block_part<LANES>(part_of<T, LANES, NV, WEIGHTS>(h, at, lane), WEIGHTS, space[turn]);
+        if (!WEIGHTS && index >= 0) { p.w = 1.f; p.d = p.m - played; }
+        const Done k = done(p, scale);
+        if (lane == 0) { loss[r] = k.loss; lse[r] = k.lse; total[r] = k.total; }
+        const bool more = r + step < l.rows;
+        const T *next = x + (more ? step * l.x_stride : 0);
+        T *g = grad + r * grad_stride;
+#pragma unroll
+        for (int u = 0; u < NV; u++) {
+            if (grad && h.has(u, lane)) gradient<T, WEIGHTS>(h.raw[u], at, k, scale, index, u * LANES * V::N + lane * V::N, V::N, g);
+            if (more) h.request(u, next, lane);
+        }
+        if (grad && h.has_tail(lane)) gradient<T, WEIGHTS>(h.tail, at, k, scale, index, h.whole * V::N, h.rest, g);
+        if (more) h.request_tail(next, lane);
+    }
+}
+
+// The same in two launches, for rows that do not fit or are too few to fill the card: every chunk's Part into the workspace, then each chunk joins its
+// row's and writes its piece of the gradient.
+constexpr int SPLIT_NV = 4;
+template <typename T>
+constexpr int split_chunk = 256 * SPLIT_NV * C6Vec<T>::N;
+
+template <typename T, bool WEIGHTS>
+__global__ __launch_bounds__(256) void c6_policy_loss_part_kernel(Rows l, Target t, Part *parts, float *at) {
+    __shared__ Part space[4];
+    const int chunks = (l.width + split_chunk<T> - 1) / split_chunk<T>, lane = threadIdx.x;
+    const int64_t items = (int64_t)l.rows * chunks;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int64_t r = item / chunks;
+        const int v0 = (int)(item % chunks) * split_chunk<T>;
+        const T *x = (const T *)l.x + r * l.x_stride;
+        Held<T, 256, SPLIT_NV> h(min(l.width - v0, split_chunk<T>));
+        h.request(x + v0, lane);
+        const Part p = block_part<256>(part_of<T, 256, SPLIT_NV, WEIGHTS>(h, beside<WEIGHTS>(l, t, r, v0), lane), WEIGHTS, space);
+        if (lane == 0) parts[item] = p;
+        if (!WEIGHTS && lane == 0) {      // (the gradient may go where x is: the second launch does not read the entry again)
+            const int index = target_index(t, r, l.width);
+            if (index >= v0 && index - v0 < split_chunk<T>) at[r] = c6_get(x[index]);
+        }
+        __syncthreads();
+    }
+}
+
+template <typename T, bool WEIGHTS>
+__global__ __launch_bounds__(256) void c6_policy_loss_join_kernel(Rows l, Target t, const Part *parts, const float *at, float *loss, float *lse, float *total, T *grad,
+                                                                  int64_t grad_stride, float scale) {
+    typedef C6Vec<T> V;
+    __shared__ Part space[4];
+    const int chunks = (l.width + split_chunk<T> - 1) / split_chunk<T>, lane = threadIdx.x;
+    const int per = grad ? chunks : 1;      // without a gradient one workgroup a row
+    const int64_t items = (int64_t)l.rows * per;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int64_t r = item / per;
+        const int v0 = (int)(item % per) * split_chunk<T>;
+        const T *x = (const T *)l.x + r * l.x_stride;
+        Held<T, 256, SPLIT_NV> h(min(l.width - v0, split_chunk<T>));
+        if (grad) h.request(x + v0, lane);
+        int index = -1;
+        if (!WEIGHTS) {
+            index = target_index(t, r, l.width);
+            if (index >= 0 && !legal(l, r, index)) index = -1;
+        }
+        Part p{-INFINITY, 0.f, 0.f, 0.f};
+        for (int i = lane; i < chunks; i += 256) {
+            const Part o = parts[r * chunks + i];
+            const float M = fmaxf(p.m, o.m);
+            const Part a = from(p, M), b = from(o, M);
+            p = Part{M, a.s + b.s, a.w + b.w, a.d + b.d};
+        }
+        p = block_part<256>(p, WEIGHTS, space);
+        if (!WEIGHTS && index >= 0) { p.w = 1.f; p.d = p.m - at[r]; }
+        const Done k = done(p, scale);
+        if (v0 == 0 && lane == 0) { loss[r] = k.loss; lse[r] = k.lse; total[r] = k.total; }
         if (grad) {
-            const float inv = w / s;
-            for (int v = threadIdx.x; v < l.width; v += 256) {
-                float g = 0.f;
-                if (some && legal(l, r, v)) g = scale * (expf(c6_get(x[v]) - m) * inv - target_weight(t, r, v, index));
-                grad[r * grad_stride + v] = c6_put<T>(g);
-            }
+            const Beside here = beside<WEIGHTS>(l, t, r, v0);
+            T *g = grad + r * grad_stride + v0;
+            index = index < 0 ? -1 : index - v0;      // (of another chunk: outside this one's columns)
+            const auto piece = [&](c6_u32x4 &u, int c, int n) {
+                if (here.mask) {
+                    const uint32_t ok = here.bits<V::N>(c);
+                    float f[V::N];
+                    V::get(u, f);
+#pragma unroll
+                    for (int i = 0; i < V::N; i++) f[i] = ok >> i & 1 ? f[i] : -INFINITY;
+                    u = V::put(f);
+                }
+                gradient<T, WEIGHTS>(u, here, k, scale, index, c, n, g);
+            };
+#pragma unroll
+            for (int u = 0; u < SPLIT_NV; u++)
+                if (h.has(u, lane)) piece(h.raw[u], (u * 256 + lane) * V::N, V::N);
+            if (h.has_tail(lane)) piece(h.tail, h.whole * V::N, h.rest);
         }
+        __syncthreads();
     }
 }
 
@@ -328,6 +602,14 @@ unsigned grid_of(const c6_logits *l, int chunk, int per) {
     return (unsigned)std::min<int64_t>((items + per - 1) / per, 1 << 22);
 }
 
+int cus() {
+    static const int n = [] {
+        int v = 0, d = 0;
+        return hipGetDevice(&d) == hipSuccess && hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, d) == hipSuccess && v > 0 ? v : 256;
+    }();
+    return n;
+}
+
 Rows rows_of(const c6_logits *l) { return Rows{l->x, l->mask, l->x_stride, l->mask_row, l->mask_byte, l->rows, l->width}; }
 
 int launched() { return hipGetLastError() == hipSuccess ? C6_OK : c6_set_error(C6_ERR_HIP, "logits: launch failed"); }
@@ -368,7 +650,65 @@ extern "C" int c6_logits_process(const c6_logits *l, const int32_t *history, int
     return launched();
 }
 
-extern "C" size_t c6_policy_loss_workspace(int rows, int width) { return 0; }
+// Which way the loss goes, by the row's pieces of N entries a lane (16 bytes): registers hold 64, 256 or 1024 lanes of up to 16 pieces; longer rows, and rows
+// too few for one workgroup each to fill the card, are split into chunks.
+#ifndef SR
+#define SR 128
+#endif
+#ifndef SW
+#define SW 2048
+#endif
+static bool splits(int64_t rows, int64_t width, int n, bool weights) { return width > (weights ? 8192 : 16384) * n || (rows <= SR && width > SW * n); }
+static size_t split_bytes(int64_t rows, int64_t width, int n) {
+    const int64_t chunk = 256 * SPLIT_NV * n;
+    return (size_t)rows * ((size_t)((width + chunk - 1) / chunk) * sizeof(Part) + sizeof(float));
+}
+
+extern "C" size_t c6_policy_loss_workspace(int rows, int width) {
+    size_t need = 0;
+    for (int n : {4, 8})      // whatever the type
+        if (rows > 0 && splits(rows, width, n, true)) need = std::max(need, split_bytes(rows, width, n));
+    return need;
+}
+
+template <typename T, bool WEIGHTS>
+static void loss_launch(const c6_logits *l, const Target &t, float *loss, float *lse, float *total, T *grad, int64_t grad_stride, float scale, void *workspace, hipStream_t s) {
+    constexpr int N = C6Vec<T>::N;
+    const Rows rows = rows_of(l);
+    if (splits(l->rows, l->width, N, WEIGHTS)) {
+        const int64_t chunks = (l->width + split_chunk<T> - 1) / split_chunk<T>, items = l->rows * chunks;
+        Part *parts = (Part *)workspace;
+        float *at = (float *)(parts + items);
+        const unsigned grid = (unsigned)std::min<int64_t>(items, 1 << 22);
+        hipLaunchKernelGGL((c6_policy_loss_part_kernel<T, WEIGHTS>), dim3(grid), dim3(256), 0, s, rows, t, parts, at);
+        hipLaunchKernelGGL((c6_policy_loss_join_kernel<T, WEIGHTS>), dim3(grad ? grid : (unsigned)std::min(l->rows, 1 << 22)), dim3(256), 0, s, rows, t, parts, at, loss, lse,
+                           total, grad, grad_stride, scale);
+        return;
+    }
+#ifndef G64
+#define G64 8
+#endif
+#ifndef G256
+#define G256 4
+#endif
+#ifndef G1024
+#define G1024 1
+#endif
+#define C6_LAUNCH(LANES, NV, RESIDENT)                                                                                                                                      \
+    hipLaunchKernelGGL((c6_policy_loss_kernel<T, LANES, NV, WEIGHTS>), dim3((unsigned)std::min<int64_t>(LANES == 64 ? ((int64_t)l->rows + 3) / 4 : l->rows, (int64_t)cus() * RESIDENT)), \
+                       dim3(LANES == 64 ? 256 : LANES), 0, s, rows, t, loss, lse, total, grad, grad_stride, scale)
+    const int pieces = (l->width + N - 1) / N;
+    if (pieces <= 64) C6_LAUNCH(64, 1, G64);
+    else if (pieces <= 128) C6_LAUNCH(64, 2, G64);
+    else if (pieces <= 256) C6_LAUNCH(64, 4, G64);
+    else if (pieces <= 512) C6_LAUNCH(256, 2, G256);
+    else if (pieces <= 1024) C6_LAUNCH(256, 4, G256);
+    else if (pieces <= 2048) C6_LAUNCH(256, 8, G256);
+    else if (pieces <= 4096) C6_LAUNCH(1024, 4, G1024);
+    else if (pieces <= 8192) C6_LAUNCH(1024, 8, G1024);
+    else if constexpr (!WEIGHTS) C6_LAUNCH(1024, 16, 1);
+#undef C6_LAUNCH
+}
 
 extern "C" int c6_policy_loss(const c6_logits *l, const void *target, int target_kind, int64_t target_stride, float *loss, float *lse, float *total, void *grad,
                               int64_t grad_stride, float grad_scale, void *workspace, size_t workspace_bytes, void *stream) {
@@ -378,13 +718,16 @@ extern "C" int c6_policy_loss(const c6_logits *l, const void *target, int target
         if (int rc = check_written(l, grad, grad_stride, "")) return rc;
     if (l->rows && (!loss || !lse || !total)) return bad("c6_policy_loss: loss, lse or total is NULL");
     if (!c6_aligned(loss, 4) || !c6_aligned(lse, 4) || !c6_aligned(total, 4)) return bad("c6_policy_loss: loss, lse and total are aligned to 4 bytes");
+    const int n = l->type == C6_TYPE_F32 ? 4 : 8;
+    if (l->rows && splits(l->rows, l->width, n, target_kind == C6_TARGET_WEIGHTS) && (!workspace || workspace_bytes < split_bytes(l->rows, l->width, n) || !c6_aligned(workspace, alignof(Part))))
+        return bad("c6_policy_loss: the workspace is NULL, smaller than c6_policy_loss_workspace() or not aligned to 16 bytes");
     if (int rc = c6_check_device(l->device)) return rc;
     if (!l->rows) return C6_OK;
     C6DeviceScope scope(l->device);
     if (!scope.ok) return c6_set_error(C6_ERR_HIP, "c6_policy_loss: hipSetDevice");
     const Target t{target, target_stride, target_kind};
-    C6_BY_TYPE(l->type, T, hipLaunchKernelGGL((c6_policy_loss_kernel<T>), dim3((unsigned)std::min(l->rows, 1 << 20)), dim3(256), 0, (hipStream_t)stream, rows_of(l), t,
-                                              loss, lse, total, (T *)grad, grad_stride, grad_scale));
+    C6_BY_TYPE(l->type, T, if (target_kind == C6_TARGET_WEIGHTS) loss_launch<T, true>(l, t, loss, lse, total, (T *)grad, grad_stride, grad_scale, workspace, (hipStream_t)stream);
+               else loss_launch<T, false>(l, t, loss, lse, total, (T *)grad, grad_stride, grad_scale, workspace, (hipStream_t)stream));
     return launched();
 }
 

@@ -594,7 +594,7 @@ enum {
     C6_TARGET_INDEX64 = 1,   /* ... int64 */
     C6_TARGET_WEIGHTS = 2    /* target: float, weight v of row r at target[r * target_stride + v]: visit counts, a teacher's distribution */
 };
-/* bytes of workspace that c6_policy_loss needs for so many rows and entries (may be 0) */
+/* bytes of workspace (aligned to 16) that c6_policy_loss needs for so many rows and entries, of any type (may be 0) */
 size_t c6_policy_loss_workspace(int rows, int width);
 /* loss, lse, total: float [rows], written.  grad (type of x, stride in elements) may be NULL: no gradient; else the gradient at
  * scale = grad_scale for every row (1 / rows: the mean's).  grad may be x itself (same pointer and stride) and overlaps nothing else. */
