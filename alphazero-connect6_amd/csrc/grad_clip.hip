@@ -11,9 +11,11 @@ struct Chunk {                    // a piece of one tensor, the work of one work
     void *dst;
     uint32_t n, type;
 };
-constexpr uint32_t CHUNK = 32768;         // elements
-constexpr int MAXPART = 2048;             // partial sums: workgroups of the norm's pass
+// 8192 elements: 32 KB or 16 KB, all of a lane's loads (8 or 4 of 16 bytes) in flight at once
+constexpr uint32_t CHUNK = 8192;
+constexpr int MAXPART = 2048;             // partial sums = workgroups: 8 a CU
 
+// over the workgroup's 256 threads, in a fixed order, the same in all of them
 __device__ double block_sum(double v, double *red) {
     v = c6_wave_sum(v);
     __syncthreads();
@@ -22,13 +24,28 @@ __device__ double block_sum(double v, double *red) {
     return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// Squares are taken and summed in 64 bits: 1e30^2 does not overflow and 1e-30^2 does not vanish.
+// Squares are taken and summed in 64 bits: 1e30^2 does not overflow and 1e-30^2 does not vanish.  (A conversion and a fused multiply-add an element: a
+// third of what the vector unit could do while the memory delivers.)
 template <typename T>
-__device__ double chunk_squares(const T *x, uint32_t n) {
+__device__ __forceinline__ double chunk_squares(const T *x, uint32_t n) {
+    typedef C6Vec<T> V;
+    constexpr int U = CHUNK / (256 * V::N);
+    c6_u32x4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const uint32_t c = (u * 256 + threadIdx.x) * V::N;
+        raw[u] = c6_u32x4{0, 0, 0, 0};
+        if (c + V::N <= n) raw[u] = V::load(x + c);
+    }
     double s = 0;
-    for (uint32_t i = threadIdx.x; i < n; i += 256) {
-        const double g = (double)c6_get(x[i]);
-        s = __builtin_fma(g, g, s);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const uint32_t c = (u * 256 + threadIdx.x) * V::N;
+        float g[V::N];
+        if (c < n && c + V::N > n) V::get_some(x + c, n - c, 0.f, g);
+        else V::get(raw[u], g);
+#pragma unroll
+        for (int i = 0; i < V::N; i++) s = __builtin_fma((double)g[i], (double)g[i], s);
     }
     return s;
 }
@@ -56,16 +73,43 @@ __global__ __launch_bounds__(256) void c6_clip_finish_kernel(const double *parti
     if (threadIdx.x == 0) *norm = (float)n;
 }
 
+template <typename T>
+__device__ __forceinline__ void chunk_scale(const T *x, T *y, uint32_t n, float f) {
+    typedef C6Vec<T> V;
+    constexpr int U = CHUNK / (256 * V::N);
+    c6_u32x4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const uint32_t c = (u * 256 + threadIdx.x) * V::N;
+        if (c + V::N <= n) raw[u] = V::load(x + c);
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const uint32_t c = (u * 256 + threadIdx.x) * V::N;
+        if (c >= n) continue;
+        const bool whole = c + V::N <= n;
+        float g[V::N];
+        if (whole) V::get(raw[u], g);
+        else V::get_some(x + c, n - c, 0.f, g);
+#pragma unroll
+        for (int i = 0; i < V::N; i++) g[i] *= f;
+        if (whole) V::store(y + c, V::put(g));
+        else V::put_some(y + c, n - c, g);
+    }
+}
+
+// Every workgroup adds up the partial sums itself (at most 16 KB, from the L2) instead of waiting for a launch between.  The chunks go from the last to the
+// first: what the norm's pass read last is what the 256 MB cache still holds.
 __global__ __launch_bounds__(256) void c6_clip_apply_kernel(const Chunk *table, int chunks, const double *partial, int parts, float max_norm, float *norm) {
     __shared__ double red[4];
     const double n = total_norm(partial, parts, red);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
     const double q = (double)max_norm / (n + 1e-6);
     const float f = q > 1.0 ? 1.f : (float)q;       // a NaN norm makes f NaN
-    for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+    for (int c = chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
         const Chunk k = table[c];
         if (f == 1.f && k.src == k.dst) continue;   // g * 1 is g
-        C6_BY_TYPE(k.type, T, for (uint32_t i = threadIdx.x; i < k.n; i += 256) ((T *)k.dst)[i] = c6_put<T>(c6_get(((const T *)k.src)[i]) * f));
+        C6_BY_TYPE(k.type, T, chunk_scale((const T *)k.src, (T *)k.dst, k.n, f));
     }
 }
 

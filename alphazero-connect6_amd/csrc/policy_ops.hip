@@ -305,20 +305,16 @@ __device__ __forceinline__ Part part_of(Held<T, LANES, NV> &h, const Beside &at,
         }
         if (h.has_tail(lane)) keep(h.tail, h.whole * V::N);
     }
-    const auto top = [&](c6_u32x4 &u) {
-        float f[V::N];
+    // some pieces' maximum, then their sums relative to the greatest so far: they need no piece that comes later, which may still be on its way
+    const auto take = [&](const c6_u32x4 &u, float (&f)[V::N]) {
         V::get(u, f);
+        float m = f[0];
 #pragma unroll
-        for (int i = 0; i < V::N; i++) p.m = fmaxf(p.m, f[i]);
-        unpack_again(u);
+        for (int i = 1; i < V::N; i++) m = fmaxf(m, f[i]);
+        return m;
     };
-#pragma unroll
-    for (int u = 0; u < NV; u++) top(h.raw[u]);
-    top(h.tail);
-    const float base = base_of(p.m);
-    const auto sum = [&](c6_u32x4 &u, bool there, int c, int n) {
-        float f[V::N];
-        V::get(u, f);
+    const auto sum = [&](const float (&f)[V::N], bool there, int c, int n) {
+        const float base = base_of(p.m);
 #pragma unroll
         for (int i = 0; i < V::N; i++) p.s += exp_of(f[i] - base);
         if (WEIGHTS && there) {
@@ -330,45 +326,59 @@ __device__ __forceinline__ Part part_of(Held<T, LANES, NV> &h, const Beside &at,
                 if (q[i] != 0.f) p.d += q[i] * (base - f[i]);
             }
         }
-        unpack_again(u);
     };
+    constexpr int GROUP = NV < 16 / V::N ? NV : 16 / V::N;
+    static_assert(NV % GROUP == 0, "whole groups of pieces");
 #pragma unroll
-    for (int u = 0; u < NV; u++) sum(h.raw[u], h.has(u, lane), u * LANES * V::N + lane * V::N, V::N);
-    sum(h.tail, h.has_tail(lane), h.whole * V::N, h.rest);
+    for (int u = 0; u < NV; u += GROUP) {
+        float f[GROUP][V::N], m = p.m;
+#pragma unroll
+        for (int j = 0; j < GROUP; j++) m = fmaxf(m, take(h.raw[u + j], f[j]));
+        p = from(p, m);
+#pragma unroll
+        for (int j = 0; j < GROUP; j++) sum(f[j], h.has(u + j, lane), (u + j) * LANES * V::N + lane * V::N, V::N);
+#pragma unroll
+        for (int j = 0; j < GROUP; j++) unpack_again(h.raw[u + j]);
+    }
+    if (h.rest) {
+        float f[V::N];
+        p = from(p, fmaxf(p.m, take(h.tail, f)));
+        sum(f, h.has_tail(lane), h.whole * V::N, h.rest);
+    }
     return p;
 }
-// what a row's Part says of it, and how its gradient goes: factor * exp(x - base) - scale * t
+// what a row's Part says of it, and how its gradient goes: factor * exp(x - base) - scale * t (both 0 where there is nothing above -infinity)
 struct Done {
-    float loss, lse, total, factor, base;
-    bool some;
+    float loss, lse, total, factor, scale, base;
 };
 __device__ __forceinline__ Done done(const Part &p, float scale) {
     Done k;
     const float log_s = LN2 * __builtin_amdgcn_logf(p.s);
-    k.some = p.s != 0.f;
+    const bool some = p.s != 0.f;
     k.base = base_of(p.m);
-    k.loss = k.some ? p.w * log_s + p.d : 0.f;
-    k.lse = k.some ? p.m + log_s : -INFINITY;
-    k.total = k.some ? p.w : 0.f;
-    k.factor = scale * (p.w / p.s);
+    k.loss = some ? p.w * log_s + p.d : 0.f;
+    k.lse = some ? p.m + log_s : -INFINITY;
+    k.total = some ? p.w : 0.f;
+    k.factor = some ? scale * (p.w / p.s) : 0.f;
+    k.scale = some ? scale : 0.f;
     return k;
 }
 template <typename T, bool WEIGHTS>
-__device__ __forceinline__ void gradient(const c6_u32x4 &u, const Beside &at, const Done &k, float scale, int index, int c, int n, T *g) {
+__device__ __forceinline__ void gradient(const c6_u32x4 &u, const Beside &at, const Done &k, int index, int c, int n, T *g) {
     typedef C6Vec<T> V;
     float f[V::N];
     V::get(u, f);
 #pragma unroll
-    for (int i = 0; i < V::N; i++) f[i] = k.some ? k.factor * exp_of(f[i] - k.base) : 0.f;
-    if (WEIGHTS && k.some) {
+    for (int i = 0; i < V::N; i++) f[i] = k.factor * exp_of(f[i] - k.base);
+    if (WEIGHTS) {
         float q[V::N];
         at.get<V::N>(c, n, q);
 #pragma unroll
-        for (int i = 0; i < V::N; i++) f[i] -= scale * q[i];
+        for (int i = 0; i < V::N; i++) f[i] -= k.scale * q[i];
     }
-    if (!WEIGHTS && k.some && (unsigned)(index - c) < (unsigned)V::N) {
+    if (!WEIGHTS && (unsigned)(index - c) < (unsigned)V::N) {
 #pragma unroll
-        for (int i = 0; i < V::N; i++) f[i] -= c + i == index ? scale : 0.f;
+        for (int i = 0; i < V::N; i++) f[i] -= c + i == index ? k.scale : 0.f;
     }
     if (n >= V::N) V::store(g + c, V::put(f));
     else V::put_some(g + c, n, f);
@@ -407,10 +417,10 @@ __global__ __launch_bounds__(LANES == 64 ? 256 : LANES) void c6_policy_loss_kern
         T *g = grad + r * grad_stride;
 #pragma unroll
         for (int u = 0; u < NV; u++) {
-            if (grad && h.has(u, lane)) gradient<T, WEIGHTS>(h.raw[u], at, k, scale, index, u * LANES * V::N + lane * V::N, V::N, g);
+            if (grad && h.has(u, lane)) gradient<T, WEIGHTS>(h.raw[u], at, k, index, u * LANES * V::N + lane * V::N, V::N, g);
             if (more) h.request(u, next, lane);
         }
-        if (grad && h.has_tail(lane)) gradient<T, WEIGHTS>(h.tail, at, k, scale, index, h.whole * V::N, h.rest, g);
+        if (grad && h.has_tail(lane)) gradient<T, WEIGHTS>(h.tail, at, k, index, h.whole * V::N, h.rest, g);
         if (more) h.request_tail(next, lane);
     }
 }
@@ -485,7 +495,7 @@ __global__ __launch_bounds__(256) void c6_policy_loss_join_kernel(Rows l, Target
                     for (int i = 0; i < V::N; i++) f[i] = ok >> i & 1 ? f[i] : -INFINITY;
                     u = V::put(f);
                 }
-                gradient<T, WEIGHTS>(u, here, k, scale, index, c, n, g);
+                gradient<T, WEIGHTS>(u, here, k, index, c, n, g);
             };
 #pragma unroll
             for (int u = 0; u < SPLIT_NV; u++)
@@ -650,15 +660,15 @@ extern "C" int c6_logits_process(const c6_logits *l, const int32_t *history, int
     return launched();
 }
 
-// Which way the loss goes, by the row's pieces of N entries a lane (16 bytes): registers hold 64, 256 or 1024 lanes of up to 16 pieces; longer rows, and rows
-// too few for one workgroup each to fill the card, are split into chunks.
-#ifndef SR
-#define SR 128
-#endif
-#ifndef SW
-#define SW 2048
-#endif
-static bool splits(int64_t rows, int64_t width, int n, bool weights) { return width > (weights ? 8192 : 16384) * n || (rows <= SR && width > SW * n); }
+// Which way the loss goes, by the pieces of N entries (16 bytes) in a row.  The registers of 64, 256 or 1024 lanes hold up to 16384 (against weights, which
+// need registers of their own, 8192).  Split into chunks go
+//   longer rows;
+//   rows of over 8192 pieces that are too few for a workgroup each to fill the card (3 x 100003 bf16: 17.7 us in one workgroup a row);
+//   without a gradient nothing need be held: from 2048 pieces on small workgroups are faster (2048 x 100003 bf16: 77 against 113 us; few rows: one launch is).
+static bool splits(int64_t rows, int64_t width, int n, bool weights, bool grad) {
+    const int64_t pieces = (width + n - 1) / n;
+    return pieces > (weights ? 8192 : 16384) || (rows <= 128 ? pieces > 8192 : !grad && pieces > 2048);
+}
 static size_t split_bytes(int64_t rows, int64_t width, int n) {
     const int64_t chunk = 256 * SPLIT_NV * n;
     return (size_t)rows * ((size_t)((width + chunk - 1) / chunk) * sizeof(Part) + sizeof(float));
@@ -667,7 +677,7 @@ static size_t split_bytes(int64_t rows, int64_t width, int n) {
 extern "C" size_t c6_policy_loss_workspace(int rows, int width) {
     size_t need = 0;
     for (int n : {4, 8})      // whatever the type
-        if (rows > 0 && splits(rows, width, n, true)) need = std::max(need, split_bytes(rows, width, n));
+        if (rows > 0 && splits(rows, width, n, true, false)) need = std::max(need, split_bytes(rows, width, n));
     return need;
 }
 
@@ -675,7 +685,7 @@ template <typename T, bool WEIGHTS>
 static void loss_launch(const c6_logits *l, const Target &t, float *loss, float *lse, float *total, T *grad, int64_t grad_stride, float scale, void *workspace, hipStream_t s) {
     constexpr int N = C6Vec<T>::N;
     const Rows rows = rows_of(l);
-    if (splits(l->rows, l->width, N, WEIGHTS)) {
+    if (splits(l->rows, l->width, N, WEIGHTS, grad != nullptr)) {
         const int64_t chunks = (l->width + split_chunk<T> - 1) / split_chunk<T>, items = l->rows * chunks;
         Part *parts = (Part *)workspace;
         float *at = (float *)(parts + items);
@@ -685,27 +695,18 @@ static void loss_launch(const c6_logits *l, const Target &t, float *loss, float 
                            total, grad, grad_stride, scale);
         return;
     }
-#ifndef G64
-#define G64 8
-#endif
-#ifndef G256
-#define G256 4
-#endif
-#ifndef G1024
-#define G1024 1
-#endif
 #define C6_LAUNCH(LANES, NV, RESIDENT)                                                                                                                                      \
     hipLaunchKernelGGL((c6_policy_loss_kernel<T, LANES, NV, WEIGHTS>), dim3((unsigned)std::min<int64_t>(LANES == 64 ? ((int64_t)l->rows + 3) / 4 : l->rows, (int64_t)cus() * RESIDENT)), \
                        dim3(LANES == 64 ? 256 : LANES), 0, s, rows, t, loss, lse, total, grad, grad_stride, scale)
     const int pieces = (l->width + N - 1) / N;
-    if (pieces <= 64) C6_LAUNCH(64, 1, G64);
-    else if (pieces <= 128) C6_LAUNCH(64, 2, G64);
-    else if (pieces <= 256) C6_LAUNCH(64, 4, G64);
-    else if (pieces <= 512) C6_LAUNCH(256, 2, G256);
-    else if (pieces <= 1024) C6_LAUNCH(256, 4, G256);
-    else if (pieces <= 2048) C6_LAUNCH(256, 8, G256);
-    else if (pieces <= 4096) C6_LAUNCH(1024, 4, G1024);
-    else if (pieces <= 8192) C6_LAUNCH(1024, 8, G1024);
+    if (pieces <= 64) C6_LAUNCH(64, 1, 1 << 14);
+    else if (pieces <= 128) C6_LAUNCH(64, 2, 1 << 14);
+    else if (pieces <= 256) C6_LAUNCH(64, 4, 1 << 14);
+    else if (pieces <= 512) C6_LAUNCH(256, 2, 1 << 14);
+    else if (pieces <= 1024) C6_LAUNCH(256, 4, 1 << 14);
+    else if (pieces <= 2048) C6_LAUNCH(256, 8, 1 << 14);
+    else if (pieces <= 4096) C6_LAUNCH(1024, 4, 1);
+    else if (pieces <= 8192) C6_LAUNCH(1024, 8, 1);
     else if constexpr (!WEIGHTS) C6_LAUNCH(1024, 16, 1);
 #undef C6_LAUNCH
 }
@@ -719,7 +720,7 @@ extern "C" int c6_policy_loss(const c6_logits *l, const void *target, int target
     if (l->rows && (!loss || !lse || !total)) return bad("c6_policy_loss: loss, lse or total is NULL");
     if (!c6_aligned(loss, 4) || !c6_aligned(lse, 4) || !c6_aligned(total, 4)) return bad("c6_policy_loss: loss, lse and total are aligned to 4 bytes");
     const int n = l->type == C6_TYPE_F32 ? 4 : 8;
-    if (l->rows && splits(l->rows, l->width, n, target_kind == C6_TARGET_WEIGHTS) && (!workspace || workspace_bytes < split_bytes(l->rows, l->width, n) || !c6_aligned(workspace, alignof(Part))))
+    if (l->rows && splits(l->rows, l->width, n, target_kind == C6_TARGET_WEIGHTS, grad != nullptr) && (!workspace || workspace_bytes < split_bytes(l->rows, l->width, n) || !c6_aligned(workspace, alignof(Part))))
         return bad("c6_policy_loss: the workspace is NULL, smaller than c6_policy_loss_workspace() or not aligned to 16 bytes");
     if (int rc = c6_check_device(l->device)) return rc;
     if (!l->rows) return C6_OK;
