@@ -24,6 +24,11 @@ struct C6Vec {
     struct __attribute__((packed, aligned(sizeof(T)))) Raw { c6_u32x4 u; };
     static __device__ __forceinline__ c6_u32x4 load(const T *p) { return reinterpret_cast<const Raw *>(p)->u; }
     static __device__ __forceinline__ void store(T *p, c6_u32x4 u) { reinterpret_cast<Raw *>(p)->u = u; }
+    // ... written past the caches: nobody reads it soon, and what they hold is still wanted
+    static __device__ __forceinline__ void store_past(T *p, c6_u32x4 u) {
+        typedef uint32_t loose __attribute__((ext_vector_type(4), aligned(2)));
+        __builtin_nontemporal_store((loose)u, reinterpret_cast<loose *>(p));
+    }
     static __device__ __forceinline__ void get(c6_u32x4 u, float (&f)[N]) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
