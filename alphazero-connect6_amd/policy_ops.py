@@ -12,6 +12,7 @@ that do not fit raise C6Error before anything runs.  Nothing here is recorded by
 `import torch` comes before the first use of the library in a process that wants both on the GPU: whichever is first brings the HIP runtime
 that the other then shares (torch does not start on another's)."""
 import ctypes as C
+import sys
 
 import torch
 
@@ -25,60 +26,72 @@ if _pkg._lib is not None and _pkg.device_count() > 0 and not torch.cuda.is_avail
 _TYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _INDEX = {torch.int32: 0, torch.int64: 1}
 _WEIGHTS = 2
+_Tensor, _F32, _I32, _U8 = torch.Tensor, torch.float32, torch.int32, torch.uint8
+_SMALL = 8192        # entries of a row up to which the loss needs no workspace whatever the type (c6_policy_loss_workspace is 0)
 
 
-def _need(ok, message):
-    if not ok:
-        raise C6Error(message)
-
-
-def _stream(device):
+def _raw_stream(device):
     return torch.cuda.current_stream(device).cuda_stream
+
+
+# the handle alone where torch has a call for it: 0.1 us instead of 1.8
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+
+# The checks below cost a call less than its launch: messages are made when they are needed, and attributes are read once.
 
 
 def _logits(x, mask):
     """-> (c6_logits, rows, width)"""
-    _need(isinstance(x, torch.Tensor) and x.is_cuda and x.dim() == 2 and x.dtype in _TYPE,
-          "logits must be a [rows, width] tensor of float32, float16 or bfloat16 on the GPU")
+    kind = _TYPE.get(x.dtype) if isinstance(x, _Tensor) and x.is_cuda else None
+    if kind is None or x.dim() != 2:
+        raise C6Error("logits must be a [rows, width] tensor of float32, float16 or bfloat16 on the GPU")
     rows, width = x.shape
     stride, step = x.stride()
-    _need(step == 1 or width <= 1, "the entries of a row of logits must lie next to each other")
-    _need(not x.requires_grad, "logits that require a gradient: autograd does not see this operator, pass logits.detach()")
+    if step != 1 and width > 1:
+        raise C6Error("the entries of a row of logits must lie next to each other")
+    if x.requires_grad:
+        raise C6Error("logits that require a gradient: autograd does not see this operator, pass logits.detach()")
     device = x.get_device()
     if mask is None:
-        return Logits(rows, width, _TYPE[x.dtype], device, x.data_ptr(), stride, None, 0, 0), rows, width
-    _need(isinstance(mask, torch.Tensor) and mask.dtype is torch.uint8 and mask.get_device() == device, "mask must be a uint8 tensor on the logits' device")
+        return Logits(rows, width, kind, device, x.data_ptr(), stride, None, 0, 0), rows, width
+    if not isinstance(mask, _Tensor) or mask.dtype is not _U8 or mask.get_device() != device:
+        raise C6Error("mask must be a uint8 tensor on the logits' device")
     if mask.dim() == 1:
         mask = mask.unsqueeze(0)
-    nb = (width + 7) // 8
-    _need(mask.dim() == 2 and mask.shape[1] == nb and mask.shape[0] in (rows, 1),
-          f"mask must be [{rows}, {nb}] (or [1, {nb}], [{nb}]): one bit per entry of logits, entry v at bit v % 8 of byte v // 8")
+    if mask.dim() != 2 or mask.shape[1] != (width + 7) // 8 or mask.shape[0] not in (rows, 1):
+        raise C6Error(f"mask must be [{rows}, {(width + 7) // 8}], or one row for all: one bit per entry of logits, entry v at bit v % 8 of byte v // 8")
     row, byte = mask.stride()
-    return Logits(rows, width, _TYPE[x.dtype], device, x.data_ptr(), stride, mask.data_ptr(), 0 if mask.shape[0] == 1 else row, byte), rows, width
+    return Logits(rows, width, kind, device, x.data_ptr(), stride, mask.data_ptr(), 0 if mask.shape[0] == 1 else row, byte), rows, width
 
 
-def _written(out, x, rows, width, what):
+def _written(out, x, what):
     if out is None:
-        return torch.empty((rows, width), dtype=x.dtype, device=x.device)
-    _need(isinstance(out, torch.Tensor) and out.get_device() == x.get_device() and out.dtype is x.dtype and out.shape == x.shape,
-          f"{what} must have the logits' shape, type and device")
-    _need(out.stride(1) == 1 or width <= 1, f"the entries of a row of {what} must lie next to each other")
+        return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if not isinstance(out, _Tensor) or out.get_device() != x.get_device() or out.dtype is not x.dtype or out.shape != x.shape:
+        raise C6Error(f"{what} must have the logits' shape, type and device")
+    if out.requires_grad:
+        raise C6Error(f"{what} must not require a gradient")
+    if out.stride(1) != 1 and x.shape[1] > 1:
+        raise C6Error(f"the entries of a row of {what} must lie next to each other")
     return out
 
 
 def _rows_by(t, dtype, device, rows, width, what):
     """(pointer, row stride) of a [rows, width] / [1, width] / [width] tensor"""
-    _need(isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == device, f"{what} must be a {dtype} tensor on the logits' device")
-    if t.dim() == 1:
-        t = t.unsqueeze(0)
-    _need(t.dim() == 2 and t.shape[1] == width and t.shape[0] in (rows, 1), f"{what} must be [{rows}, {width}], [1, {width}] or [{width}]")
-    _need(t.stride(1) == 1 or width <= 1, f"the entries of a row of {what} must lie next to each other")
-    return t.data_ptr(), 0 if t.shape[0] == 1 else t.stride(0)
+    if not isinstance(t, _Tensor) or t.dtype is not dtype or t.get_device() != device:
+        raise C6Error(f"{what} must be a {dtype} tensor on the logits' device")
+    shape, stride = t.shape, t.stride()
+    dim = len(shape)
+    if dim not in (1, 2) or shape[-1] != width or (dim == 2 and shape[0] not in (rows, 1)):
+        raise C6Error(f"{what} must be [{rows}, {width}], [1, {width}] or [{width}]")
+    if stride[-1] != 1 and width > 1:
+        raise C6Error(f"the entries of a row of {what} must lie next to each other")
+    return t.data_ptr(), 0 if dim == 1 or shape[0] == 1 else stride[0]
 
 
-def _per_row(t, device, rows, what):
-    _need(isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.get_device() == device and t.shape == (rows,) and (rows <= 1 or t.stride(0) == 1),
-          f"{what} must be a contiguous float32 tensor [{rows}] on the logits' device")
+def _per_row(t, dtype, device, rows, what):
+    if not isinstance(t, _Tensor) or t.dtype is not dtype or t.get_device() != device or t.dim() != 1 or t.shape[0] != rows or (rows > 1 and t.stride(0) != 1):
+        raise C6Error(f"{what} must be a contiguous {dtype} tensor [{rows}] on the logits' device")
     return t.data_ptr()
 
 
@@ -94,37 +107,38 @@ def logits_process(logits, mask=None, bias=None, history=None, history_len=None,
     out: a tensor like logits, possibly logits itself.  Returns out."""
     l, rows, width = _logits(logits, mask)
     dev = l.device
-    out = _written(out, logits, rows, width, "out")
+    out = _written(out, logits, "out")
     h = n = p = b = None
     hs = ps = bs = cap = 0
     if history is not None:
-        _need(isinstance(history, torch.Tensor) and history.dim() in (1, 2), "history must be an int32 tensor [rows, cap] or [cap]")
+        if not isinstance(history, _Tensor) or history.dim() not in (1, 2) or penalties is None:
+            raise C6Error("history must be an int32 tensor [rows, cap] or [cap], and needs penalties")
         cap = history.shape[-1]
-        h, hs = _rows_by(history, torch.int32, dev, rows, cap, "history")
-        _need(penalties is not None, "a history needs penalties")
-        p, ps = _rows_by(penalties, torch.float32, dev, rows, 3, "penalties")
+        h, hs = _rows_by(history, _I32, dev, rows, cap, "history")
+        p, ps = _rows_by(penalties, _F32, dev, rows, 3, "penalties")
         if history_len is not None:
-            _need(isinstance(history_len, torch.Tensor) and history_len.dtype is torch.int32 and history_len.get_device() == dev
-                  and history_len.shape == (rows,) and (rows <= 1 or history_len.stride(0) == 1), f"history_len must be a contiguous int32 tensor [{rows}]")
-            n = history_len.data_ptr()
-    else:
-        _need(history_len is None and penalties is None, "history_len and penalties need a history")
+            n = _per_row(history_len, _I32, dev, rows, "history_len")
+    elif history_len is not None or penalties is not None:
+        raise C6Error("history_len and penalties need a history")
     if bias is not None:
-        b, bs = _rows_by(bias, torch.float32, dev, rows, width, "bias")
+        b, bs = _rows_by(bias, _F32, dev, rows, width, "bias")
     _chk(lib().c6_logits_process(l, h, hs, n, cap, p, ps, b, bs, out.data_ptr(), out.stride(0), _stream(dev)))
     return out
 
 
 def _target(targets, device, rows, width):
     """-> (pointer, kind, stride)"""
-    _need(isinstance(targets, torch.Tensor) and targets.get_device() == device, "targets must be a tensor on the logits' device")
-    if targets.dtype in _INDEX:
-        _need(targets.shape == (rows,) and (rows <= 1 or targets.stride(0) == 1), f"targets of indices must be contiguous, [{rows}]")
-        return targets.data_ptr(), _INDEX[targets.dtype], 0
-    _need(targets.dtype is torch.float32 and targets.dim() == 2 and targets.shape == (rows, width),
-          f"targets must be int32 or int64 indices [{rows}], or float32 weights [{rows}, {width}]")
-    _need(targets.stride(1) == 1 or width <= 1, "the weights of a row must lie next to each other")
-    return targets.data_ptr(), _WEIGHTS, targets.stride(0)
+    if not isinstance(targets, _Tensor) or targets.get_device() != device:
+        raise C6Error("targets must be a tensor on the logits' device")
+    kind = _INDEX.get(targets.dtype)
+    if kind is not None:
+        return _per_row(targets, targets.dtype, device, rows, "targets of indices"), kind, 0
+    if targets.dtype is not _F32 or targets.dim() != 2 or targets.shape[0] != rows or targets.shape[1] != width:
+        raise C6Error(f"targets must be int32 or int64 indices [{rows}], or float32 weights [{rows}, {width}]")
+    stride, step = targets.stride()
+    if step != 1 and width > 1:
+        raise C6Error("the weights of a row must lie next to each other")
+    return targets.data_ptr(), _WEIGHTS, stride
 
 
 def policy_loss(logits, targets, mask=None, grad_scale=None, grad=None):
@@ -137,21 +151,22 @@ def policy_loss(logits, targets, mask=None, grad_scale=None, grad=None):
     l, rows, width = _logits(logits, mask)
     dev = l.device
     t, kind, ts = _target(targets, dev, rows, width)
-    stats = torch.empty((3, rows), dtype=torch.float32, device=logits.device)
     g, gs = None, 0
     if grad_scale is not None:
-        grad = _written(grad, logits, rows, width, "grad")
+        grad = _written(grad, logits, "grad")
         g, gs = grad.data_ptr(), grad.stride(0)
-    else:
-        _need(grad is None, "grad needs a grad_scale")
-        grad_scale = 0.0
-    L = lib()
-    nbytes = L.c6_policy_loss_workspace(rows, width)
-    space = torch.empty(nbytes, dtype=torch.uint8, device=logits.device) if nbytes else None
+    elif grad is not None:
+        raise C6Error("grad needs a grad_scale")
+    stats = torch.empty((3, rows), dtype=_F32, device=logits.device)
     at = stats.data_ptr()
-    _chk(L.c6_policy_loss(l, t, kind, ts, at, at + 4 * rows, at + 8 * rows, g, gs, grad_scale, space.data_ptr() if nbytes else None, nbytes, _stream(dev)))
+    L = lib()
+    space, nbytes = None, L.c6_policy_loss_workspace(rows, width) if width > _SMALL else 0
+    if nbytes:
+        keep = torch.empty(nbytes, dtype=_U8, device=logits.device)
+        space = keep.data_ptr()
+    _chk(L.c6_policy_loss(l, t, kind, ts, at, at + 4 * rows, at + 8 * rows, g, gs, grad_scale or 0.0, space, nbytes, _stream(dev)))
     loss, lse, total = stats.unbind(0)
-    return (loss, lse, total) if g is None else (loss, lse, total, grad)
+    return (loss, lse, total) if grad is None else (loss, lse, total, grad)
 
 
 def policy_loss_grad(logits, targets, lse, total, dloss, mask=None, out=None):
@@ -160,11 +175,11 @@ def policy_loss_grad(logits, targets, lse, total, dloss, mask=None, out=None):
     l, rows, width = _logits(logits, mask)
     dev = l.device
     t, kind, ts = _target(targets, dev, rows, width)
-    out = _written(out, logits, rows, width, "out")
-    one = isinstance(dloss, torch.Tensor) and dloss.shape == (1,) and rows != 1
-    d = _per_row(dloss, dev, 1 if one else rows, "dloss")
-    _chk(lib().c6_policy_loss_grad(l, t, kind, ts, _per_row(lse, dev, rows, "lse"), _per_row(total, dev, rows, "total"), d, 0 if one else 1, out.data_ptr(),
-                                   out.stride(0), _stream(dev)))
+    out = _written(out, logits, "out")
+    one = rows != 1 and isinstance(dloss, _Tensor) and dloss.dim() == 1 and dloss.shape[0] == 1
+    d = _per_row(dloss, _F32, dev, 1 if one else rows, "dloss")
+    _chk(lib().c6_policy_loss_grad(l, t, kind, ts, _per_row(lse, _F32, dev, rows, "lse"), _per_row(total, _F32, dev, rows, "total"), d, 0 if one else 1,
+                                   out.data_ptr(), out.stride(0), _stream(dev)))
     return out
 
 
@@ -180,12 +195,16 @@ class GradClip:
         grads = list(grads)
         outs = None if outs is None else list(outs)
         self.h = None
-        _need(grads and all(isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _TYPE and t.is_contiguous() for t in grads + (outs or [])),
-              "GradClip needs contiguous float32, float16 or bfloat16 tensors on the GPU")
+        for t in grads + (outs or []):
+            if not isinstance(t, _Tensor) or not t.is_cuda or t.dtype not in _TYPE or not t.is_contiguous():
+                raise C6Error("GradClip needs contiguous float32, float16 or bfloat16 tensors on the GPU")
+            if t.device != grads[0].device:
+                raise C6Error("GradClip's tensors live on one device")
+        if not grads:
+            raise C6Error("GradClip needs tensors")
+        if outs is not None and (len(outs) != len(grads) or any(o.shape != g.shape or o.dtype is not g.dtype for o, g in zip(outs, grads))):
+            raise C6Error("outs must be tensors like grads")
         self.device = grads[0].device
-        _need(all(t.device == self.device for t in grads + (outs or [])), "GradClip's tensors live on one device")
-        if outs is not None:
-            _need(len(outs) == len(grads) and all(o.shape == g.shape and o.dtype is g.dtype for o, g in zip(outs, grads)), "outs must be tensors like grads")
         k = len(grads)
         ptrs = (C.c_void_p * k)(*[t.data_ptr() for t in grads])
         optrs = None if outs is None else (C.c_void_p * k)(*[t.data_ptr() for t in outs])
@@ -198,36 +217,40 @@ class GradClip:
 
     def close(self):
         """frees the table once nothing that uses it runs any more"""
-        if getattr(self, "h", None):
-            _need(not torch.cuda.is_current_stream_capturing(), "GradClip cannot be closed during a capture")
+        if self.h:
+            if torch.cuda.is_current_stream_capturing():
+                raise C6Error("GradClip cannot be closed during a capture")
             torch.cuda.synchronize(self.device)
             while GradClip._late:
                 lib().c6_clip_destroy(GradClip._late.pop())
             lib().c6_clip_destroy(self.h)
             self.h = self._keep = None
 
-    def __del__(self):
-        if getattr(self, "h", None) and torch.cuda.is_current_stream_capturing():
+    def __del__(self, _ending=sys.is_finalizing):
+        if _ending() or not getattr(self, "h", None):
+            return
+        if torch.cuda.is_current_stream_capturing():
             GradClip._late.append(self.h)
         else:
             self.close()
 
     def _call(self, norm):
-        _need(self.h is not None, "GradClip is closed")
+        if not self.h:
+            raise C6Error("GradClip is closed")
         if norm is None:
-            norm = torch.empty(1, dtype=torch.float32, device=self.device)
-        _need(isinstance(norm, torch.Tensor) and norm.dtype is torch.float32 and norm.shape == (1,) and norm.device == self.device,
-              "norm must be a float32 tensor [1] on the gradients' device")
-        return norm, torch.empty(self._bytes, dtype=torch.uint8, device=self.device)
+            norm = torch.empty(1, dtype=_F32, device=self.device)
+        elif not isinstance(norm, _Tensor) or norm.dtype is not _F32 or norm.shape != (1,) or norm.device != self.device:
+            raise C6Error("norm must be a float32 tensor [1] on the gradients' device")
+        return norm, torch.empty(self._bytes, dtype=_U8, device=self.device)
 
     def norm(self, norm=None):
         """the global norm, a float32 tensor [1]; the gradients stay as they are"""
         norm, space = self._call(norm)
-        _chk(lib().c6_clip_norm(self.h, norm.data_ptr(), space.data_ptr(), self._bytes, _stream(self.device)))
+        _chk(lib().c6_clip_norm(self.h, norm.data_ptr(), space.data_ptr(), self._bytes, _stream(self.device.index)))
         return norm
 
     def clip(self, max_norm, norm=None):
         """scales the gradients; returns their norm before that, a float32 tensor [1]"""
         norm, space = self._call(norm)
-        _chk(lib().c6_clip_apply(self.h, max_norm, norm.data_ptr(), space.data_ptr(), self._bytes, _stream(self.device)))
+        _chk(lib().c6_clip_apply(self.h, max_norm, norm.data_ptr(), space.data_ptr(), self._bytes, _stream(self.device.index)))
         return norm
