@@ -221,33 +221,28 @@ __device__ __forceinline__ Part block_part(const Part &p, bool weights, Part *sp
     return q;
 }
 
-// A row (or a chunk of one) in the registers of LANES lanes, in pieces of N entries (16 bytes): lane i holds the pieces i, i + LANES, ...; the entries behind
-// the last whole piece are one more piece of the last lane.  What is not there, or not legal, is -infinity.
+// A row (or a chunk of one) in the registers of LANES lanes, in pieces of N entries (16 bytes): lane i holds the pieces i, i + LANES, ...; of the entries
+// behind the last whole piece (a board's 81, 225 or 361 leave one) lane i holds the i-th.  What is not there, or not legal, is -infinity.
 template <typename T, int LANES, int NV>
 struct Held {
     typedef C6Vec<T> V;
-    c6_u32x4 raw[NV], tail;
+    c6_u32x4 raw[NV];
+    float tail;
     int whole, rest;       // whole pieces, entries behind them
 
-    __device__ __forceinline__ Held(int width) : whole(width / V::N), rest(width % V::N) {
+    __device__ __forceinline__ Held(int width) : tail(-INFINITY), whole(width / V::N), rest(width % V::N) {
         float f[V::N];
 #pragma unroll
         for (int i = 0; i < V::N; i++) f[i] = -INFINITY;
-        tail = V::put(f);
 #pragma unroll
-        for (int u = 0; u < NV; u++) raw[u] = tail;
+        for (int u = 0; u < NV; u++) raw[u] = V::put(f);
     }
     __device__ __forceinline__ bool has(int u, int lane) const { return lane < whole - u * LANES; }
-    __device__ __forceinline__ bool has_tail(int lane) const { return rest && lane == LANES - 1; }
     __device__ __forceinline__ void request(int u, const T *x, int lane) {
         if (has(u, lane)) raw[u] = V::load(x + u * LANES * V::N + lane * V::N);
     }
     __device__ __forceinline__ void request_tail(const T *x, int lane) {
-        if (has_tail(lane)) {
-            float f[V::N];
-            V::get_some(x + whole * V::N, rest, -INFINITY, f);
-            tail = V::put(f);
-        }
+        if (lane < rest) tail = c6_get(x[whole * V::N + lane]);
     }
     __device__ __forceinline__ void request(const T *x, int lane) {
 #pragma unroll
@@ -255,6 +250,7 @@ struct Held {
         request_tail(x, lane);
     }
 };
+
 // what was unpacked from u before is not kept for later: unpacking again is cheaper than two or four registers a word
 __device__ __forceinline__ void unpack_again(c6_u32x4 &u) { asm volatile("" : "+v"(u)); }
 
@@ -265,19 +261,20 @@ struct Beside {
     int64_t byte;
     template <int N>
     __device__ __forceinline__ uint32_t bits(int c) const { return mask ? (uint32_t)mask[(int64_t)(c >> 3) * byte] >> (N == 4 ? c & 4 : 0) : ~0u; }
-    // weights of n entries from column c on, 0 where illegal
+    __device__ __forceinline__ bool legal(int c) const { return !mask || (mask[(int64_t)(c >> 3) * byte] >> (c & 7) & 1); }
+    // weights of a piece, or of one entry, from column c on: 0 where illegal
     template <int N>
-    __device__ __forceinline__ void get(int c, int n, float (&q)[N]) const {
+    __device__ __forceinline__ void get(int c, float (&q)[N]) const {
         const uint32_t ok = bits<N>(c);
 #pragma unroll
         for (int i = 0; i < N; i += 4) {
             float f[4];
-            if (n >= N) C6Vec<float>::get(C6Vec<float>::load(weights + c + i), f);
-            else C6Vec<float>::get_some(weights + c + i, n - i, 0.f, f);
+            C6Vec<float>::get(C6Vec<float>::load(weights + c + i), f);
 #pragma unroll
             for (int j = 0; j < 4; j++) q[i + j] = ok >> (i + j) & 1 ? f[j] : 0.f;
         }
     }
+    __device__ __forceinline__ float get(int c) const { return legal(c) ? weights[c] : 0.f; }
 };
 
 template <bool WEIGHTS>
@@ -303,7 +300,7 @@ __device__ __forceinline__ Part part_of(Held<T, LANES, NV> &h, const Beside &at,
             if (h.has(u, lane)) keep(h.raw[u], u * LANES * V::N + lane * V::N);
             unpack_again(h.raw[u]);
         }
-        if (h.has_tail(lane)) keep(h.tail, h.whole * V::N);
+        if (lane < h.rest && !at.legal(h.whole * V::N + lane)) h.tail = -INFINITY;
     }
     // some pieces' maximum, then their sums relative to the greatest so far: they need no piece that comes later, which may still be on its way
     const auto take = [&](const c6_u32x4 &u, float (&f)[V::N]) {
@@ -313,18 +310,19 @@ __device__ __forceinline__ Part part_of(Held<T, LANES, NV> &h, const Beside &at,
         for (int i = 1; i < V::N; i++) m = fmaxf(m, f[i]);
         return m;
     };
-    const auto sum = [&](const float (&f)[V::N], bool there, int c, int n) {
+    const auto weigh = [&](float x, float q) {
+        p.w += q;
+        if (q != 0.f) p.d += q * (base_of(p.m) - x);
+    };
+    const auto sum = [&](const float (&f)[V::N], bool there, int c) {
         const float base = base_of(p.m);
 #pragma unroll
         for (int i = 0; i < V::N; i++) p.s += exp_of(f[i] - base);
         if (WEIGHTS && there) {
             float q[V::N];
-            at.get<V::N>(c, n, q);
+            at.get<V::N>(c, q);
 #pragma unroll
-            for (int i = 0; i < V::N; i++) {
-                p.w += q[i];
-                if (q[i] != 0.f) p.d += q[i] * (base - f[i]);
-            }
+            for (int i = 0; i < V::N; i++) weigh(f[i], q[i]);
         }
     };
     constexpr int GROUP = NV < 16 / V::N ? NV : 16 / V::N;
@@ -336,14 +334,14 @@ __device__ __forceinline__ Part part_of(Held<T, LANES, NV> &h, const Beside &at,
         for (int j = 0; j < GROUP; j++) m = fmaxf(m, take(h.raw[u + j], f[j]));
         p = from(p, m);
 #pragma unroll
-        for (int j = 0; j < GROUP; j++) sum(f[j], h.has(u + j, lane), (u + j) * LANES * V::N + lane * V::N, V::N);
+        for (int j = 0; j < GROUP; j++) sum(f[j], h.has(u + j, lane), (u + j) * LANES * V::N + lane * V::N);
 #pragma unroll
         for (int j = 0; j < GROUP; j++) unpack_again(h.raw[u + j]);
     }
     if (h.rest) {
-        float f[V::N];
-        p = from(p, fmaxf(p.m, take(h.tail, f)));
-        sum(f, h.has_tail(lane), h.whole * V::N, h.rest);
+        p = from(p, fmaxf(p.m, h.tail));
+        p.s += exp_of(h.tail - base_of(p.m));
+        if (WEIGHTS && lane < h.rest) weigh(h.tail, at.get(h.whole * V::N + lane));
     }
     return p;
 }
@@ -364,7 +362,7 @@ __device__ __forceinline__ Done done(const Part &p, float scale) {
     return k;
 }
 template <typename T, bool WEIGHTS>
-__device__ __forceinline__ void gradient(const c6_u32x4 &u, const Beside &at, const Done &k, int index, int c, int n, T *g) {
+__device__ __forceinline__ void gradient(const c6_u32x4 &u, const Beside &at, const Done &k, int index, int c, T *g) {
     typedef C6Vec<T> V;
     float f[V::N];
     V::get(u, f);
@@ -372,7 +370,7 @@ __device__ __forceinline__ void gradient(const c6_u32x4 &u, const Beside &at, co
     for (int i = 0; i < V::N; i++) f[i] = k.factor * exp_of(f[i] - k.base);
     if (WEIGHTS) {
         float q[V::N];
-        at.get<V::N>(c, n, q);
+        at.get<V::N>(c, q);
 #pragma unroll
         for (int i = 0; i < V::N; i++) f[i] -= k.scale * q[i];
     }
@@ -380,8 +378,12 @@ __device__ __forceinline__ void gradient(const c6_u32x4 &u, const Beside &at, co
 #pragma unroll
         for (int i = 0; i < V::N; i++) f[i] -= c + i == index ? k.scale : 0.f;
     }
-    if (n >= V::N) V::store(g + c, V::put(f));
-    else V::put_some(g + c, n, f);
+    V::store(g + c, V::put(f));
+}
+template <typename T, bool WEIGHTS>
+__device__ __forceinline__ void gradient(float x, const Beside &at, const Done &k, int index, int c, T *g) {
+    const float q = WEIGHTS ? at.get(c) : (c == index ? 1.f : 0.f);
+    g[c] = c6_put<T>(k.factor * exp_of(x - k.base) - k.scale * q);
 }
 
 // One pass over rows that fit the registers of LANES lanes: read once, the gradient written once.  A lane takes the maximum of its own entries, the sums
@@ -417,10 +419,10 @@ __global__ __launch_bounds__(LANES == 64 ? 256 : LANES) void c6_policy_loss_kern
         T *g = grad + r * grad_stride;
 #pragma unroll
         for (int u = 0; u < NV; u++) {
-            if (grad && h.has(u, lane)) gradient<T, WEIGHTS>(h.raw[u], at, k, index, u * LANES * V::N + lane * V::N, V::N, g);
+            if (grad && h.has(u, lane)) gradient<T, WEIGHTS>(h.raw[u], at, k, index, u * LANES * V::N + lane * V::N, g);
             if (more) h.request(u, next, lane);
         }
-        if (grad && h.has_tail(lane)) gradient<T, WEIGHTS>(h.tail, at, k, index, h.whole * V::N, h.rest, g);
+        if (grad && lane < h.rest) gradient<T, WEIGHTS>(h.tail, at, k, index, h.whole * V::N + lane, g);
         if (more) h.request_tail(next, lane);
     }
 }
@@ -486,7 +488,7 @@ __global__ __launch_bounds__(256) void c6_policy_loss_join_kernel(Rows l, Target
             const Beside here = beside<WEIGHTS>(l, t, r, v0);
             T *g = grad + r * grad_stride + v0;
             index = index < 0 ? -1 : index - v0;      // (of another chunk: outside this one's columns)
-            const auto piece = [&](c6_u32x4 &u, int c, int n) {
+            const auto piece = [&](c6_u32x4 &u, int c) {
                 if (here.mask) {
                     const uint32_t ok = here.bits<V::N>(c);
                     float f[V::N];
@@ -495,12 +497,15 @@ __global__ __launch_bounds__(256) void c6_policy_loss_join_kernel(Rows l, Target
                     for (int i = 0; i < V::N; i++) f[i] = ok >> i & 1 ? f[i] : -INFINITY;
                     u = V::put(f);
                 }
-                gradient<T, WEIGHTS>(u, here, k, index, c, n, g);
+                gradient<T, WEIGHTS>(u, here, k, index, c, g);
             };
 #pragma unroll
             for (int u = 0; u < SPLIT_NV; u++)
-                if (h.has(u, lane)) piece(h.raw[u], (u * 256 + lane) * V::N, V::N);
-            if (h.has_tail(lane)) piece(h.tail, h.whole * V::N, h.rest);
+                if (h.has(u, lane)) piece(h.raw[u], (u * 256 + lane) * V::N);
+            if (lane < h.rest) {
+                const int c = h.whole * V::N + lane;
+                gradient<T, WEIGHTS>(here.legal(c) ? h.tail : -INFINITY, here, k, index, c, g);
+            }
         }
         __syncthreads();
     }
