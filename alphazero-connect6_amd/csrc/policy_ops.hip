@@ -254,18 +254,19 @@ struct Held {
 // what was unpacked from u before is not kept for later: unpacking again is cheaper than two or four registers a word
 __device__ __forceinline__ void unpack_again(c6_u32x4 &u) { asm volatile("" : "+v"(u)); }
 
-// weights and mask of the row (or chunk), whose first column is a multiple of 8
+// weights and mask of the row (or chunk), whose first column is a multiple of 8: of piece u, which begins at column c, and of single entries
 struct Beside {
     const float *weights;
     const uint8_t *mask;
     int64_t byte;
     template <int N>
-    __device__ __forceinline__ uint32_t bits(int c) const { return mask ? (uint32_t)mask[(int64_t)(c >> 3) * byte] >> (N == 4 ? c & 4 : 0) : ~0u; }
+    __device__ __forceinline__ uint32_t bits(int, int c) const { return mask ? (uint32_t)mask[(int64_t)(c >> 3) * byte] >> (N == 4 ? c & 4 : 0) : ~0u; }
+    __device__ __forceinline__ bool masked() const { return mask; }
     __device__ __forceinline__ bool legal(int c) const { return !mask || (mask[(int64_t)(c >> 3) * byte] >> (c & 7) & 1); }
-    // weights of a piece, or of one entry, from column c on: 0 where illegal
+    // weights: 0 where illegal
     template <int N>
-    __device__ __forceinline__ void get(int c, float (&q)[N]) const {
-        const uint32_t ok = bits<N>(c);
+    __device__ __forceinline__ void get(int u, int c, float (&q)[N]) const {
+        const uint32_t ok = bits<N>(u, c);
 #pragma unroll
         for (int i = 0; i < N; i += 4) {
             float f[4];
@@ -276,19 +277,60 @@ struct Beside {
     }
     __device__ __forceinline__ float get(int c) const { return legal(c) ? weights[c] : 0.f; }
 };
+// ... requested all at once and held: a wave with a short row waits for memory once
+template <typename T, int LANES, int NV, bool WEIGHTS>
+struct Fetched {
+    static constexpr int N = C6Vec<T>::N;
+    uint32_t ok[NV];
+    c6_u32x4 w[WEIGHTS ? NV : 1][N / 4];
+    bool any, tail_ok;
+    float tail_w;
+
+    __device__ __forceinline__ Fetched(const Beside &at, const Held<T, LANES, NV> &h, int lane) : any(at.mask), tail_ok(true), tail_w(0.f) {
+#pragma unroll
+        for (int u = 0; u < NV; u++) {
+            const int c = (u * LANES + lane) * N;
+            ok[u] = ~0u;
+            if (!h.has(u, lane)) continue;
+            if (any) ok[u] = at.template bits<N>(u, c);
+            if constexpr (WEIGHTS)
+#pragma unroll
+                for (int i = 0; i < N / 4; i++) w[u][i] = C6Vec<float>::load(at.weights + c + 4 * i);
+        }
+        if (lane < h.rest) {
+            const int c = h.whole * N + lane;
+            if (any) tail_ok = at.legal(c);
+            if (WEIGHTS) tail_w = at.weights[c];
+        }
+    }
+    __device__ __forceinline__ bool masked() const { return any; }
+    template <int M>
+    __device__ __forceinline__ uint32_t bits(int u, int) const { return ok[u]; }
+    __device__ __forceinline__ bool legal(int) const { return tail_ok; }
+    template <int M>
+    __device__ __forceinline__ void get(int u, int, float (&q)[M]) const {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            float f[4];
+            C6Vec<float>::get(w[WEIGHTS ? u : 0][i / 4], f);
+#pragma unroll
+            for (int j = 0; j < 4; j++) q[i + j] = ok[u] >> (i + j) & 1 ? f[j] : 0.f;
+        }
+    }
+    __device__ __forceinline__ float get(int) const { return tail_ok ? tail_w : 0.f; }
+};
 
 template <bool WEIGHTS>
 __device__ __forceinline__ Beside beside(const Rows &l, const Target &t, int64_t r, int v0) {
     return Beside{WEIGHTS ? (const float *)t.p + r * t.stride + v0 : nullptr, l.mask ? l.mask + r * l.mask_row + (int64_t)(v0 >> 3) * l.mask_byte : nullptr, l.mask_byte};
 }
 
-template <typename T, int LANES, int NV, bool WEIGHTS>
-__device__ __forceinline__ Part part_of(Held<T, LANES, NV> &h, const Beside &at, int lane) {
+template <typename T, int LANES, int NV, bool WEIGHTS, typename At>
+__device__ __forceinline__ Part part_of(Held<T, LANES, NV> &h, const At &at, int lane) {
     typedef C6Vec<T> V;
     Part p{-INFINITY, 0.f, 0.f, 0.f};
-    if (at.mask) {
-        const auto keep = [&](c6_u32x4 &u, int c) {
-            const uint32_t ok = at.bits<V::N>(c);
+    if (at.masked()) {
+        const auto keep = [&](c6_u32x4 &u, uint32_t ok) {
             float f[V::N];
             V::get(u, f);
 #pragma unroll
@@ -297,7 +339,7 @@ __device__ __forceinline__ Part part_of(Held<T, LANES, NV> &h, const Beside &at,
         };
 #pragma unroll
         for (int u = 0; u < NV; u++) {
-            if (h.has(u, lane)) keep(h.raw[u], u * LANES * V::N + lane * V::N);
+            if (h.has(u, lane)) keep(h.raw[u], at.template bits<V::N>(u, u * LANES * V::N + lane * V::N));
             unpack_again(h.raw[u]);
         }
         if (lane < h.rest && !at.legal(h.whole * V::N + lane)) h.tail = -INFINITY;
@@ -314,13 +356,13 @@ __device__ __forceinline__ Part part_of(Held<T, LANES, NV> &h, const Beside &at,
         p.w += q;
         if (q != 0.f) p.d += q * (base_of(p.m) - x);
     };
-    const auto sum = [&](const float (&f)[V::N], bool there, int c) {
+    const auto sum = [&](const float (&f)[V::N], bool there, int u, int c) {
         const float base = base_of(p.m);
 #pragma unroll
         for (int i = 0; i < V::N; i++) p.s += exp_of(f[i] - base);
         if (WEIGHTS && there) {
             float q[V::N];
-            at.get<V::N>(c, q);
+            at.template get<V::N>(u, c, q);
 #pragma unroll
             for (int i = 0; i < V::N; i++) weigh(f[i], q[i]);
         }
@@ -334,7 +376,7 @@ __device__ __forceinline__ Part part_of(Held<T, LANES, NV> &h, const Beside &at,
         for (int j = 0; j < GROUP; j++) m = fmaxf(m, take(h.raw[u + j], f[j]));
         p = from(p, m);
 #pragma unroll
-        for (int j = 0; j < GROUP; j++) sum(f[j], h.has(u + j, lane), (u + j) * LANES * V::N + lane * V::N);
+        for (int j = 0; j < GROUP; j++) sum(f[j], h.has(u + j, lane), u + j, (u + j) * LANES * V::N + lane * V::N);
 #pragma unroll
         for (int j = 0; j < GROUP; j++) unpack_again(h.raw[u + j]);
     }
@@ -361,16 +403,16 @@ __device__ __forceinline__ Done done(const Part &p, float scale) {
     k.scale = some ? scale : 0.f;
     return k;
 }
-template <typename T, bool WEIGHTS>
-__device__ __forceinline__ void gradient(const c6_u32x4 &u, const Beside &at, const Done &k, int index, int c, T *g) {
+template <typename T, bool WEIGHTS, typename At>
+__device__ __forceinline__ void gradient(const c6_u32x4 &raw, const At &at, const Done &k, int index, int u, int c, T *g) {
     typedef C6Vec<T> V;
     float f[V::N];
-    V::get(u, f);
+    V::get(raw, f);
 #pragma unroll
     for (int i = 0; i < V::N; i++) f[i] = k.factor * exp_of(f[i] - k.base);
     if (WEIGHTS) {
         float q[V::N];
-        at.get<V::N>(c, q);
+        at.template get<V::N>(u, c, q);
 #pragma unroll
         for (int i = 0; i < V::N; i++) f[i] -= k.scale * q[i];
     }
@@ -380,8 +422,8 @@ __device__ __forceinline__ void gradient(const c6_u32x4 &u, const Beside &at, co
     }
     V::store(g + c, V::put(f));
 }
-template <typename T, bool WEIGHTS>
-__device__ __forceinline__ void gradient(float x, const Beside &at, const Done &k, int index, int c, T *g) {
+template <typename T, bool WEIGHTS, typename At>
+__device__ __forceinline__ void gradient(float x, const At &at, const Done &k, int index, int c, T *g) {
     const float q = WEIGHTS ? at.get(c) : (c == index ? 1.f : 0.f);
     g[c] = c6_put<T>(k.factor * exp_of(x - k.base) - k.scale * q);
 }
@@ -402,13 +444,18 @@ __global__ __launch_bounds__(LANES == 64 ? 256 : LANES) void c6_policy_loss_kern
         int lane = threadIdx.x % LANES;
         asm volatile("" : "+v"(lane));      // (what follows from it is computed in every turn, not kept in registers across them)
         const T *x = (const T *)l.x + r * l.x_stride;
-        const Beside at = beside<WEIGHTS>(l, t, r, 0);
+        // what is beside a short row is fetched with it, beside a long one as it is needed
+        const auto at = [&] {
+            if constexpr (LANES == 64) return Fetched<T, LANES, NV, WEIGHTS>(beside<WEIGHTS>(l, t, r, 0), h, lane);
+            else return beside<WEIGHTS>(l, t, r, 0);
+        }();
         int index = -1;
         float played = 0.f;
-        if (!WEIGHTS) {
-            index = target_index(t, r, l.width);
-            if (index >= 0 && !legal(l, r, index)) index = -1;
-            if (index >= 0) played = c6_get(x[index]);
+        if (!WEIGHTS && l.width) {
+            const int i = target_index(t, r, l.width), there = max(i, 0);
+            const bool ok = legal(l, r, there);
+            played = c6_get(x[there]);
+            index = ok ? i : -1;
         }
         Part p = block_part<LANES>(part_of<T, LANES, NV, WEIGHTS>(h, at, lane), WEIGHTS, space[turn]);
         if (!WEIGHTS && index >= 0) { p.w = 1.f; p.d = p.m - played; }
@@ -419,7 +466,7 @@ __global__ __launch_bounds__(LANES == 64 ? 256 : LANES) void c6_policy_loss_kern
         T *g = grad + r * grad_stride;
 #pragma unroll
         for (int u = 0; u < NV; u++) {
-            if (grad && h.has(u, lane)) gradient<T, WEIGHTS>(h.raw[u], at, k, index, u * LANES * V::N + lane * V::N, g);
+            if (grad && h.has(u, lane)) gradient<T, WEIGHTS>(h.raw[u], at, k, index, u, u * LANES * V::N + lane * V::N, g);
             if (more) h.request(u, next, lane);
         }
         if (grad && lane < h.rest) gradient<T, WEIGHTS>(h.tail, at, k, index, h.whole * V::N + lane, g);
@@ -490,14 +537,14 @@ __global__ __launch_bounds__(256) void c6_policy_loss_join_kernel(Rows l, Target
             index = index < 0 ? -1 : index - v0;      // (of another chunk: outside this one's columns)
             const auto piece = [&](c6_u32x4 &u, int c) {
                 if (here.mask) {
-                    const uint32_t ok = here.bits<V::N>(c);
+                    const uint32_t ok = here.bits<V::N>(0, c);
                     float f[V::N];
                     V::get(u, f);
 #pragma unroll
                     for (int i = 0; i < V::N; i++) f[i] = ok >> i & 1 ? f[i] : -INFINITY;
                     u = V::put(f);
                 }
-                gradient<T, WEIGHTS>(u, here, k, index, c, g);
+                gradient<T, WEIGHTS>(u, here, k, index, 0, c, g);
             };
 #pragma unroll
             for (int u = 0; u < SPLIT_NV; u++)
