@@ -60,6 +60,22 @@ struct C6Vec {
         }
         return u;
     }
+    // elements whose bit of `ok` is clear become -infinity, in place: all ones or zeros for each bit (a signed bit field), then a bitwise select
+    static __device__ __forceinline__ uint32_t ones(uint32_t ok, int i) { return (uint32_t)((int32_t)(ok << (31 - i)) >> 31); }
+    static __device__ __forceinline__ void keep(c6_u32x4 &u, uint32_t ok) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            uint32_t m, fill;
+            if constexpr (sizeof(T) == 4) {
+                m = ones(ok, i);
+                fill = 0xff800000u;
+            } else {
+                m = (ones(ok, 2 * i) & 0xffffu) | (ones(ok, 2 * i + 1) & 0xffff0000u);
+                fill = __is_same(T, __bf16) ? 0xff80ff80u : 0xfc00fc00u;
+            }
+            u[i] = (u[i] & m) | (fill & ~m);
+        }
+    }
     // the first n of N elements (the end of a row); the rest reads as `fill`
     static __device__ __forceinline__ void get_some(const T *p, int n, float fill, float (&f)[N]) {
 #pragma unroll

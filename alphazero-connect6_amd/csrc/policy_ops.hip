@@ -191,34 +191,31 @@ __device__ __forceinline__ Part from(const Part &p, float M) {
     q.d = p.d + (p.w != 0.f && p.m != -INFINITY ? p.w * (M - p.m) : 0.f);      // (m = -infinity and w > 0: d is infinite already)
     return q;
 }
-__device__ __forceinline__ Part wave_part(const Part &p, bool weights) {
-    Part q = from(p, c6_wave_max(p.m));
-    q.s = c6_wave_sum(q.s);
+// over the lanes of a row of 16 (WIDE = false) or of the wave, the same in all of them
+template <bool WIDE>
+__device__ __forceinline__ Part lanes_part(const Part &p, bool weights) {
+    const auto top = [](float a, float b) { return fmaxf(a, b); };
+    const auto add = [](float a, float b) { return a + b; };
+    const auto all = [](float v, auto f) { return WIDE ? c6_wave_all(v, f) : c6_row_all(v, f); };
+    Part q = from(p, all(p.m, top));
+    q.s = all(q.s, add);
     if (weights) {
-        q.w = c6_wave_sum(q.w);
-        q.d = c6_wave_sum(q.d);
+        q.w = all(q.w, add);
+        q.d = all(q.d, add);
     }
     return q;
 }
-// over the waves of a workgroup, the same in every thread; `space`: one Part a wave, not in use by an earlier call that some wave may still read
+// over the lanes that share a row, the same in all of them; `space`: one Part a wave, not in use by an earlier call that some wave may still read
 template <int LANES>
 __device__ __forceinline__ Part block_part(const Part &p, bool weights, Part *space) {
-    Part q = wave_part(p, weights);
+    if (LANES == 16) return lanes_part<false>(p, weights);
+    const Part q = lanes_part<true>(p, weights);
     if (LANES == 64) return q;
     if ((threadIdx.x & 63) == 0) space[threadIdx.x >> 6] = q;
     __syncthreads();
-    // every row of 16 lanes takes all the waves' Parts, one a lane
+    static_assert(LANES / 64 <= 16, "one lane of a row of 16 for each wave");
     const int i = threadIdx.x & 15;
-    static_assert(LANES / 64 <= 16, "one lane of a row for each wave");
-    q = i < LANES / 64 ? space[i] : Part{-INFINITY, 0.f, 0.f, 0.f};
-    const auto add = [](float a, float b) { return a + b; };
-    q = from(q, c6_row_all(q.m, [](float a, float b) { return fmaxf(a, b); }));
-    q.s = c6_row_all(q.s, add);
-    if (weights) {
-        q.w = c6_row_all(q.w, add);
-        q.d = c6_row_all(q.d, add);
-    }
-    return q;
+    return lanes_part<false>(i < LANES / 64 ? space[i] : Part{-INFINITY, 0.f, 0.f, 0.f}, weights);
 }
 
 // A row (or a chunk of one) in the registers of LANES lanes, in pieces of N entries (16 bytes): lane i holds the pieces i, i + LANES, ...; of the entries
@@ -226,6 +223,7 @@ __device__ __forceinline__ Part block_part(const Part &p, bool weights, Part *sp
 template <typename T, int LANES, int NV>
 struct Held {
     typedef C6Vec<T> V;
+    static constexpr int PIECES = NV;
     c6_u32x4 raw[NV];
     float tail;
     int whole, rest;       // whole pieces, entries behind them
@@ -238,6 +236,7 @@ struct Held {
         for (int u = 0; u < NV; u++) raw[u] = V::put(f);
     }
     __device__ __forceinline__ bool has(int u, int lane) const { return lane < whole - u * LANES; }
+    __device__ __forceinline__ int column(int u, int lane) const { return (u * LANES + lane) * V::N; }
     __device__ __forceinline__ void request(int u, const T *x, int lane) {
         if (has(u, lane)) raw[u] = V::load(x + u * LANES * V::N + lane * V::N);
     }
@@ -261,7 +260,6 @@ struct Beside {
     int64_t byte;
     template <int N>
     __device__ __forceinline__ uint32_t bits(int, int c) const { return mask ? (uint32_t)mask[(int64_t)(c >> 3) * byte] >> (N == 4 ? c & 4 : 0) : ~0u; }
-    __device__ __forceinline__ bool masked() const { return mask; }
     __device__ __forceinline__ bool legal(int c) const { return !mask || (mask[(int64_t)(c >> 3) * byte] >> (c & 7) & 1); }
     // weights: 0 where illegal
     template <int N>
@@ -272,10 +270,20 @@ struct Beside {
             float f[4];
             C6Vec<float>::get(C6Vec<float>::load(weights + c + i), f);
 #pragma unroll
-            for (int j = 0; j < 4; j++) q[i + j] = ok >> (i + j) & 1 ? f[j] : 0.f;
+            for (int j = 0; j < 4; j++) q[i + j] = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, f[j]) & C6Vec<float>::ones(ok, i + j));
         }
     }
     __device__ __forceinline__ float get(int c) const { return legal(c) ? weights[c] : 0.f; }
+    template <typename H>
+    __device__ __forceinline__ void settle(H &h, int lane) {
+        if (!mask) return;
+#pragma unroll
+        for (int u = 0; u < H::PIECES; u++) {
+            if (h.has(u, lane)) H::V::keep(h.raw[u], bits<H::V::N>(u, h.column(u, lane)));
+            unpack_again(h.raw[u]);
+        }
+        if (lane < h.rest && !legal(h.whole * H::V::N + lane)) h.tail = -INFINITY;
+    }
 };
 // ... requested all at once and held: a wave with a short row waits for memory once
 template <typename T, int LANES, int NV, bool WEIGHTS>
@@ -303,21 +311,27 @@ struct Fetched {
             if (WEIGHTS) tail_w = at.weights[c];
         }
     }
-    __device__ __forceinline__ bool masked() const { return any; }
-    template <int M>
-    __device__ __forceinline__ uint32_t bits(int u, int) const { return ok[u]; }
-    __device__ __forceinline__ bool legal(int) const { return tail_ok; }
+    // the mask goes into the row and its weights, once
+    __device__ __forceinline__ void settle(Held<T, LANES, NV> &h, int) {
+        if (!any) return;
+#pragma unroll
+        for (int u = 0; u < NV; u++) {
+            C6Vec<T>::keep(h.raw[u], ok[u]);
+            if constexpr (WEIGHTS)
+#pragma unroll
+                for (int i = 0; i < N; i++) w[u][i / 4][i % 4] &= C6Vec<T>::ones(ok[u], i);
+        }
+        if (!tail_ok) { h.tail = -INFINITY; tail_w = 0.f; }
+    }
     template <int M>
     __device__ __forceinline__ void get(int u, int, float (&q)[M]) const {
 #pragma unroll
-        for (int i = 0; i < N; i += 4) {
-            float f[4];
-            C6Vec<float>::get(w[WEIGHTS ? u : 0][i / 4], f);
-#pragma unroll
-            for (int j = 0; j < 4; j++) q[i + j] = ok[u] >> (i + j) & 1 ? f[j] : 0.f;
+        for (int i = 0; i < N; i++) {
+            const uint32_t word = w[WEIGHTS ? u : 0][i / 4][i % 4];
+            q[i] = __builtin_bit_cast(float, word);
         }
     }
-    __device__ __forceinline__ float get(int) const { return tail_ok ? tail_w : 0.f; }
+    __device__ __forceinline__ float get(int) const { return tail_w; }
 };
 
 template <bool WEIGHTS>
@@ -326,24 +340,10 @@ __device__ __forceinline__ Beside beside(const Rows &l, const Target &t, int64_t
 }
 
 template <typename T, int LANES, int NV, bool WEIGHTS, typename At>
-__device__ __forceinline__ Part part_of(Held<T, LANES, NV> &h, const At &at, int lane) {
+__device__ __forceinline__ Part part_of(Held<T, LANES, NV> &h, At &at, int lane) {
     typedef C6Vec<T> V;
     Part p{-INFINITY, 0.f, 0.f, 0.f};
-    if (at.masked()) {
-        const auto keep = [&](c6_u32x4 &u, uint32_t ok) {
-            float f[V::N];
-            V::get(u, f);
-#pragma unroll
-            for (int i = 0; i < V::N; i++) f[i] = ok >> i & 1 ? f[i] : -INFINITY;
-            u = V::put(f);
-        };
-#pragma unroll
-        for (int u = 0; u < NV; u++) {
-            if (h.has(u, lane)) keep(h.raw[u], at.template bits<V::N>(u, u * LANES * V::N + lane * V::N));
-            unpack_again(h.raw[u]);
-        }
-        if (lane < h.rest && !at.legal(h.whole * V::N + lane)) h.tail = -INFINITY;
-    }
+    at.settle(h, lane);
     // some pieces' maximum, then their sums relative to the greatest so far: they need no piece that comes later, which may still be on its way
     const auto take = [&](const c6_u32x4 &u, float (&f)[V::N]) {
         V::get(u, f);
@@ -352,22 +352,27 @@ __device__ __forceinline__ Part part_of(Held<T, LANES, NV> &h, const At &at, int
         for (int i = 1; i < V::N; i++) m = fmaxf(m, f[i]);
         return m;
     };
-    const auto weigh = [&](float x, float q) {
+    // a = x - base: -infinity against a weight of 0 is nothing
+    const auto weigh = [&](float a, float q) {
         p.w += q;
-        if (q != 0.f) p.d += q * (base_of(p.m) - x);
+        p.d = __builtin_fmaf(q, q != 0.f ? -a : 0.f, p.d);
     };
     const auto sum = [&](const float (&f)[V::N], bool there, int u, int c) {
         const float base = base_of(p.m);
+        float a[V::N];
 #pragma unroll
-        for (int i = 0; i < V::N; i++) p.s += exp_of(f[i] - base);
+        for (int i = 0; i < V::N; i++) {
+            a[i] = f[i] - base;
+            p.s += exp_of(a[i]);
+        }
         if (WEIGHTS && there) {
             float q[V::N];
             at.template get<V::N>(u, c, q);
 #pragma unroll
-            for (int i = 0; i < V::N; i++) weigh(f[i], q[i]);
+            for (int i = 0; i < V::N; i++) weigh(a[i], q[i]);
         }
     };
-    constexpr int GROUP = NV < 16 / V::N ? NV : 16 / V::N;
+    constexpr int GROUP = NV % (16 / V::N) ? NV : 16 / V::N;      // 16 entries, in short rows all
     static_assert(NV % GROUP == 0, "whole groups of pieces");
 #pragma unroll
     for (int u = 0; u < NV; u += GROUP) {
@@ -376,14 +381,15 @@ __device__ __forceinline__ Part part_of(Held<T, LANES, NV> &h, const At &at, int
         for (int j = 0; j < GROUP; j++) m = fmaxf(m, take(h.raw[u + j], f[j]));
         p = from(p, m);
 #pragma unroll
-        for (int j = 0; j < GROUP; j++) sum(f[j], h.has(u + j, lane), u + j, (u + j) * LANES * V::N + lane * V::N);
+        for (int j = 0; j < GROUP; j++) sum(f[j], h.has(u + j, lane), u + j, h.column(u + j, lane));
 #pragma unroll
         for (int j = 0; j < GROUP; j++) unpack_again(h.raw[u + j]);
     }
     if (h.rest) {
         p = from(p, fmaxf(p.m, h.tail));
-        p.s += exp_of(h.tail - base_of(p.m));
-        if (WEIGHTS && lane < h.rest) weigh(h.tail, at.get(h.whole * V::N + lane));
+        const float a = h.tail - base_of(p.m);
+        p.s += exp_of(a);
+        if (WEIGHTS && lane < h.rest) weigh(a, at.get(h.whole * V::N + lane));
     }
     return p;
 }
@@ -414,7 +420,7 @@ __device__ __forceinline__ void gradient(const c6_u32x4 &raw, const At &at, cons
         float q[V::N];
         at.template get<V::N>(u, c, q);
 #pragma unroll
-        for (int i = 0; i < V::N; i++) f[i] -= k.scale * q[i];
+        for (int i = 0; i < V::N; i++) f[i] = __builtin_fmaf(-k.scale, q[i], f[i]);
     }
     if (!WEIGHTS && (unsigned)(index - c) < (unsigned)V::N) {
 #pragma unroll
@@ -432,12 +438,12 @@ __device__ __forceinline__ void gradient(float x, const At &at, const Done &k, i
 // relative to that, and one reduction over the lanes joins them.  As a piece's gradient leaves, the same piece of the workgroup's next row is requested
 // into its registers: loads and stores overlap, and the sums of a row begin as its first pieces arrive.
 template <typename T, int LANES, int NV, bool WEIGHTS>
-__global__ __launch_bounds__(LANES == 64 ? 256 : LANES) void c6_policy_loss_kernel(Rows l, Target t, float *loss, float *lse, float *total, T *grad, int64_t grad_stride, float scale) {
+__global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void c6_policy_loss_kernel(Rows l, Target t, float *loss, float *lse, float *total, T *grad, int64_t grad_stride, float scale) {
     typedef C6Vec<T> V;
-    constexpr int PER = LANES == 64 ? 4 : 1;
-    __shared__ Part space[2][LANES / 64];
+    constexpr int PER = LANES < 256 ? 256 / LANES : 1;
+    __shared__ Part space[2][LANES < 64 ? 1 : LANES / 64];
     const int64_t step = (int64_t)gridDim.x * PER;
-    int64_t r = (int64_t)blockIdx.x * PER + (LANES == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
+    int64_t r = (int64_t)blockIdx.x * PER + (LANES == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : LANES == 16 ? threadIdx.x >> 4 : 0);
     Held<T, LANES, NV> h(l.width);
     if (r < l.rows) h.request((const T *)l.x + r * l.x_stride, threadIdx.x % LANES);
     for (int turn = 0; r < l.rows; r += step, turn ^= 1) {
@@ -445,8 +451,8 @@ __global__ __launch_bounds__(LANES == 64 ? 256 : LANES) void c6_policy_loss_kern
         asm volatile("" : "+v"(lane));      // (what follows from it is computed in every turn, not kept in registers across them)
         const T *x = (const T *)l.x + r * l.x_stride;
         // what is beside a short row is fetched with it, beside a long one as it is needed
-        const auto at = [&] {
-            if constexpr (LANES == 64) return Fetched<T, LANES, NV, WEIGHTS>(beside<WEIGHTS>(l, t, r, 0), h, lane);
+        auto at = [&] {
+            if constexpr (LANES <= 64) return Fetched<T, LANES, NV, WEIGHTS>(beside<WEIGHTS>(l, t, r, 0), h, lane);
             else return beside<WEIGHTS>(l, t, r, 0);
         }();
         int index = -1;
@@ -466,7 +472,7 @@ __global__ __launch_bounds__(LANES == 64 ? 256 : LANES) void c6_policy_loss_kern
         T *g = grad + r * grad_stride;
 #pragma unroll
         for (int u = 0; u < NV; u++) {
-            if (grad && h.has(u, lane)) gradient<T, WEIGHTS>(h.raw[u], at, k, index, u, u * LANES * V::N + lane * V::N, g);
+            if (grad && h.has(u, lane)) gradient<T, WEIGHTS>(h.raw[u], at, k, index, u, h.column(u, lane), g);
             if (more) h.request(u, next, lane);
         }
         if (grad && lane < h.rest) gradient<T, WEIGHTS>(h.tail, at, k, index, h.whole * V::N + lane, g);
@@ -491,7 +497,8 @@ __global__ __launch_bounds__(256) void c6_policy_loss_part_kernel(Rows l, Target
         const T *x = (const T *)l.x + r * l.x_stride;
         Held<T, 256, SPLIT_NV> h(min(l.width - v0, split_chunk<T>));
         h.request(x + v0, lane);
-        const Part p = block_part<256>(part_of<T, 256, SPLIT_NV, WEIGHTS>(h, beside<WEIGHTS>(l, t, r, v0), lane), WEIGHTS, space);
+        Beside here = beside<WEIGHTS>(l, t, r, v0);
+        const Part p = block_part<256>(part_of<T, 256, SPLIT_NV, WEIGHTS>(h, here, lane), WEIGHTS, space);
         if (lane == 0) parts[item] = p;
         if (!WEIGHTS && lane == 0) {      // (the gradient may go where x is: the second launch does not read the entry again)
             const int index = target_index(t, r, l.width);
@@ -532,27 +539,14 @@ __global__ __launch_bounds__(256) void c6_policy_loss_join_kernel(Rows l, Target
         const Done k = done(p, scale);
         if (v0 == 0 && lane == 0) { loss[r] = k.loss; lse[r] = k.lse; total[r] = k.total; }
         if (grad) {
-            const Beside here = beside<WEIGHTS>(l, t, r, v0);
+            Beside here = beside<WEIGHTS>(l, t, r, v0);
             T *g = grad + r * grad_stride + v0;
             index = index < 0 ? -1 : index - v0;      // (of another chunk: outside this one's columns)
-            const auto piece = [&](c6_u32x4 &u, int c) {
-                if (here.mask) {
-                    const uint32_t ok = here.bits<V::N>(0, c);
-                    float f[V::N];
-                    V::get(u, f);
-#pragma unroll
-                    for (int i = 0; i < V::N; i++) f[i] = ok >> i & 1 ? f[i] : -INFINITY;
-                    u = V::put(f);
-                }
-                gradient<T, WEIGHTS>(u, here, k, index, 0, c, g);
-            };
+            here.settle(h, lane);
 #pragma unroll
             for (int u = 0; u < SPLIT_NV; u++)
-                if (h.has(u, lane)) piece(h.raw[u], (u * 256 + lane) * V::N);
-            if (lane < h.rest) {
-                const int c = h.whole * V::N + lane;
-                gradient<T, WEIGHTS>(here.legal(c) ? h.tail : -INFINITY, here, k, index, c, g);
-            }
+                if (h.has(u, lane)) gradient<T, WEIGHTS>(h.raw[u], here, k, index, u, h.column(u, lane), g);
+            if (lane < h.rest) gradient<T, WEIGHTS>(h.tail, here, k, index, h.whole * V::N + lane, g);
         }
         __syncthreads();
     }
@@ -733,6 +727,9 @@ extern "C" size_t c6_policy_loss_workspace(int rows, int width) {
     return need;
 }
 
+#ifndef MANY
+#define MANY 4096
+#endif
 template <typename T, bool WEIGHTS>
 static void loss_launch(const c6_logits *l, const Target &t, float *loss, float *lse, float *total, T *grad, int64_t grad_stride, float scale, void *workspace, hipStream_t s) {
     constexpr int N = C6Vec<T>::N;
@@ -747,11 +744,17 @@ static void loss_launch(const c6_logits *l, const Target &t, float *loss, float 
                            total, grad, grad_stride, scale);
         return;
     }
-#define C6_LAUNCH(LANES, NV, RESIDENT)                                                                                                                                      \
-    hipLaunchKernelGGL((c6_policy_loss_kernel<T, LANES, NV, WEIGHTS>), dim3((unsigned)std::min<int64_t>(LANES == 64 ? ((int64_t)l->rows + 3) / 4 : l->rows, (int64_t)cus() * RESIDENT)), \
-                       dim3(LANES == 64 ? 256 : LANES), 0, s, rows, t, loss, lse, total, grad, grad_stride, scale)
+#define C6_LAUNCH(LANES, NV, RESIDENT)                                                                                                                                       \
+    hipLaunchKernelGGL((c6_policy_loss_kernel<T, LANES, NV, WEIGHTS>),                                                                                                       \
+                       dim3((unsigned)std::min<int64_t>(LANES < 256 ? ((int64_t)l->rows * LANES + 255) / 256 : l->rows, (int64_t)cus() * RESIDENT)), dim3(LANES < 256 ? 256 : LANES), 0, s, \
+                       rows, t, loss, lse, total, grad, grad_stride, scale)
     const int pieces = (l->width + N - 1) / N;
-    if (pieces <= 64) C6_LAUNCH(64, 1, 1 << 14);
+    const bool many = l->rows >= MANY;
+    if (many && pieces <= 32) C6_LAUNCH(16, 2, 1 << 14);
+    else if (many && pieces <= 48) C6_LAUNCH(16, 3, 1 << 14);
+    else if (many && pieces <= 64) C6_LAUNCH(16, 4, 1 << 14);
+    else if (many && pieces <= 96) C6_LAUNCH(16, 6, 1 << 14);
+    else if (pieces <= 64) C6_LAUNCH(64, 1, 1 << 14);
     else if (pieces <= 128) C6_LAUNCH(64, 2, 1 << 14);
     else if (pieces <= 256) C6_LAUNCH(64, 4, 1 << 14);
     else if (pieces <= 512) C6_LAUNCH(256, 2, 1 << 14);
