@@ -29,6 +29,7 @@ PREC_DEFAULT, PREC_FP32, PREC_BF16X3, PREC_BF16 = 0, 1, 3, 4      # PREC_BF16: r
 PREC_F16F8 = 5      # opt-in: fp16 main term + MX-fp8 cross terms, bounded range (guarded: C6_ERR_RANGE)
 PREC_FP32_DIRECT = 6
 ERR_OVERFLOW, ERR_RANGE = 3, 7
+POLICY_LOSS_REFERENCE, POLICY_LOSS_LEGAL, POLICY_LOSS_VISITS = 0, 1, 2      # Trainer.set_policy_loss
 REF_N = 15
 
 DROPIN_SYMBOLS = ["cpp_play", "cpp_self_play", "cpp_play_with", "test_new_raw_path", "test_with_raw_path",
@@ -53,7 +54,8 @@ ENGINE_SYMBOLS = ["c6_last_error", "c6_version", "c6_rng_spec", "c6_device_count
                   "c6_group_fetch_games", "c6_group_enable_tuples", "c6_group_pool_begin", "c6_group_pool_end", "c6_group_pool_tuples",
                   "c6_group_pooled", "c6_group_fetch_pooled", "c6_group_push_pooled",
                   "c6_logits_process", "c6_policy_loss_workspace", "c6_policy_loss", "c6_policy_loss_grad", "c6_clip_create", "c6_clip_destroy",
-                  "c6_clip_workspace", "c6_clip_norm", "c6_clip_apply"]
+                  "c6_clip_workspace", "c6_clip_norm", "c6_clip_apply", "c6_trainer_set_policy_loss", "c6_trainer_set_clip", "c6_trainer_grad_norm",
+                  "c6_replay_sample_device_pi"]
 
 
 class C6Error(RuntimeError):
@@ -255,6 +257,9 @@ def lib():
         L.c6_clip_workspace.argtypes = [vp]
         L.c6_clip_workspace.restype = C.c_size_t
         L.c6_clip_norm.argtypes = [vp, vp, vp, C.c_size_t, vp]
+        L.c6_trainer_set_policy_loss.argtypes = [vp, C.c_int]
+        L.c6_trainer_set_clip.argtypes = [vp, C.c_float]
+        L.c6_trainer_grad_norm.argtypes = [vp, f32p]
         L.c6_clip_apply.argtypes = [vp, C.c_float, vp, vp, C.c_size_t, vp]
     L.cpp_self_play.restype = Vec
     L.cpp_self_play.argtypes = [CALLBACK, ALLOC_PATH, ALLOC_RESULT, C.c_int, C.c_float, C.c_double, C.c_float, C.c_bool, C.c_int]
@@ -862,6 +867,7 @@ class Trainer:
         (the same arithmetic on the direct kernels), PREC_BF16X3 (split-bf16 products: the fast option, gradients within ~1e-3)"""
         self.n, self.cells, self.C, self.blocks, self.batch = board_size, board_size * board_size, channels, blocks, batch
         self.nfloats = lib().c6_net_blob_floats(board_size, channels, blocks)
+        self.policy_loss = POLICY_LOSS_REFERENCE
         self.h = C.c_void_p()
         _chk(lib().c6_trainer_create(board_size, channels, blocks, batch, lr, momentum, device, C.byref(self.h)))
         _chk(lib().c6_trainer_set_precision(self.h, precision))
@@ -888,12 +894,28 @@ class Trainer:
         _chk(lib().c6_trainer_gradients(self.h, _p(b, C.c_float), b.size))
         return b
 
+    def set_policy_loss(self, kind):
+        """POLICY_LOSS_REFERENCE (softmax over all cells, the reference's loss), _LEGAL (cross entropy of the move over the empty cells) or _VISITS (against
+        the search's visit counts: `poses` of step / loss is then ReplayBuffer.sample(want_pi=True)'s pi [batch, N*N]; step_replay draws it itself)"""
+        _chk(lib().c6_trainer_set_policy_loss(self.h, kind))
+        self.policy_loss = kind
+
+    def set_clip(self, max_norm):
+        """clip the gradients of every step to a global norm of max_norm before SGD; None: no clipping"""
+        _chk(lib().c6_trainer_set_clip(self.h, -1.0 if max_norm is None else max_norm))
+
+    def grad_norm(self):
+        """the global gradient norm of the last step, before it was clipped"""
+        v = C.c_float()
+        _chk(lib().c6_trainer_grad_norm(self.h, C.byref(v)))
+        return v.value
+
     def _batch(self, winners, players, boards, poses):
         w = np.ascontiguousarray(winners, dtype=np.float32).reshape(-1)
         p = np.ascontiguousarray(players, dtype=np.float32).reshape(-1)
         b = np.ascontiguousarray(boards, dtype=np.float32).reshape(-1)
         q = np.ascontiguousarray(poses, dtype=np.float32).reshape(-1)
-        if not (w.size == p.size == q.size == self.batch and b.size == self.batch * self.cells):
+        if not (w.size == p.size == self.batch and q.size == self.batch * (self.cells if self.policy_loss == POLICY_LOSS_VISITS else 1) and b.size == self.batch * self.cells):
             raise C6Error("batch shapes do not match the trainer's mini-batch size")
         return w, p, b, q
 

@@ -44,3 +44,7 @@ void c6t_sgd(size_t n, float lr, float momentum, int first, const unsigned char 
 int c6t_wgrad_splits(int C, int B);
 size_t c6t_wgrad_partial_floats(int C, int B);
 bool c6t_wgrad(int N, int C, int B, const float *dy, const float *x, float *partial, float *dw, hipStream_t s, int split_bf16 = 0);
+
+// what c6_policy_loss takes, from a batch (policy_ops.hip): mask [B][(cells + 7) / 8] of the empty cells and, from poses [B], the moves as indices, or, from
+// visits [B][cells], weights of sum 1 over the empty cells (0 where there are no visits)
+void c6t_policy_targets(int B, int cells, const float *boards, const float *poses, const float *visits, unsigned char *mask, int *index, float *weights, hipStream_t s);

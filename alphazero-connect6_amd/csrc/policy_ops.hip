@@ -1,6 +1,7 @@
 // policy_ops.hip -- what a policy's logits go through before a move is chosen, and the loss they are trained on
 // (include/connect6_amd.h part 7): penalties / biases / masks, cross entropy over the legal entries, and its gradient.
 #include "c6_ops.h"
+#include "c6_train.h"
 
 #include <algorithm>
 
@@ -812,4 +813,28 @@ extern "C" int c6_policy_loss_grad(const c6_logits *l, const void *target, int t
     else C6_LAUNCH(256, false);
 #undef C6_LAUNCH
     return launched();
+}
+
+// The trainer's batch in the operator's terms; a wave a position.
+__global__ __launch_bounds__(256) void c6t_policy_targets_kernel(int B, int cells, const float *boards, const float *poses, const float *visits, uint8_t *mask, int *index,
+                                                                 float *weights) {
+    const int lane = threadIdx.x & 63, b = blockIdx.x * 4 + (threadIdx.x >> 6), bytes = (cells + 7) / 8;
+    if (b >= B) return;
+    float sum = 0.f;
+    for (int v0 = 0; v0 < cells; v0 += 64) {
+        const int v = v0 + lane;
+        const bool empty = v < cells && boards[(size_t)b * cells + v] == 0.f;
+        const uint64_t bits = __ballot(empty);
+        if (lane < 8 && v0 / 8 + lane < bytes) mask[(size_t)b * bytes + v0 / 8 + lane] = (uint8_t)(bits >> (8 * lane));
+        if (visits && empty) sum += visits[(size_t)b * cells + v];
+    }
+    if (!visits) {
+        if (lane == 0) index[b] = (int)poses[b];
+        return;
+    }
+    sum = c6_wave_sum(sum);
+    for (int v = lane; v < cells; v += 64) weights[(size_t)b * cells + v] = sum > 0.f ? visits[(size_t)b * cells + v] / sum : 0.f;
+}
+void c6t_policy_targets(int B, int cells, const float *boards, const float *poses, const float *visits, unsigned char *mask, int *index, float *weights, hipStream_t s) {
+    hipLaunchKernelGGL(c6t_policy_targets_kernel, dim3((B + 3) / 4), dim3(256), 0, s, B, cells, boards, poses, visits, mask, index, weights);
 }

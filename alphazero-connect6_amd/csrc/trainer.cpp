@@ -65,6 +65,15 @@ struct c6_trainer {
     float *wpack32 = nullptr;
     float *wpackw = nullptr, *vbuf = nullptr;      // FP32 at 256 channels: Winograd F(4x4) (conv_wino4.hip), transformed weights + its scratch
     float *wgpart = nullptr;                        // ... and the partial sums of its weight gradient
+    // the policy's loss over the empty cells (c6_policy_loss) and clipping (c6_clip): made when they are asked for
+    int policy_loss = C6_POLICY_LOSS_REFERENCE;
+    unsigned char *legal = nullptr;
+    int *move = nullptr;
+    float *visits = nullptr, *weights = nullptr, *row_stats = nullptr;
+    float clip = -1.f, *norm = nullptr;
+    double *clip_space = nullptr;
+    c6_clip *clipper = nullptr;
+    bool clipped = false;
     std::vector<float *> vkeep;                     // ... and every layer's transformed input, kept from the forward pass for the weight gradient
 };
 
@@ -172,6 +181,7 @@ extern "C" void c6_trainer_destroy(c6_trainer *t) {
     if (!t) return;
     hipSetDevice(t->device);
     hipStreamSynchronize(t->stream);
+    c6_clip_destroy(t->clipper);
     for (void *p : t->allocs) hipFree(p);
     hipStreamDestroy(t->stream);
     delete t;
@@ -277,7 +287,16 @@ static int forward_loss(c6_trainer *t, bool want_grad_seed) {
     c6t_policy_bn_apply(R, n2, t->yp, t->pmean, t->pvar, P + t->pn.g, P + t->pn.be, t->hp, s);
     c6t_bn_running(2, R, t->pmean, t->pvar, P + t->pn.rm, P + t->pn.rv, s);
     c6t_gemm(B, n2, 2 * n2, t->hp, 2 * n2, 1, P + t->pl_w, 1, 2 * n2, P + t->pl_b, t->logits, n2, 0, s);      // hp x Wl^T + bl
-    c6t_softmax_loss(B, n2, t->logits, t->poses, t->prob, t->lossp, t->dlogits, s);
+    if (t->policy_loss == C6_POLICY_LOSS_REFERENCE) {
+        c6t_softmax_loss(B, n2, t->logits, t->poses, t->prob, t->lossp, t->dlogits, s);
+    } else {
+        const bool visits = t->policy_loss == C6_POLICY_LOSS_VISITS;
+        c6t_policy_targets(B, n2, t->boards, t->poses, visits ? t->visits : nullptr, t->legal, t->move, t->weights, s);
+        const c6_logits l = {B, n2, C6_TYPE_F32, t->device, t->logits, n2, t->legal, (n2 + 7) / 8, 1};
+        const int rc = c6_policy_loss(&l, visits ? (const void *)t->weights : t->move, visits ? C6_TARGET_WEIGHTS : C6_TARGET_INDEX32, n2, t->lossp, t->row_stats,
+                                      t->row_stats + B, t->dlogits, n2, 1.0f / (float)B, nullptr, 0, s);      // (a board's row needs no workspace)
+        if (rc) return tfail(rc, c6_last_error());
+    }
     c6t_colstats(0, (size_t)B, n2, t->yv, nullptr, nullptr, nullptr, nullptr, t->partial, t->vmean, t->vvar, s);   // BatchNorm1d over the batch
     c6t_bn_apply((size_t)B, n2, t->yv, t->vmean, t->vvar, P + t->vn.g, P + t->vn.be, nullptr, t->hv, 1, s);
     c6t_bn_running(n2, (size_t)B, t->vmean, t->vvar, P + t->vn.rm, P + t->vn.rv, s);
@@ -354,13 +373,18 @@ static int backward(c6_trainer *t) {
 static int upload_batch(c6_trainer *t, const float *winners, const float *players, const float *boards, const float *poses, int on_device) {
     if (!winners || !players || !boards || !poses) return tfail(C6_ERR_BAD_ARG, "trainer: NULL batch pointer");
     const hipMemcpyKind kind = on_device ? hipMemcpyDeviceToDevice : hipMemcpyHostToDevice;
-    if (!on_device)
+    const bool visits = t->policy_loss == C6_POLICY_LOSS_VISITS;
+    if (!on_device && visits) {
+        for (size_t i = 0; i < (size_t)t->B * t->cells; i++)
+            if (!(poses[i] >= 0.f && poses[i] <= 3.402823466e38f)) return tfail(C6_ERR_BAD_ARG, "trainer: visit counts are finite and not negative");
+    } else if (!on_device)
         for (int i = 0; i < t->B; i++)
             if (!(poses[i] >= 0.f && poses[i] < (float)t->cells)) return tfail(C6_ERR_BAD_ARG, "trainer: position outside the board");
     TCHK(hipMemcpyAsync(t->winners, winners, (size_t)t->B * 4, kind, t->stream));
     TCHK(hipMemcpyAsync(t->players, players, (size_t)t->B * 4, kind, t->stream));
     TCHK(hipMemcpyAsync(t->boards, boards, (size_t)t->B * t->cells * 4, kind, t->stream));
-    TCHK(hipMemcpyAsync(t->poses, poses, (size_t)t->B * 4, kind, t->stream));
+    if (visits) TCHK(hipMemcpyAsync(t->visits, poses, (size_t)t->B * t->cells * 4, kind, t->stream));
+    else TCHK(hipMemcpyAsync(t->poses, poses, (size_t)t->B * 4, kind, t->stream));
     return C6_OK;
 }
 
@@ -379,6 +403,11 @@ static int step_resident(c6_trainer *t, float *loss_out) {
     TCHK(hipMemsetAsync(t->G, 0, t->nfloats * sizeof(float), t->stream));       // optimizer.zero_grad()
     rc = backward(t);
     if (rc) return rc;
+    if (t->clip >= 0.f) {      // (the running statistics in the blob have no gradient: they add nothing to the norm)
+        rc = c6_clip_apply(t->clipper, t->clip, t->norm, t->clip_space, c6_clip_workspace(t->clipper), t->stream);
+        if (rc) return tfail(rc, c6_last_error());
+    }
+    t->clipped = t->clip >= 0.f;
     c6t_sgd(t->nfloats, t->lr, t->momentum, t->steps == 0, t->mask, t->G, t->M, t->P, t->stream);
     t->steps++;
     return read_loss(t, loss_out);
@@ -406,14 +435,12 @@ extern "C" int c6_trainer_loss(c6_trainer *t, const float *winners, const float 
 
 // sample a mini-batch from the device-resident replay buffer and train on it: ReplayBuffer::sample -> loss -> step without
 // a host round trip (main.cpp:151-157)
-extern "C" int c6_replay_sample_device(c6_replay *r, int num_sample, uint64_t seed, uint32_t draw_id, float *winners, float *players,
-                                       float *boards, float *poses, void *stream);
-extern "C" int c6_replay_board_size(const c6_replay *r);
 extern "C" int c6_trainer_step_replay(c6_trainer *t, c6_replay *r, uint64_t seed, uint32_t draw_id, float *loss_out) {
     if (!t || !r) return tfail(C6_ERR_BAD_ARG, "c6_trainer_step_replay: NULL argument");
     if (c6_replay_board_size(r) != t->n) return tfail(C6_ERR_BAD_ARG, "c6_trainer_step_replay: board size mismatch");
     TCHK(hipSetDevice(t->device));
-    int rc = c6_replay_sample_device(r, t->B, seed, draw_id, t->winners, t->players, t->boards, t->poses, t->stream);
+    int rc = c6_replay_sample_device_pi(r, t->B, seed, draw_id, t->winners, t->players, t->boards, t->poses,
+                                        t->policy_loss == C6_POLICY_LOSS_VISITS ? t->visits : nullptr, t->stream);
     if (rc) return rc;
     return step_resident(t, loss_out);
 }
@@ -421,6 +448,56 @@ extern "C" int c6_trainer_step_replay(c6_trainer *t, c6_replay *r, uint64_t seed
 extern "C" int c6_trainer_set_lr(c6_trainer *t, float lr, float momentum) {
     if (!t) return tfail(C6_ERR_BAD_ARG, "c6_trainer_set_lr: NULL trainer");
     t->lr = lr; t->momentum = momentum;
+    return C6_OK;
+}
+
+extern "C" int c6_trainer_set_policy_loss(c6_trainer *t, int kind) {
+    if (!t) return tfail(C6_ERR_BAD_ARG, "c6_trainer_set_policy_loss: NULL trainer");
+    if (kind != C6_POLICY_LOSS_REFERENCE && kind != C6_POLICY_LOSS_LEGAL && kind != C6_POLICY_LOSS_VISITS)
+        return tfail(C6_ERR_BAD_ARG, "c6_trainer_set_policy_loss: C6_POLICY_LOSS_REFERENCE, C6_POLICY_LOSS_LEGAL or C6_POLICY_LOSS_VISITS");
+    TCHK(hipSetDevice(t->device));
+    const size_t B = t->B, n2 = t->cells;
+    int rc = C6_OK;
+    if (kind != C6_POLICY_LOSS_REFERENCE && !t->row_stats) {
+        rc = talloc(t, &t->legal, B * ((n2 + 7) / 8));
+        if (!rc) rc = talloc(t, &t->move, B);
+        if (!rc) rc = talloc(t, &t->row_stats, 2 * B);
+    }
+    if (!rc && kind == C6_POLICY_LOSS_VISITS && !t->weights) {
+        rc = talloc(t, &t->visits, B * n2);
+        if (!rc) rc = talloc(t, &t->weights, B * n2);
+    }
+    if (!rc) t->policy_loss = kind;
+    return rc;
+}
+
+extern "C" int c6_trainer_set_clip(c6_trainer *t, float max_norm) {
+    if (!t) return tfail(C6_ERR_BAD_ARG, "c6_trainer_set_clip: NULL trainer");
+    if (!(max_norm <= 3.402823466e38f)) return tfail(C6_ERR_BAD_ARG, "c6_trainer_set_clip: max_norm must be finite");
+    if (max_norm >= 0.f && !t->clipper) {
+        TCHK(hipSetDevice(t->device));
+        if (!t->norm)
+            if (int rc = talloc(t, &t->norm, 1)) return rc;
+        const void *grad = t->G;
+        const int type = C6_TYPE_F32;
+        c6_clip *c = nullptr;
+        if (int rc = c6_clip_create(1, &grad, nullptr, &t->nfloats, &type, t->device, &c)) return tfail(rc, c6_last_error());
+        if (int rc = talloc(t, &t->clip_space, c6_clip_workspace(c) / sizeof(double))) {
+            c6_clip_destroy(c);
+            return rc;
+        }
+        t->clipper = c;
+    }
+    t->clip = max_norm;
+    return C6_OK;
+}
+
+extern "C" int c6_trainer_grad_norm(c6_trainer *t, float *norm) {
+    if (!t || !norm) return tfail(C6_ERR_BAD_ARG, "c6_trainer_grad_norm: NULL argument");
+    if (!t->clipped) return tfail(C6_ERR_BAD_ARG, "c6_trainer_grad_norm: the last step was not clipped");
+    TCHK(hipSetDevice(t->device));
+    TCHK(hipMemcpyAsync(norm, t->norm, sizeof(float), hipMemcpyDeviceToHost, t->stream));
+    TCHK(hipStreamSynchronize(t->stream));
     return C6_OK;
 }
 

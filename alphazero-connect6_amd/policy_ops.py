@@ -157,7 +157,7 @@ def policy_loss(logits, targets, mask=None, grad_scale=None, grad=None):
         g, gs = grad.data_ptr(), grad.stride(0)
     elif grad is not None:
         raise C6Error("grad needs a grad_scale")
-    stats = torch.empty((3, rows), dtype=_F32, device=logits.device)
+    stats = torch.empty_strided((3, rows), (rows, 1), dtype=_F32, device=logits.device)
     at = stats.data_ptr()
     L = lib()
     space, nbytes = None, L.c6_policy_loss_workspace(rows, width) if width > _SMALL else 0

@@ -418,6 +418,9 @@ int c6_replay_sample(c6_replay *r, int num_sample, uint64_t seed, uint32_t draw_
 /* the same draw into DEVICE buffers on a caller's HIP stream (hipStream_t passed as void*): the trainer's mini-batch */
 int c6_replay_sample_device(c6_replay *r, int num_sample, uint64_t seed, uint32_t draw_id, float *winners, float *players,
                             float *boards, float *poses, void *stream);
+/* ... with the visit counts, pi float [num_sample][N*N] (NULL: as above) */
+int c6_replay_sample_device_pi(c6_replay *r, int num_sample, uint64_t seed, uint32_t draw_id, float *winners, float *players, float *boards, float *poses,
+                               float *pi, void *stream);
 int c6_replay_board_size(const c6_replay *r);
 
 /* =====================================================================================================================
@@ -440,6 +443,18 @@ int c6_trainer_set_lr(c6_trainer *t, float lr, float momentum);
  * Winograd domain; gradient parity with an FP32 framework to ~1e-6.  C6_PREC_FP32_DIRECT: the same arithmetic on the direct kernels
  * (the yardstick).  C6_PREC_BF16X3: the evaluator's split-bf16 kernels, weight gradient included -- 1.3x faster, gradients to ~1e-3. */
 int c6_trainer_set_precision(c6_trainer *t, int precision);
+/* What the trainer's policy is trained on (set before a step; the initial setting is the reference's loss, model.hpp:97-108):
+ *   C6_POLICY_LOSS_REFERENCE  mean(-log(softmax over ALL cells[pos] + 1e-7))
+ *   C6_POLICY_LOSS_LEGAL      cross entropy of the move played over the EMPTY cells of the position (c6_policy_loss)
+ *   C6_POLICY_LOSS_VISITS     ... against the search's visit counts, normalised to 1 over the empty cells: `poses` of c6_trainer_step and
+ *                             c6_trainer_loss is then [B][N*N] (c6_replay_sample's pi); c6_trainer_step_replay draws them itself
+ * A position whose move is not on an empty cell, or that has no visits, adds nothing to the policy's loss. */
+enum { C6_POLICY_LOSS_REFERENCE = 0, C6_POLICY_LOSS_LEGAL = 1, C6_POLICY_LOSS_VISITS = 2 };
+int c6_trainer_set_policy_loss(c6_trainer *t, int kind);
+/* Clips the gradients of every step to a global norm of max_norm (c6_clip) before SGD; max_norm < 0 (initially): no clipping.
+ * c6_trainer_gradients then returns the clipped ones, c6_trainer_grad_norm the norm of the last step before clipping. */
+int c6_trainer_set_clip(c6_trainer *t, float max_norm);
+int c6_trainer_grad_norm(c6_trainer *t, float *norm);
 /* parity-test operator: dW (OIHW [C][C][3][3], f32) of y = conv3x3(x, w) from dy and x (host buffers, NHWC [B][N*N][C]).
  * method 0: the direct kernel, 1: in the Winograd domain (C = 256) -- the two implementations the FP32 trainer chooses between */
 int c6_conv_wgrad_op(int n, int C, int B, const float *dy, const float *x, int method, float *dw);

@@ -149,6 +149,52 @@ def test_loss_and_gradient(i, shape, target, kind):
         assert f(z, z) is z and torch.equal(z, ref)
 
 
+# Which way a loss goes depends on rows and width (policy_ops.hip, splits() and loss_launch()): four rows a wave from 4096 rows on, 16 to 1024 lanes a row, rows that a
+# workgroup takes one after the other, rows split into chunks.  (rows, width, type, target, mask): a case on each side of each border.
+WAYS = [(4096, 81, "f32", "index32", "rows"), (4097, 225, "bf16", "weights", "soa"), (4099, 361, "f16", "weights", "shared"), (5000, 384, "f32", "index64", "none"),
+        (4096, 385, "f32", "weights", "rows"), (4095, 361, "bf16", "weights", "rows"), (4100, 768, "bf16", "index32", "rows"), (4100, 769, "bf16", "index32", "none"),
+        (70, 1024, "f32", "weights", "none"), (70, 1025, "f32", "weights", "rows"), (300, 4097, "f16", "weights", "rows"), (300, 8192, "f32", "index32", "rows"),
+        (300, 8193, "f32", "weights", "rows"), (600, 16385, "f32", "index32", "none"), (520, 40001, "bf16", "weights", "shared"), (300, 65536, "bf16", "weights", "none"),
+        (300, 65537, "bf16", "weights", "rows"), (300, 65537, "bf16", "index32", "rows"), (129, 65536, "f32", "index64", "rows"), (130, 65537, "f32", "index32", "none"),
+        (128, 32769, "f32", "index32", "rows"), (129, 32769, "f32", "index32", "rows"), (257, 131072, "f16", "index32", "none"), (2, 1000003, "bf16", "weights", "rows")]
+
+
+@pytest.mark.parametrize("rows,width,kind,target,mask", WAYS)
+def test_every_way_a_loss_goes(rows, width, kind, target, mask):
+    torch, ops, _ = setup()
+    rng = np.random.default_rng(rows + width)
+    x, vals, m, packed = make(rows, width, kind, rows * 7 + width, mask)
+    if target == "weights":
+        t = (rng.random((rows, width)) ** 6).astype(np.float32)
+        t[5:9] = 0
+    else:
+        t = rng.integers(0, width, rows).astype(np.int32 if target == "index32" else np.int64)
+    td = torch.tensor(t, device="cuda")
+    before = x.clone()
+    got = ops.policy_loss(x, td, mask=m, grad_scale=0.5)
+    fwd = ops.policy_loss(x, td, mask=m)
+    assert torch.equal(x.nan_to_num(nan=99.0), before.nan_to_num(nan=99.0))
+    pick = np.unique(np.r_[:min(rows, 12), rng.integers(0, rows, 40), rows - 1])      # these rows against float64, all of them against one another
+    sub = packed if packed is None or packed.shape[0] == 1 else packed[pick]
+    want, tol = po.loss(vals[pick], t[pick], sub, 0.5)
+    idx = torch.tensor(pick, device="cuda")
+    for k, v in zip(("loss", "lse", "total"), got):
+        po.near(host(v[idx]), want[k], tol[k], "f32", k)
+    po.near(host(got[3][idx]), want["grad"], tol["grad"], kind, "grad")
+    # the forward pass alone may go another way: as far apart as two roundings
+    for k, a, b in zip(("loss", "lse", "total"), fwd, got):
+        po.near(host(a[idx]), want[k], tol[k], "f32", k + " alone")
+        fin = torch.isfinite(b)
+        assert torch.equal(torch.isfinite(a), fin) and bool(((a - b)[fin].abs() <= 1e-4 * (1 + b[fin].abs())).all())
+    # the backward pass alone agrees over ALL rows
+    g = ops.policy_loss_grad(x, td, got[1], got[2], torch.full((1,), 0.5, device="cuda"), mask=m)
+    d = (g.float() - got[3].float()).abs()
+    assert bool((d <= 2 * po.HALF_STEP[kind] * (g.float().abs() + got[3].float().abs()) + 2e-5 * got[2][:, None] + po.TINY[kind]).all())
+    # in place
+    z = x.clone()
+    assert torch.equal(ops.policy_loss(z, td, mask=m, grad_scale=0.5, grad=z)[3], got[3])
+
+
 @pytest.mark.parametrize("width", [5, 300, 40000])
 def test_rows_with_infinities_and_nan(width):
     """what stands at LEGAL entries: -infinity is an entry of probability 0, +infinity and NaN make the row NaN, a row of nothing but -infinity is empty"""

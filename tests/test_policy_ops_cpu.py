@@ -105,6 +105,13 @@ def test_clip_sound_tables_get_as_far_as_the_device():
         assert clip_create(spec) == NO_GPU, spec
 
 
+def test_trainer_refusals_without_a_trainer():
+    L = pkg.lib()
+    f = C.c_float()
+    assert L.c6_trainer_set_policy_loss(None, 0) == BAD and L.c6_trainer_set_clip(None, 1.0) == BAD and L.c6_trainer_grad_norm(None, C.byref(f)) == BAD
+    assert L.c6_replay_sample_device_pi(None, 1, 0, 0, None, None, None, None, None, None) == BAD
+
+
 def test_python_face_refuses_host_tensors():
     import torch
     from alphazero_connect6_amd import policy_ops as ops
