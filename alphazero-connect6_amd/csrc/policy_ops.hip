@@ -40,7 +40,7 @@ template <typename T, int LANES, bool HIST, bool BIAS>
 __global__ __launch_bounds__(256) void c6_logits_process_kernel(Rows l, Repeats h, const float *bias, int64_t bias_stride, T *out, int64_t out_stride) {
     typedef C6Vec<T> V;
     constexpr int CHUNK = LANES == 64 ? PROCESS_WAVE : PROCESS_BLOCK, U = CHUNK / (LANES * V::N), PER = 256 / LANES;
-    __shared__ uint32_t counters[HIST ? PER * CHUNK : 1];
+    __shared__ alignas(16) uint32_t counters[HIST ? PER * CHUNK : 1];
     const int lane = threadIdx.x % LANES, part = threadIdx.x / LANES;
     uint32_t *count = counters + (HIST ? part * CHUNK : 0);
     const auto meet = [] {      // one wave's LDS operations are performed in order: only the compiler has to keep them so
@@ -611,7 +611,7 @@ bool fits(int64_t rows, int64_t stride, int64_t width, int64_t bytes) {
 
 int check_logits(const c6_logits *l) {
     if (!l) return bad("logits: NULL argument");
-    if (l->rows < 0 || l->width < 0) return bad("logits: negative size");
+    if (l->rows < 0 || l->width < 0 || l->width > 1 << 30) return bad("logits: a size is negative, or the width over 2^30");
     if (!c6_type_ok(l->type)) return bad("logits: type must be C6_TYPE_F32, C6_TYPE_F16 or C6_TYPE_BF16");
     if (l->x_stride < 0 || l->mask_row < 0 || l->mask_byte < 0) return bad("logits: negative stride");
     const int64_t es = (int64_t)c6_type_bytes(l->type);

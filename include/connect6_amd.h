@@ -578,7 +578,7 @@ enum { C6_TYPE_F32 = 0, C6_TYPE_F16 = 1, C6_TYPE_BF16 = 2 };
 
 /* rows of logits, and which of their entries are legal */
 typedef struct c6_logits {
-    int rows, width;         /* >= 0 */
+    int rows, width;         /* >= 0, the width at most 2^30 */
     int type;                /* C6_TYPE_* of x, and of what is computed for every entry */
     int device;              /* HIP ordinal */
     const void *x;           /* entry v of row r: x[r * x_stride + v]; aligned to its type */
@@ -603,7 +603,8 @@ int c6_logits_process(const c6_logits *l, const int32_t *history, int64_t histor
 /* Cross entropy over the legal entries.  With target weights t >= 0 over the entries (those of illegal entries count for nothing):
  *     lse = log sum exp(x),   total = sum t,   loss = sum t (lse - x),   gradient = scale * (total * exp(x - lse) - t)
  * over the legal entries; the gradient of the others is 0.  A row without a legal entry above -infinity: loss = total = 0,
- * lse = -infinity, gradient 0.  NaN or +infinity at a legal entry makes the row NaN.  Statistics are held in 32 bits. */
+ * lse = -infinity, gradient 0.  NaN or +infinity at a legal entry makes the row NaN: its loss, lse and gradient (there at the legal entries for
+ * certain, at the others either NaN or 0).  Statistics are held in 32 bits. */
 enum {
     C6_TARGET_INDEX32 = 0,   /* target: int32 [rows], t = 1 at that entry; an index outside [0, width) or at an illegal entry: t = 0 everywhere */
     C6_TARGET_INDEX64 = 1,   /* ... int64 */

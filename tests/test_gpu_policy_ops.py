@@ -278,6 +278,56 @@ def test_legal_mask_of_the_board_kernel_goes_straight_in():
     assert np.array_equal(y, np.where(boards == 0, x.astype(np.float64), -np.inf))
 
 
+def test_masks_and_histories_of_any_stride():
+    """rows of masks, histories, penalties and biases out of larger buffers; bits behind the row's end mean nothing"""
+    torch, ops, _ = setup()
+    rng = np.random.default_rng(11)
+    for rows, width in ((6, 85), (5, 5003)):
+        x = rng.normal(0, 2, (rows, width)).astype(np.float32)
+        keep = rng.random((rows, width)) < 0.5
+        packed = po.pack(keep)
+        noisy = packed.copy()
+        noisy[:, -1] |= (0xff << (width % 8)) & 0xff
+        hist = rng.integers(0, width, (rows, 33)).astype(np.int32)
+        pen = rng.uniform(0.5, 1.5, (rows, 3)).astype(np.float32)
+        bias = rng.normal(0, 1, (rows, width)).astype(np.float32)
+
+        def inside(a):      # a in the middle of a buffer twice as large
+            buf = torch.zeros((a.shape[0] * 2, a.shape[1] + 7), dtype=torch.tensor(a).dtype, device="cuda")
+            v = buf[::2, 3:3 + a.shape[1]]
+            v.copy_(torch.tensor(a))
+            return v
+        wide = torch.zeros((rows, packed.shape[1] * 3), dtype=torch.uint8, device="cuda")
+        wide[:, ::3] = torch.tensor(noisy, device="cuda")
+        want, tol = po.process(x, packed, bias=bias, history=hist, penalties=pen)
+        xd = torch.tensor(x, device="cuda")
+        for m in (inside(noisy), wide[:, ::3], torch.tensor(noisy, device="cuda")):
+            y = ops.logits_process(xd, mask=m, bias=inside(bias), history=inside(hist), penalties=inside(pen))
+            po.near(host(y), want, tol, "f32", "strides")
+            t = torch.zeros(rows, dtype=torch.int64, device="cuda")
+            lw, lt = po.loss(x, t.cpu().numpy(), packed, 1.0)
+            got = ops.policy_loss(inside(x), t, mask=m, grad_scale=1.0)
+            po.near(host(got[0]), lw["loss"], lt["loss"], "f32", "loss")
+            po.near(host(got[3]), lw["grad"], lt["grad"], "f32", "grad")
+
+
+def test_two_at_once():
+    """the same logits on two streams, rows split into chunks on both: a workspace each"""
+    torch, ops, _ = setup()
+    x = torch.randn(4, 200003, device="cuda")
+    t = torch.tensor([0, 7, 200002, 9], dtype=torch.int32, device="cuda")
+    want = ops.policy_loss(x, t, grad_scale=1.0)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(20):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(ops.policy_loss(x, t, grad_scale=1.0))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+
+
 def test_python_refusals():
     torch, ops, _ = setup()
     x = torch.zeros(4, 10, device="cuda")

@@ -29,7 +29,7 @@ def grad_of(l, target=2 * A, kind=0, ts=0, lse=3 * A, total=3 * A, dloss=3 * A, 
     return pkg.lib().c6_policy_loss_grad(l, target, kind, ts, lse, total, dloss, ds, grad, gs, None)
 
 
-@pytest.mark.parametrize("kw", [dict(rows=-1), dict(width=-1), dict(type=3), dict(x=None), dict(x=A + 2), dict(type=1, x=A + 1), dict(x_stride=-1),
+@pytest.mark.parametrize("kw", [dict(rows=-1), dict(width=-1), dict(width=(1 << 30) + 1, x_stride=1 << 31), dict(type=3), dict(x=None), dict(x=A + 2), dict(type=1, x=A + 1), dict(x_stride=-1),
                                 dict(mask_row=-1, mask=A), dict(mask_byte=-1, mask=A), dict(x_stride=1 << 62)])
 def test_bad_logits_are_refused_by_every_entry_point(kw):
     l = logits(**kw)
