@@ -12,6 +12,7 @@ that do not fit raise C6Error before anything runs.  Nothing here is recorded by
 `import torch` comes before the first use of the library in a process that wants both on the GPU: whichever is first brings the HIP runtime
 that the other then shares (torch does not start on another's)."""
 import ctypes as C
+import functools
 import sys
 
 import torch
@@ -27,7 +28,6 @@ _TYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _INDEX = {torch.int32: 0, torch.int64: 1}
 _WEIGHTS = 2
 _Tensor, _F32, _I32, _U8 = torch.Tensor, torch.float32, torch.int32, torch.uint8
-_SMALL = 8192        # entries of a row up to which the loss needs no workspace whatever the type (c6_policy_loss_workspace is 0)
 
 
 def _raw_stream(device):
@@ -36,6 +36,11 @@ def _raw_stream(device):
 
 # the handle alone where torch has a call for it: 0.1 us instead of 1.8
 _stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+
+@functools.lru_cache(maxsize=1024)
+def _loss_workspace(rows, width):
+    return lib().c6_policy_loss_workspace(rows, width)
+
 
 # The checks below cost a call less than its launch: messages are made when they are needed, and attributes are read once.
 
@@ -159,12 +164,11 @@ def policy_loss(logits, targets, mask=None, grad_scale=None, grad=None):
         raise C6Error("grad needs a grad_scale")
     stats = torch.empty_strided((3, rows), (rows, 1), dtype=_F32, device=logits.device)
     at = stats.data_ptr()
-    L = lib()
-    space, nbytes = None, L.c6_policy_loss_workspace(rows, width) if width > _SMALL else 0
+    space, nbytes = None, _loss_workspace(rows, width)
     if nbytes:
-        keep = torch.empty(nbytes, dtype=_U8, device=logits.device)
+        keep = torch.empty_strided((nbytes,), (1,), dtype=_U8, device=logits.device)
         space = keep.data_ptr()
-    _chk(L.c6_policy_loss(l, t, kind, ts, at, at + 4 * rows, at + 8 * rows, g, gs, grad_scale or 0.0, space, nbytes, _stream(dev)))
+    _chk(lib().c6_policy_loss(l, t, kind, ts, at, at + 4 * rows, at + 8 * rows, g, gs, grad_scale or 0.0, space, nbytes, _stream(dev)))
     loss, lse, total = stats.unbind(0)
     return (loss, lse, total) if grad is None else (loss, lse, total, grad)
 
@@ -238,10 +242,10 @@ class GradClip:
         if not self.h:
             raise C6Error("GradClip is closed")
         if norm is None:
-            norm = torch.empty(1, dtype=_F32, device=self.device)
+            norm = torch.empty_strided((1,), (1,), dtype=_F32, device=self.device)
         elif not isinstance(norm, _Tensor) or norm.dtype is not _F32 or norm.shape != (1,) or norm.device != self.device:
             raise C6Error("norm must be a float32 tensor [1] on the gradients' device")
-        return norm, torch.empty(self._bytes, dtype=_U8, device=self.device)
+        return norm, torch.empty_strided((self._bytes,), (1,), dtype=_U8, device=self.device)
 
     def norm(self, norm=None):
         """the global norm, a float32 tensor [1]; the gradients stay as they are"""
