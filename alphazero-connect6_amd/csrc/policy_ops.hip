@@ -25,9 +25,13 @@ __device__ __forceinline__ uint32_t legal_bits(const Rows &l, const uint8_t *mas
 }
 
 // ---- penalties, biases, masks -------------------------------------------------------------------------------------------
-// A row is cut into chunks; LANES threads take one chunk: a wave for rows of up to 1024 entries (four rows a workgroup), else a workgroup per 8192.
-// The chunk's logits are requested first, 16 bytes a lane and all in flight, and wait in registers while the row's history is counted in LDS:
-// each chunk reads the whole history and counts the ids that fall into it (integer adds: the order does not matter).
+// Bound by memory: every logit in and out once.  A row is cut into chunks; LANES threads take one chunk: a wave for rows of up to 1024 entries (four rows a
+// workgroup), else a workgroup per 4096 (with histories of up to 8191 ids 512 rows of 131072 f32 took 131 us so, 143 in chunks of 8192, 210 of 16384: a
+// larger chunk scans the history less often but leaves fewer waves).  The chunk's logits, mask and bias are requested first, 16 bytes a lane and all in
+// flight, and wait in registers while the row's history is counted in LDS: each chunk reads the whole history and counts the ids that fall into it
+// (integer adds: the order does not matter).
+// Measured, kernel alone: 512 x 131072 f32 96 us without mask and history (5.6 TB/s; a copy of that size 99), 121 us with both; 48 x 100003 bf16 with 2048
+// ids, mask and bias 9.7 us; 4096 x 361 f32 with 200 moves, legal masks and bias 7.8 us; one row of 361 2.2 us.
 struct Repeats {
     const int32_t *history, *len;
     const float *penalties;
@@ -440,6 +444,10 @@ __device__ __forceinline__ void gradient(float x, const At &at, const Done &k, i
 // One pass over rows that fit the registers of LANES lanes: read once, the gradient written once.  A lane takes the maximum of its own entries, the sums
 // relative to that, and one reduction over the lanes joins them.  As a piece's gradient leaves, the same piece of the workgroup's next row is requested
 // into its registers: loads and stores overlap, and the sums of a row begin as its first pieces arrive.
+// Measured, loss and gradient: 2049 x 100003 bf16 187 us (4.4 TB/s; 1020 in three passes over each row).  There a workgroup has a CU to itself (97 registers
+// a lane, 16 waves) and the vector unit is busy for half the time, two exponentials an element of it: what is left over the 149 us of a copy is the part of
+// that work which one row's loads do not cover, a row address aligned to two bytes (3 us), and the 2049th row.  2048 x 16000 f32 45 us (5.8 TB/s),
+// 16384 x 361 bf16 against weights 12 us, 2048 x 225 f32 4 us.
 template <typename T, int LANES, int NV, bool WEIGHTS>
 __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void c6_policy_loss_kernel(Rows l, Target t, float *loss, float *lse, float *total, T *grad, int64_t grad_stride, float scale) {
     typedef C6Vec<T> V;
@@ -485,7 +493,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void c6_policy_loss_kern
 }
 
 // The same in two launches, for rows that do not fit or are too few to fill the card: every chunk's Part into the workspace, then each chunk joins its
-// row's and writes its piece of the gradient.
+// row's and writes its piece of the gradient.  3 x 131072 f32: 3.2 + 4.6 us; without a gradient 2048 x 100003 bf16 77 us (5.3 TB/s).
 constexpr int SPLIT_NV = 4;
 template <typename T>
 constexpr int split_chunk = 256 * SPLIT_NV * C6Vec<T>::N;
@@ -556,7 +564,8 @@ __global__ __launch_bounds__(256) void c6_policy_loss_join_kernel(Rows l, Target
     }
 }
 
-// The gradient from what the forward pass saved: elementwise, in chunks like those of c6_logits_process_kernel.
+// The gradient from what the forward pass saved: elementwise, in chunks like those of c6_logits_process_kernel.  Bound by memory: 777 x 32768 f16 against
+// weights 35 us for 206 MB (5.9 TB/s).
 constexpr int GRAD_WAVE = 1024, GRAD_BLOCK = 4096;
 
 template <typename T, int LANES, bool WEIGHTS>
