@@ -18,11 +18,13 @@
 #include <string>
 #include <vector>
 
+int c6_set_error(int code, const char *msg);      // engine.cpp
+
 static thread_local std::string t_err;
 static int tfail(int code, const std::string &msg) {
     t_err = msg;
     fprintf(stderr, "libconnect6_amd: %s\n", msg.c_str());
-    return code;
+    return c6_set_error(code, t_err.c_str());      // c6_last_error() has it too: there, an older message of another call would be taken for this one's
 }
 #define TCHK(x)                                                                                         \
     do {                                                                                                \

@@ -150,3 +150,10 @@ def test_oracle_against_torch():
         e[r, v] = 1e-5
         d = (po.loss(x + e, t, po.pack(keep))[0]["loss"] - po.loss(x - e, t, po.pack(keep))[0]["loss"])[r] / 2e-5
         assert abs(0.25 * d - out["grad"][r, v]) < 1e-8
+
+
+def test_a_trainers_error_is_not_hidden_behind_an_older_one():
+    L = pkg.lib()
+    assert process(None) == BAD and b"logits" in L.c6_last_error()
+    assert L.c6_trainer_set_clip(None, 1.0) == BAD
+    assert b"c6_trainer_set_clip" in L.c6_last_error() and b"c6_trainer_set_clip" in L.c6_trainer_last_error()
