@@ -494,7 +494,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void c6_policy_loss_kern
 
 // The same in two launches, for rows that do not fit or are too few to fill the card: every chunk's Part into the workspace, then each chunk joins its
 // row's and writes its piece of the gradient.  3 x 131072 f32: 3.2 + 4.6 us; without a gradient 2048 x 100003 bf16 77 us (5.3 TB/s).
-constexpr int SPLIT_NV = 4;
+constexpr int SPLIT_NV = 4, JOIN_MOST = 1024;
 template <typename T>
 constexpr int split_chunk = 256 * SPLIT_NV * C6Vec<T>::N;
 
@@ -526,14 +526,14 @@ __global__ __launch_bounds__(256) void c6_policy_loss_join_kernel(Rows l, Target
     typedef C6Vec<T> V;
     __shared__ Part space[4];
     const int chunks = (l.width + split_chunk<T> - 1) / split_chunk<T>, lane = threadIdx.x;
-    const int per = grad ? chunks : 1;      // without a gradient one workgroup a row
+    const int per = grad ? min(chunks, JOIN_MOST) : 1;      // workgroups a row (without a gradient one): each joins ALL the row's Parts, then takes every per-th chunk
     const int64_t items = (int64_t)l.rows * per;
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
         const int64_t r = item / per;
-        const int v0 = (int)(item % per) * split_chunk<T>;
+        const int first = (int)(item % per);
         const T *x = (const T *)l.x + r * l.x_stride;
-        Held<T, 256, SPLIT_NV> h(min(l.width - v0, split_chunk<T>));
-        if (grad) h.request(x + v0, lane);
+        Held<T, 256, SPLIT_NV> h(min(l.width - first * split_chunk<T>, split_chunk<T>));
+        if (grad) h.request(x + first * split_chunk<T>, lane);
         int index = -1;
         if (!WEIGHTS) {
             index = target_index(t, r, l.width);
@@ -549,16 +549,21 @@ __global__ __launch_bounds__(256) void c6_policy_loss_join_kernel(Rows l, Target
         p = block_part<256>(p, WEIGHTS, space);
         if (!WEIGHTS && index >= 0) { p.w = 1.f; p.d = p.m - at[r]; }
         const Done k = done(p, scale);
-        if (v0 == 0 && lane == 0) { loss[r] = k.loss; lse[r] = k.lse; total[r] = k.total; }
-        if (grad) {
+        if (first == 0 && lane == 0) { loss[r] = k.loss; lse[r] = k.lse; total[r] = k.total; }
+        for (int chunk = first; grad && chunk < chunks; chunk += per) {
+            const int v0 = chunk * split_chunk<T>;
+            if (chunk != first) {
+                h = Held<T, 256, SPLIT_NV>(min(l.width - v0, split_chunk<T>));
+                h.request(x + v0, lane);
+            }
             Beside here = beside<WEIGHTS>(l, t, r, v0);
             T *g = grad + r * grad_stride + v0;
-            index = index < 0 ? -1 : index - v0;      // (of another chunk: outside this one's columns)
+            const int at_index = index < 0 ? -1 : index - v0;      // (of another chunk: outside this one's columns)
             here.settle(h, lane);
 #pragma unroll
             for (int u = 0; u < SPLIT_NV; u++)
-                if (h.has(u, lane)) gradient<T, WEIGHTS>(h.raw[u], here, k, index, u, h.column(u, lane), g);
-            if (lane < h.rest) gradient<T, WEIGHTS>(h.tail, here, k, index, h.whole * V::N + lane, g);
+                if (h.has(u, lane)) gradient<T, WEIGHTS>(h.raw[u], here, k, at_index, u, h.column(u, lane), g);
+            if (lane < h.rest) gradient<T, WEIGHTS>(h.tail, here, k, at_index, h.whole * V::N + lane, g);
         }
         __syncthreads();
     }
@@ -751,9 +756,9 @@ static void loss_launch(const c6_logits *l, const Target &t, float *loss, float 
         const int64_t chunks = (l->width + split_chunk<T> - 1) / split_chunk<T>, items = l->rows * chunks;
         Part *parts = (Part *)workspace;
         float *at = (float *)(parts + items);
-        const unsigned grid = (unsigned)std::min<int64_t>(items, 1 << 22);
+        const unsigned grid = (unsigned)std::min<int64_t>(items, 1 << 22), join = (unsigned)std::min<int64_t>(l->rows * (grad ? std::min<int64_t>(chunks, JOIN_MOST) : 1), 1 << 22);
         hipLaunchKernelGGL((c6_policy_loss_part_kernel<T, WEIGHTS>), dim3(grid), dim3(256), 0, s, rows, t, parts, at);
-        hipLaunchKernelGGL((c6_policy_loss_join_kernel<T, WEIGHTS>), dim3(grad ? grid : (unsigned)std::min(l->rows, 1 << 22)), dim3(256), 0, s, rows, t, parts, at, loss, lse,
+        hipLaunchKernelGGL((c6_policy_loss_join_kernel<T, WEIGHTS>), dim3(join), dim3(256), 0, s, rows, t, parts, at, loss, lse,
                            total, grad, grad_stride, scale);
         return;
     }

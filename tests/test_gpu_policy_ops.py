@@ -156,7 +156,8 @@ WAYS = [(4096, 81, "f32", "index32", "rows"), (4097, 225, "bf16", "weights", "so
         (70, 1024, "f32", "weights", "none"), (70, 1025, "f32", "weights", "rows"), (300, 4097, "f16", "weights", "rows"), (300, 8192, "f32", "index32", "rows"),
         (300, 8193, "f32", "weights", "rows"), (600, 16385, "f32", "index32", "none"), (520, 40001, "bf16", "weights", "shared"), (300, 65536, "bf16", "weights", "none"),
         (300, 65537, "bf16", "weights", "rows"), (300, 65537, "bf16", "index32", "rows"), (129, 65536, "f32", "index64", "rows"), (130, 65537, "f32", "index32", "none"),
-        (128, 32769, "f32", "index32", "rows"), (129, 32769, "f32", "index32", "rows"), (257, 131072, "f16", "index32", "none"), (2, 1000003, "bf16", "weights", "rows")]
+        (128, 32769, "f32", "index32", "rows"), (129, 32769, "f32", "index32", "rows"), (257, 131072, "f16", "index32", "none"), (2, 1000003, "bf16", "weights", "rows"),
+        (2, 9000001, "f32", "index32", "rows"), (1, 9000001, "f16", "weights", "none")]      # (more chunks than workgroups a row)
 
 
 @pytest.mark.parametrize("rows,width,kind,target,mask", WAYS)
@@ -415,6 +416,13 @@ def test_clip_neither_overflows_nor_vanishes():
     g = torch.full((100000,), 1e30, device="cuda")
     ops.GradClip([g]).clip(1.0)
     assert abs(float(g[7]) * np.sqrt(1e5) - 1) < 1e-6
+
+
+def test_clip_of_nothing():
+    torch, ops, _ = setup()
+    e = torch.empty(0, device="cuda")
+    c = ops.GradClip([e, e.half()])
+    assert float(c.norm()) == 0 and float(c.clip(1.0)) == 0
 
 
 def test_clip_infinities_and_nan():
