@@ -81,11 +81,6 @@ struct C6Vec {
 #pragma unroll
         for (int i = 0; i < N; i++) f[i] = i < n ? c6_get(p[i]) : fill;
     }
-    static __device__ __forceinline__ c6_u32x4 load_some(const T *p, int n, float fill) {
-        float f[N];
-        get_some(p, n, fill, f);
-        return put(f);
-    }
     static __device__ __forceinline__ void put_some(T *p, int n, const float (&f)[N]) {
 #pragma unroll
         for (int i = 0; i < N; i++)
@@ -112,7 +107,6 @@ __device__ __forceinline__ float c6_wave_all(float v, F f) {
     return f(f(row(0), row(16)), f(row(32), row(48)));
 }
 __device__ __forceinline__ float c6_wave_sum(float v) { return c6_wave_all(v, [](float a, float b) { return a + b; }); }
-__device__ __forceinline__ float c6_wave_max(float v) { return c6_wave_all(v, [](float a, float b) { return fmaxf(a, b); }); }
 __device__ __forceinline__ double c6_wave_sum(double v) {
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
@@ -139,7 +133,7 @@ static inline size_t c6_type_bytes(int type) { return type == C6_TYPE_F32 ? 4 : 
 static inline bool c6_type_ok(int type) { return type == C6_TYPE_F32 || type == C6_TYPE_F16 || type == C6_TYPE_BF16; }
 static inline bool c6_aligned(const void *p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
-// the visible devices, counted once; `what`'s caller reports the message
+// the visible devices, counted once
 static inline int c6_check_device(int device) {
     static const int count = c6_device_count();
     if (count < 1) return c6_set_error(C6_ERR_NO_GPU, "no HIP device visible; this library has no CPU fallback");

@@ -47,26 +47,27 @@ def _loss_workspace(rows, width):
 
 def _logits(x, mask):
     """-> (c6_logits, rows, width)"""
-    kind = _TYPE.get(x.dtype) if isinstance(x, _Tensor) and x.is_cuda else None
-    if kind is None or x.dim() != 2:
+    kind = _TYPE.get(x.dtype) if isinstance(x, _Tensor) else None
+    shape = x.shape if kind is not None else ()
+    device = x.get_device() if kind is not None else -1
+    if device < 0 or len(shape) != 2:
         raise C6Error("logits must be a [rows, width] tensor of float32, float16 or bfloat16 on the GPU")
-    rows, width = x.shape
+    rows, width = shape
     stride, step = x.stride()
     if step != 1 and width > 1:
         raise C6Error("the entries of a row of logits must lie next to each other")
     if x.requires_grad:
         raise C6Error("logits that require a gradient: autograd does not see this operator, pass logits.detach()")
-    device = x.get_device()
     if mask is None:
         return Logits(rows, width, kind, device, x.data_ptr(), stride, None, 0, 0), rows, width
     if not isinstance(mask, _Tensor) or mask.dtype is not _U8 or mask.get_device() != device:
         raise C6Error("mask must be a uint8 tensor on the logits' device")
-    if mask.dim() == 1:
-        mask = mask.unsqueeze(0)
-    if mask.dim() != 2 or mask.shape[1] != (width + 7) // 8 or mask.shape[0] not in (rows, 1):
+    shape, strides = mask.shape, mask.stride()
+    if len(shape) == 1:
+        shape, strides = (1, *shape), (0, *strides)
+    if len(shape) != 2 or shape[1] != (width + 7) // 8 or (shape[0] != rows and shape[0] != 1):
         raise C6Error(f"mask must be [{rows}, {(width + 7) // 8}], or one row for all: one bit per entry of logits, entry v at bit v % 8 of byte v // 8")
-    row, byte = mask.stride()
-    return Logits(rows, width, kind, device, x.data_ptr(), stride, mask.data_ptr(), 0 if mask.shape[0] == 1 else row, byte), rows, width
+    return Logits(rows, width, kind, device, x.data_ptr(), stride, mask.data_ptr(), 0 if shape[0] == 1 else strides[0], strides[1]), rows, width
 
 
 def _written(out, x, what):
@@ -87,7 +88,7 @@ def _rows_by(t, dtype, device, rows, width, what):
         raise C6Error(f"{what} must be a {dtype} tensor on the logits' device")
     shape, stride = t.shape, t.stride()
     dim = len(shape)
-    if dim not in (1, 2) or shape[-1] != width or (dim == 2 and shape[0] not in (rows, 1)):
+    if (dim != 2 and dim != 1) or shape[-1] != width or (dim == 2 and shape[0] != rows and shape[0] != 1):
         raise C6Error(f"{what} must be [{rows}, {width}], [1, {width}] or [{width}]")
     if stride[-1] != 1 and width > 1:
         raise C6Error(f"the entries of a row of {what} must lie next to each other")
@@ -95,7 +96,7 @@ def _rows_by(t, dtype, device, rows, width, what):
 
 
 def _per_row(t, dtype, device, rows, what):
-    if not isinstance(t, _Tensor) or t.dtype is not dtype or t.get_device() != device or t.dim() != 1 or t.shape[0] != rows or (rows > 1 and t.stride(0) != 1):
+    if not isinstance(t, _Tensor) or t.dtype is not dtype or t.get_device() != device or t.shape != (rows,) or (rows > 1 and not t.is_contiguous()):
         raise C6Error(f"{what} must be a contiguous {dtype} tensor [{rows}] on the logits' device")
     return t.data_ptr()
 
