@@ -18,11 +18,10 @@ __device__ __forceinline__ bool legal(const Rows &l, int64_t r, int v) {
     return !l.mask || (l.mask[r * l.mask_row + (int64_t)(v >> 3) * l.mask_byte] >> (v & 7) & 1);
 }
 
-// the legal bits of the N entries from column c (a multiple of N) on
+// the legal bits of the N entries from column c (a multiple of N) on, out of their byte of the mask: apart, so that no wait for the byte comes before the
+// loads after it
 template <int N>
-__device__ __forceinline__ uint32_t legal_bits(const Rows &l, const uint8_t *mask_row, int c) {
-    return (uint32_t)mask_row[(int64_t)(c >> 3) * l.mask_byte] >> (N == 4 ? c & 4 : 0);
-}
+__device__ __forceinline__ uint32_t legal_bits(uint32_t byte, int c) { return byte >> (N == 4 ? c & 4 : 0); }
 
 // ---- penalties, biases, masks -------------------------------------------------------------------------------------------
 // Bound by memory: every logit in and out once.  A row is cut into chunks; LANES threads take one chunk: a wave for rows of up to 1024 entries (four rows a
@@ -38,17 +37,19 @@ struct Repeats {
     int64_t history_stride, penalties_stride;
     int cap;
 };
-constexpr int PROCESS_WAVE = 1024, PROCESS_BLOCK = 4096;
+// entries of a chunk: of 16 lanes (four rows a wave), of a wave, of a workgroup
+template <int LANES>
+constexpr int chunk_of = LANES == 16 ? 384 : LANES == 64 ? 1024 : 4096;
 
 template <typename T, int LANES, bool HIST, bool BIAS>
 __global__ __launch_bounds__(256) void c6_logits_process_kernel(Rows l, Repeats h, const float *bias, int64_t bias_stride, T *out, int64_t out_stride) {
     typedef C6Vec<T> V;
-    constexpr int CHUNK = LANES == 64 ? PROCESS_WAVE : PROCESS_BLOCK, U = CHUNK / (LANES * V::N), PER = 256 / LANES;
+    constexpr int CHUNK = chunk_of<LANES>, U = CHUNK / (LANES * V::N), PER = 256 / LANES;
     __shared__ alignas(16) uint32_t counters[HIST ? PER * CHUNK : 1];
     const int lane = threadIdx.x % LANES, part = threadIdx.x / LANES;
     uint32_t *count = counters + (HIST ? part * CHUNK : 0);
     const auto meet = [] {      // one wave's LDS operations are performed in order: only the compiler has to keep them so
-        if (LANES == 64) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (LANES <= 64) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         else __syncthreads();
     };
     const int chunks = (l.width + CHUNK - 1) / CHUNK;
@@ -56,22 +57,31 @@ __global__ __launch_bounds__(256) void c6_logits_process_kernel(Rows l, Repeats 
     for (int64_t item = (int64_t)blockIdx.x * PER + part; item < items; item += (int64_t)gridDim.x * PER) {
         const int64_t r = item / chunks;
         const int v0 = (int)(item % chunks) * CHUNK, nv = min(CHUNK, l.width - v0);
+        const int whole = nv / V::N, rest = nv % V::N, last = whole * V::N + lane;      // whole pieces; the entries behind them one a lane
         const T *x = (const T *)l.x + r * l.x_stride + v0;
         T *o = out + r * out_stride + v0;
         const uint8_t *mask = l.mask ? l.mask + r * l.mask_row : nullptr;
         const float *b = BIAS ? bias + r * bias_stride + v0 : nullptr;
+        // every lane loads U pieces, behind the last one that again: no branch stands between the loads
         c6_u32x4 raw[U], add[BIAS ? U : 1][V::N / 4];
-        uint32_t ok[U];
+        uint32_t bits[U], tail_bits = 0xff;
+        T tail = c6_put<T>(0.f);
+        float tail_add = 0.f;
+        if (whole) {
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int c = (u * LANES + lane) * V::N;
-            ok[u] = ~0u;
-            if (c + V::N <= nv) raw[u] = V::load(x + c);
-            if (mask && c < nv) ok[u] = legal_bits<V::N>(l, mask, v0 + c);
-            if constexpr (BIAS)
-                if (c + V::N <= nv)
+            for (int u = 0; u < U; u++) {
+                const int c = min(u * LANES + lane, whole - 1) * V::N;
+                raw[u] = V::load(x + c);
+                bits[u] = mask ? mask[(int64_t)((v0 + c) >> 3) * l.mask_byte] : 0xff;
+                if constexpr (BIAS)
 #pragma unroll
                     for (int i = 0; i < V::N / 4; i++) add[u][i] = C6Vec<float>::load(b + c + 4 * i);
+            }
+        }
+        if (lane < rest) {
+            tail = x[last];
+            if (mask) tail_bits = mask[(int64_t)((v0 + last) >> 3) * l.mask_byte];
+            if (BIAS) tail_add = b[last];
         }
         float rep = 1.f, freq = 0.f, pres = 0.f;
         if (HIST) {
@@ -107,40 +117,43 @@ __global__ __launch_bounds__(256) void c6_logits_process_kernel(Rows l, Repeats 
             }
             meet();
         }
+        const auto less = [&](float y, uint32_t k) { return (y > 0.f ? y / rep : y * rep) - (freq * (float)k + pres); };
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int c = (u * LANES + lane) * V::N;
-            if (c >= nv) continue;
-            const bool whole = c + V::N <= nv;
+            if (u * LANES + lane >= whole) continue;
             float y[V::N];
-            if (whole) V::get(raw[u], y);
-            else V::get_some(x + c, nv - c, 0.f, y);
+            V::get(raw[u], y);
             if (HIST) {
-                uint32_t k[V::N];
+                uint32_t k[V::N], any = 0;
 #pragma unroll
                 for (int i = 0; i < V::N; i += 4) *reinterpret_cast<uint4 *>(k + i) = *reinterpret_cast<const uint4 *>(count + c + i);
-                uint32_t any = 0;
 #pragma unroll
                 for (int i = 0; i < V::N; i++) any |= k[i];
                 if (any)
 #pragma unroll
                     for (int i = 0; i < V::N; i++)
-                        if (k[i]) y[i] = (y[i] > 0.f ? y[i] / rep : y[i] * rep) - (freq * (float)k[i] + pres);
+                        if (k[i]) y[i] = less(y[i], k[i]);
             }
             if constexpr (BIAS) {
 #pragma unroll
                 for (int i = 0; i < V::N; i += 4) {
                     float q[4];
-                    if (whole) C6Vec<float>::get(add[u][i / 4], q);
-                    else C6Vec<float>::get_some(b + c + i, nv - c - i, 0.f, q);
+                    C6Vec<float>::get(add[u][i / 4], q);
 #pragma unroll
                     for (int j = 0; j < 4; j++) y[i + j] += q[j];
                 }
             }
-#pragma unroll
-            for (int i = 0; i < V::N; i++) y[i] = ok[u] >> i & 1 ? y[i] : -INFINITY;
-            if (whole) V::store(o + c, V::put(y));
-            else V::put_some(o + c, nv - c, y);
+            c6_u32x4 done = V::put(y);
+            V::keep(done, legal_bits<V::N>(bits[u], c));
+            V::store(o + c, done);
+        }
+        if (lane < rest) {
+            float y = c6_get(tail);
+            if (HIST)
+                if (const uint32_t k = count[last]) y = less(y, k);
+            if (BIAS) y += tail_add;
+            o[last] = c6_put<T>(tail_bits >> (last & 7) & 1 ? y : -INFINITY);
         }
         if (HIST) meet();      // the counters are read before the next item clears them
     }
@@ -156,27 +169,6 @@ __device__ __forceinline__ int target_index(const Target &t, int64_t r, int widt
     if (t.kind == C6_TARGET_WEIGHTS) return -1;
     const int64_t i = t.kind == C6_TARGET_INDEX64 ? ((const int64_t *)t.p)[r] : ((const int32_t *)t.p)[r];
     return i >= 0 && i < width ? (int)i : -1;
-}
-__device__ __forceinline__ float target_weight(const Target &t, int64_t r, int v, int index) {
-    return t.kind == C6_TARGET_WEIGHTS ? ((const float *)t.p)[r * t.stride + v] : (v == index ? 1.f : 0.f);
-}
-
-// target weights of the N entries from column c on, of nv columns; `index`: the column of an index target
-template <int N, bool WEIGHTS>
-__device__ __forceinline__ void get_weights(const float *weights, int c, int nv, int index, float (&q)[N]) {
-    if (!WEIGHTS) {
-#pragma unroll
-        for (int i = 0; i < N; i++) q[i] = c + i == index ? 1.f : 0.f;
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < N; i += 4) {
-        float f[4];
-        if (c + N <= nv) C6Vec<float>::get(C6Vec<float>::load(weights + c + i), f);
-        else C6Vec<float>::get_some(weights + c + i, nv - c - i, 0.f, f);
-#pragma unroll
-        for (int j = 0; j < 4; j++) q[i + j] = f[j];
-    }
 }
 
 // What is known of some legal entries of a row: their maximum m, s = sum exp(x - m), w = sum t, d = sum t (m - x).  All terms of s, w and d are
@@ -266,7 +258,7 @@ struct Beside {
     const uint8_t *mask;
     int64_t byte;
     template <int N>
-    __device__ __forceinline__ uint32_t bits(int, int c) const { return mask ? (uint32_t)mask[(int64_t)(c >> 3) * byte] >> (N == 4 ? c & 4 : 0) : ~0u; }
+    __device__ __forceinline__ uint32_t bits(int, int c) const { return mask ? legal_bits<N>(mask[(int64_t)(c >> 3) * byte], c) : ~0u; }
     __device__ __forceinline__ bool legal(int c) const { return !mask || (mask[(int64_t)(c >> 3) * byte] >> (c & 7) & 1); }
     // weights: 0 where illegal
     template <int N>
@@ -296,39 +288,40 @@ struct Beside {
 template <typename T, int LANES, int NV, bool WEIGHTS>
 struct Fetched {
     static constexpr int N = C6Vec<T>::N;
-    uint32_t ok[NV];
+    uint32_t byte[NV], tail_byte;
     c6_u32x4 w[WEIGHTS ? NV : 1][N / 4];
-    bool any, tail_ok;
+    bool any;
     float tail_w;
 
-    __device__ __forceinline__ Fetched(const Beside &at, const Held<T, LANES, NV> &h, int lane) : any(at.mask), tail_ok(true), tail_w(0.f) {
+    __device__ __forceinline__ Fetched(const Beside &at, const Held<T, LANES, NV> &h, int lane) : tail_byte(0xff), any(at.mask), tail_w(0.f) {
 #pragma unroll
         for (int u = 0; u < NV; u++) {
-            const int c = (u * LANES + lane) * N;
-            ok[u] = ~0u;
+            const int c = h.column(u, lane);
+            byte[u] = 0xff;
             if (!h.has(u, lane)) continue;
-            if (any) ok[u] = at.template bits<N>(u, c);
+            if (any) byte[u] = at.mask[(int64_t)(c >> 3) * at.byte];
             if constexpr (WEIGHTS)
 #pragma unroll
                 for (int i = 0; i < N / 4; i++) w[u][i] = C6Vec<float>::load(at.weights + c + 4 * i);
         }
         if (lane < h.rest) {
             const int c = h.whole * N + lane;
-            if (any) tail_ok = at.legal(c);
+            if (any) tail_byte = at.mask[(int64_t)(c >> 3) * at.byte];
             if (WEIGHTS) tail_w = at.weights[c];
         }
     }
     // the mask goes into the row and its weights, once
-    __device__ __forceinline__ void settle(Held<T, LANES, NV> &h, int) {
+    __device__ __forceinline__ void settle(Held<T, LANES, NV> &h, int lane) {
         if (!any) return;
 #pragma unroll
         for (int u = 0; u < NV; u++) {
-            C6Vec<T>::keep(h.raw[u], ok[u]);
+            const uint32_t ok = legal_bits<N>(byte[u], h.column(u, lane));
+            C6Vec<T>::keep(h.raw[u], ok);
             if constexpr (WEIGHTS)
 #pragma unroll
-                for (int i = 0; i < N; i++) w[u][i / 4][i % 4] &= C6Vec<T>::ones(ok[u], i);
+                for (int i = 0; i < N; i++) w[u][i / 4][i % 4] &= C6Vec<T>::ones(ok, i);
         }
-        if (!tail_ok) { h.tail = -INFINITY; tail_w = 0.f; }
+        if (!(tail_byte >> ((h.whole * N + lane) & 7) & 1)) { h.tail = -INFINITY; tail_w = 0.f; }
     }
     template <int M>
     __device__ __forceinline__ void get(int u, int, float (&q)[M]) const {
@@ -571,47 +564,71 @@ __global__ __launch_bounds__(256) void c6_policy_loss_join_kernel(Rows l, Target
 
 // The gradient from what the forward pass saved: elementwise, in chunks like those of c6_logits_process_kernel.  Bound by memory: 777 x 32768 f16 against
 // weights 35 us for 206 MB (5.9 TB/s).
-constexpr int GRAD_WAVE = 1024, GRAD_BLOCK = 4096;
-
 template <typename T, int LANES, bool WEIGHTS>
 __global__ __launch_bounds__(256) void c6_policy_loss_grad_kernel(Rows l, Target t, const float *lse, const float *total, const float *dloss, int64_t dloss_stride,
                                                                   T *grad, int64_t grad_stride) {
     typedef C6Vec<T> V;
-    constexpr int CHUNK = LANES == 64 ? GRAD_WAVE : GRAD_BLOCK, U = CHUNK / (LANES * V::N), PER = 256 / LANES;
+    constexpr int CHUNK = chunk_of<LANES>, U = CHUNK / (LANES * V::N), PER = 256 / LANES;
     const int lane = threadIdx.x % LANES, part = threadIdx.x / LANES;
     const int chunks = (l.width + CHUNK - 1) / CHUNK;
     const int64_t items = (int64_t)l.rows * chunks;
     for (int64_t item = (int64_t)blockIdx.x * PER + part; item < items; item += (int64_t)gridDim.x * PER) {
         const int64_t r = item / chunks;
         const int v0 = (int)(item % chunks) * CHUNK, nv = min(CHUNK, l.width - v0);
+        const int whole = nv / V::N, rest = nv % V::N, last = whole * V::N + lane;
         const T *x = (const T *)l.x + r * l.x_stride + v0;
         T *g = grad + r * grad_stride + v0;
-        const float *weights = WEIGHTS ? (const float *)t.p + r * t.stride + v0 : nullptr;
-        const uint8_t *mask = l.mask ? l.mask + r * l.mask_row : nullptr;
-        c6_u32x4 raw[U];
+        const Beside at = beside<WEIGHTS>(l, t, r, v0);
+        c6_u32x4 raw[U], w[WEIGHTS ? U : 1][V::N / 4];
+        uint32_t bits[U], tail_bits = 0xff;
+        T tail = c6_put<T>(0.f);
+        float tail_w = 0.f;
+        if (whole) {
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int c = (u * LANES + lane) * V::N;
-            if (c + V::N <= nv) raw[u] = V::load(x + c);
+            for (int u = 0; u < U; u++) {
+                const int c = min(u * LANES + lane, whole - 1) * V::N;
+                raw[u] = V::load(x + c);
+                bits[u] = at.mask ? at.mask[(int64_t)(c >> 3) * at.byte] : 0xff;
+                if constexpr (WEIGHTS)
+#pragma unroll
+                    for (int i = 0; i < V::N / 4; i++) w[u][i] = C6Vec<float>::load(at.weights + c + 4 * i);
+            }
         }
-        const int index = target_index(t, r, l.width) - v0;      // of this chunk; elsewhere or none: outside it
-        const float z = lse[r], scale = dloss[r * dloss_stride], w = total[r];
+        if (lane < rest) {
+            tail = x[last];
+            if (at.mask) tail_bits = at.mask[(int64_t)(last >> 3) * at.byte];
+            if (WEIGHTS) tail_w = at.weights[last];
+        }
+        // of this chunk; another chunk's lies outside its columns, and so does none
+        const int index = WEIGHTS ? -1 : target_index(t, r, l.width) - v0;
+        const float z = lse[r], scale = dloss[r * dloss_stride], factor = scale * total[r];
         const bool some = z != -INFINITY;
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int c = (u * LANES + lane) * V::N;
-            if (c >= nv) continue;
-            const bool whole = c + V::N <= nv;
-            float y[V::N], q[V::N];
-            if (whole) V::get(raw[u], y);
-            else V::get_some(x + c, nv - c, 0.f, y);
-            get_weights<V::N, WEIGHTS>(weights, c, nv, index, q);
-            uint32_t ok = some ? ~0u : 0u;
-            if (mask) ok &= legal_bits<V::N>(l, mask, v0 + c);
+            if (u * LANES + lane >= whole) continue;
+            float f[V::N];
+            V::get(raw[u], f);
 #pragma unroll
-            for (int i = 0; i < V::N; i++) y[i] = ok >> i & 1 ? scale * (w * expf(y[i] - z) - q[i]) : 0.f;
-            if (whole) V::store(g + c, V::put(y));
-            else V::put_some(g + c, nv - c, y);
+            for (int i = 0; i < V::N; i++) f[i] = factor * exp_of(f[i] - z);
+            if constexpr (WEIGHTS) {
+#pragma unroll
+                for (int i = 0; i < V::N; i++) {
+                    const uint32_t q = w[u][i / 4][i % 4];
+                    f[i] = __builtin_fmaf(-scale, __builtin_bit_cast(float, q), f[i]);
+                }
+            } else if ((unsigned)(index - c) < (unsigned)V::N) {
+#pragma unroll
+                for (int i = 0; i < V::N; i++) f[i] -= c + i == index ? scale : 0.f;
+            }
+            const uint32_t ok = some ? legal_bits<V::N>(bits[u], c) : 0u;
+#pragma unroll
+            for (int i = 0; i < V::N; i++) f[i] = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, f[i]) & C6Vec<float>::ones(ok, i));      // 0 where illegal
+            V::store(g + c, V::put(f));
+        }
+        if (lane < rest) {
+            const float q = WEIGHTS ? tail_w : (last == index ? 1.f : 0.f);
+            g[last] = c6_put<T>(some && tail_bits >> (last & 7) & 1 ? __builtin_fmaf(-scale, q, factor * exp_of(c6_get(tail) - z)) : 0.f);
         }
     }
 }
@@ -670,9 +687,14 @@ int check_target(const c6_logits *l, const void *target, int kind, int64_t strid
     return C6_OK;
 }
 
-// workgroups for all chunks of all rows, `per` chunks a workgroup (what exceeds the grid's limit is looped over)
-unsigned grid_of(const c6_logits *l, int chunk, int per) {
-    const int64_t items = (int64_t)l->rows * ((l->width + chunk - 1) / chunk);
+// four rows a wave once that still leaves every SIMD one (the loss of 16384 x 361 bf16 against weights: 13.2 instead of 14.9 us, of 1024 rows 5.2 instead of 3.8)
+constexpr int MANY = 4096;
+
+// the lanes that share a chunk of a row, and the workgroups for all chunks of all rows (what exceeds the grid's limit is looped over)
+int lanes_of(const c6_logits *l) { return l->rows >= MANY && l->width <= chunk_of<16> ? 16 : l->width <= chunk_of<64> ? 64 : 256; }
+template <int LANES>
+unsigned grid_of(const c6_logits *l) {
+    const int64_t items = (int64_t)l->rows * ((l->width + chunk_of<LANES> - 1) / chunk_of<LANES>), per = 256 / LANES;
     return (unsigned)std::min<int64_t>((items + per - 1) / per, 1 << 22);
 }
 
@@ -707,18 +729,19 @@ extern "C" int c6_logits_process(const c6_logits *l, const int32_t *history, int
     C6DeviceScope scope(l->device);
     if (!scope.ok) return c6_set_error(C6_ERR_HIP, "c6_logits_process: hipSetDevice");
     const Repeats h{history, history_len, penalties, history_stride, penalties_stride, history_cap};
-    const bool wave = l->width <= PROCESS_WAVE;
-    const unsigned grid = grid_of(l, wave ? PROCESS_WAVE : PROCESS_BLOCK, wave ? 4 : 1);
 #define C6_LAUNCH(LANES, HIST, BIAS)                                                                                                                        \
-    C6_BY_TYPE(l->type, T, hipLaunchKernelGGL((c6_logits_process_kernel<T, LANES, HIST, BIAS>), dim3(grid), dim3(256), 0, (hipStream_t)stream, rows_of(l), \
+    C6_BY_TYPE(l->type, T, hipLaunchKernelGGL((c6_logits_process_kernel<T, LANES, HIST, BIAS>), dim3(grid_of<LANES>(l)), dim3(256), 0, (hipStream_t)stream, rows_of(l), \
                                               h, bias, bias_stride, (T *)out, out_stride))
 #define C6_LAUNCH_LANES(LANES)                         \
     if (history && bias) C6_LAUNCH(LANES, true, true); \
     else if (history) C6_LAUNCH(LANES, true, false);   \
     else if (bias) C6_LAUNCH(LANES, false, true);      \
     else C6_LAUNCH(LANES, false, false)
-    if (wave) { C6_LAUNCH_LANES(64); }
-    else { C6_LAUNCH_LANES(256); }
+    switch (lanes_of(l)) {
+    case 16: C6_LAUNCH_LANES(16); break;
+    case 64: C6_LAUNCH_LANES(64); break;
+    default: C6_LAUNCH_LANES(256);
+    }
 #undef C6_LAUNCH_LANES
 #undef C6_LAUNCH
     return launched();
@@ -744,9 +767,6 @@ extern "C" size_t c6_policy_loss_workspace(int rows, int width) {
         if (rows > 0 && splits(rows, width, n, true, false)) need = std::max(need, split_bytes(rows, width, n));
     return need;
 }
-
-// four rows a wave once that still leaves every SIMD one: 16384 x 361 bf16 against weights 13.2 instead of 14.9 us, 1024 rows 5.2 instead of 3.8
-constexpr int MANY = 4096;
 
 template <typename T, bool WEIGHTS>
 static void loss_launch(const c6_logits *l, const Target &t, float *loss, float *lse, float *total, T *grad, int64_t grad_stride, float scale, void *workspace, hipStream_t s) {
@@ -819,16 +839,15 @@ extern "C" int c6_policy_loss_grad(const c6_logits *l, const void *target, int t
     C6DeviceScope scope(l->device);
     if (!scope.ok) return c6_set_error(C6_ERR_HIP, "c6_policy_loss_grad: hipSetDevice");
     const Target t{target, target_stride, target_kind};
-    const bool wave = l->width <= GRAD_WAVE;
-    const unsigned grid = grid_of(l, wave ? GRAD_WAVE : GRAD_BLOCK, wave ? 4 : 1);
 #define C6_LAUNCH(LANES, WEIGHTS)                                                                                                                          \
-    C6_BY_TYPE(l->type, T, hipLaunchKernelGGL((c6_policy_loss_grad_kernel<T, LANES, WEIGHTS>), dim3(grid), dim3(256), 0, (hipStream_t)stream, rows_of(l), t, \
+    C6_BY_TYPE(l->type, T, hipLaunchKernelGGL((c6_policy_loss_grad_kernel<T, LANES, WEIGHTS>), dim3(grid_of<LANES>(l)), dim3(256), 0, (hipStream_t)stream, rows_of(l), t, \
                                               lse, total, dloss, dloss_stride, (T *)grad, grad_stride))
     const bool weights = target_kind == C6_TARGET_WEIGHTS;
-    if (wave && weights) C6_LAUNCH(64, true);
-    else if (wave) C6_LAUNCH(64, false);
-    else if (weights) C6_LAUNCH(256, true);
-    else C6_LAUNCH(256, false);
+    switch (lanes_of(l)) {
+    case 16: if (weights) C6_LAUNCH(16, true); else C6_LAUNCH(16, false); break;
+    case 64: if (weights) C6_LAUNCH(64, true); else C6_LAUNCH(64, false); break;
+    default: if (weights) C6_LAUNCH(256, true); else C6_LAUNCH(256, false);
+    }
 #undef C6_LAUNCH
     return launched();
 }
