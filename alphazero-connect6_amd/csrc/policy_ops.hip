@@ -24,13 +24,13 @@ template <int N>
 __device__ __forceinline__ uint32_t legal_bits(uint32_t byte, int c) { return byte >> (N == 4 ? c & 4 : 0); }
 
 // ---- penalties, biases, masks -------------------------------------------------------------------------------------------
-// Bound by memory: every logit in and out once.  A row is cut into chunks; LANES threads take one chunk: a wave for rows of up to 1024 entries (four rows a
-// workgroup), else a workgroup per 4096 (with histories of up to 8191 ids 512 rows of 131072 f32 took 131 us so, 143 in chunks of 8192, 210 of 16384: a
-// larger chunk scans the history less often but leaves fewer waves).  The chunk's logits, mask and bias are requested first, 16 bytes a lane and all in
-// flight, and wait in registers while the row's history is counted in LDS: each chunk reads the whole history and counts the ids that fall into it
-// (integer adds: the order does not matter).
-// Measured, kernel alone: 512 x 131072 f32 96 us without mask and history (5.6 TB/s; a copy of that size 99), 121 us with both; 48 x 100003 bf16 with 2048
-// ids, mask and bias 9.7 us; 4096 x 361 f32 with 200 moves, legal masks and bias 7.8 us; one row of 361 2.2 us.
+// Bound by memory: every logit in and out once.  A row is cut into chunks; LANES threads take one chunk: of many rows of up to 384 entries 16 lanes each
+// (lanes_of()), a wave for rows of up to 1024, else a workgroup per 4096 (48 rows of 100003 bf16 with up to 2048 ids take 8.8 us so, 10.8 in chunks of
+// 8192: a larger chunk scans the history less often but leaves fewer waves).  The chunk's logits, mask and bias and the history's beginning are requested
+// first, 16 bytes a lane and all in flight, and wait in registers while the row's history is counted in LDS: each chunk reads the whole history and counts
+// the ids that fall into it (integer adds: the order does not matter).  Asking for the history's length only once the row had come cost 15 % of the time.
+// Measured, kernel alone: 512 x 131072 f32 96 us without mask and history (5.6 TB/s; a copy of that size 99), 104 us with both; 48 x 100003 bf16 with 2048
+// ids, mask and bias 9.2 us; 4096 x 361 f32 with 200 moves, legal masks and bias 7.2 us; one row of 361 2.0 us.
 struct Repeats {
     const int32_t *history, *len;
     const float *penalties;
@@ -62,6 +62,17 @@ __global__ __launch_bounds__(256) void c6_logits_process_kernel(Rows l, Repeats 
         T *o = out + r * out_stride + v0;
         const uint8_t *mask = l.mask ? l.mask + r * l.mask_row : nullptr;
         const float *b = BIAS ? bias + r * bias_stride + v0 : nullptr;
+        // the first ids of a lane are asked for with the row, whatever the history's length (the room of `cap` ids is the caller's)
+        const int32_t *ids = HIST ? h.history + r * h.history_stride : nullptr;
+        const float *p = HIST ? h.penalties + r * h.penalties_stride : nullptr;
+        float rep = 1.f, freq = 0.f, pres = 0.f;
+        int n = 0;
+        c6_u32x4 early{0, 0, 0, 0};
+        if (HIST) {
+            n = min(h.len ? h.len[r] : h.cap, h.cap);
+            rep = p[0]; freq = p[1]; pres = p[2];
+            if (lane * 4 + 4 <= h.cap) early = C6Vec<float>::load((const float *)ids + lane * 4);
+        }
         // every lane loads U pieces, behind the last one that again: no branch stands between the loads
         c6_u32x4 raw[U], add[BIAS ? U : 1][V::N / 4];
         uint32_t bits[U], tail_bits = 0xff;
@@ -83,22 +94,21 @@ __global__ __launch_bounds__(256) void c6_logits_process_kernel(Rows l, Repeats 
             if (mask) tail_bits = mask[(int64_t)((v0 + last) >> 3) * l.mask_byte];
             if (BIAS) tail_add = b[last];
         }
-        float rep = 1.f, freq = 0.f, pres = 0.f;
         if (HIST) {
-            const float *p = h.penalties + r * h.penalties_stride;
-            rep = p[0]; freq = p[1]; pres = p[2];
             for (int c = lane * 4; c < nv; c += LANES * 4) *reinterpret_cast<uint4 *>(count + c) = uint4{0, 0, 0, 0};
             meet();
-            const int32_t *ids = h.history + r * h.history_stride;
-            const int n = min(h.len ? h.len[r] : h.cap, h.cap);
             const auto seen = [&](int32_t id) {
                 const uint32_t at = (uint32_t)id - (uint32_t)v0;      // (an id below v0, or below 0, wraps to far beyond nv)
                 if (at < (uint32_t)nv) atomicAdd(&count[at], 1u);
             };
-            // 8 ids of a lane in flight: the loop is bound by the latency of its loads, and what more of them gain costs waves (512 rows of 131072 f32 with up to
-            // 8191 ids: 4 in flight 127 us, 8 121 us, 16 131 us)
+            // 8 ids of a lane in flight (64 rows of 131072 bf16 with up to 8191 ids: 4 in flight 13.3 us, 8 13.1, 16 14.5)
             constexpr int FLIGHT = 2;
             int i = lane * 4;
+            if (i + 4 <= h.cap) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) seen(i + j < n ? (int32_t)early[j] : -1);
+                i += LANES * 4;
+            }
             for (; i + 4 + (FLIGHT - 1) * LANES * 4 <= n; i += FLIGHT * LANES * 4) {
                 c6_u32x4 q[FLIGHT];
 #pragma unroll
@@ -132,8 +142,7 @@ __global__ __launch_bounds__(256) void c6_logits_process_kernel(Rows l, Repeats 
                 for (int i = 0; i < V::N; i++) any |= k[i];
                 if (any)
 #pragma unroll
-                    for (int i = 0; i < V::N; i++)
-                        if (k[i]) y[i] = less(y[i], k[i]);
+                    for (int i = 0; i < V::N; i++) y[i] = k[i] ? less(y[i], k[i]) : y[i];
             }
             if constexpr (BIAS) {
 #pragma unroll
@@ -165,10 +174,12 @@ struct Target {
     int64_t stride;
     int kind;
 };
-__device__ __forceinline__ int target_index(const Target &t, int64_t r, int width) {      // -1: none
+// -1: none.  Both kinds are read as 32-bit words, no branch before the load; width <= 2^30, so a low word below it is not negative
+__device__ __forceinline__ int target_index(const Target &t, int64_t r, int width) {
     if (t.kind == C6_TARGET_WEIGHTS) return -1;
-    const int64_t i = t.kind == C6_TARGET_INDEX64 ? ((const int64_t *)t.p)[r] : ((const int32_t *)t.p)[r];
-    return i >= 0 && i < width ? (int)i : -1;
+    const int words = t.kind == C6_TARGET_INDEX64 ? 2 : 1;
+    const int32_t *p = (const int32_t *)t.p + r * words, low = p[0], high = p[words - 1];
+    return (uint32_t)low < (uint32_t)width && (words == 1 || high == 0) ? low : -1;
 }
 
 // What is known of some legal entries of a row: their maximum m, s = sum exp(x - m), w = sum t, d = sum t (m - x).  All terms of s, w and d are
@@ -579,6 +590,9 @@ __global__ __launch_bounds__(256) void c6_policy_loss_grad_kernel(Rows l, Target
         const T *x = (const T *)l.x + r * l.x_stride + v0;
         T *g = grad + r * grad_stride + v0;
         const Beside at = beside<WEIGHTS>(l, t, r, v0);
+        // what the row has one of, asked for before its entries.  index: of this chunk; another chunk's lies outside its columns, and so does none
+        const int index = WEIGHTS ? -1 : target_index(t, r, l.width) - v0;
+        const float z = lse[r], scale = dloss[r * dloss_stride], sum = total[r];
         c6_u32x4 raw[U], w[WEIGHTS ? U : 1][V::N / 4];
         uint32_t bits[U], tail_bits = 0xff;
         T tail = c6_put<T>(0.f);
@@ -599,9 +613,7 @@ __global__ __launch_bounds__(256) void c6_policy_loss_grad_kernel(Rows l, Target
             if (at.mask) tail_bits = at.mask[(int64_t)(last >> 3) * at.byte];
             if (WEIGHTS) tail_w = at.weights[last];
         }
-        // of this chunk; another chunk's lies outside its columns, and so does none
-        const int index = WEIGHTS ? -1 : target_index(t, r, l.width) - v0;
-        const float z = lse[r], scale = dloss[r * dloss_stride], factor = scale * total[r];
+        const float factor = scale * sum;
         const bool some = z != -INFINITY;
 #pragma unroll
         for (int u = 0; u < U; u++) {
@@ -687,11 +699,18 @@ int check_target(const c6_logits *l, const void *target, int kind, int64_t strid
     return C6_OK;
 }
 
-// four rows a wave once that still leaves every SIMD one (the loss of 16384 x 361 bf16 against weights: 13.2 instead of 14.9 us, of 1024 rows 5.2 instead of 3.8)
-constexpr int MANY = 4096;
+// Four rows a wave once that still leaves every SIMD one; 16 lanes count a history for longer, and take twice the rows for it.  Four rows a wave against
+// one, 361 wide, us:  rows                         2048         4096         8192        32768
+//   process, bias, f32                        3.5 / 3.3    4.2 / 4.6    6.8 / 7.3  16.6 / 18.3
+//   process, bias, 50 ids, bf16               6.0 / 4.6    6.2 / 5.6    8.1 / 9.7  18.3 / 24.6
+//   loss, index, bf16                         3.3 / 3.3    3.4 / 4.0    4.1 / 5.8   9.8 / 17.0
+//   loss and gradient, weights, f32           4.4 / 3.9    5.5 / 5.7    8.6 / 8.7  26.8 / 25.9
+//   gradient alone, weights, bf16             3.2 / 3.3    3.9 / 4.4    6.3 / 6.6  16.3 / 18.1
+// (81 wide: 2048 rows within 0.2 us of one another, 32768 by half to two thirds faster).
+constexpr int MANY = 4096, MANY_HISTORIES = 2 * MANY;
 
 // the lanes that share a chunk of a row, and the workgroups for all chunks of all rows (what exceeds the grid's limit is looped over)
-int lanes_of(const c6_logits *l) { return l->rows >= MANY && l->width <= chunk_of<16> ? 16 : l->width <= chunk_of<64> ? 64 : 256; }
+int lanes_of(const c6_logits *l, int many = MANY) { return l->rows >= many && l->width <= chunk_of<16> ? 16 : l->width <= chunk_of<64> ? 64 : 256; }
 template <int LANES>
 unsigned grid_of(const c6_logits *l) {
     const int64_t items = (int64_t)l->rows * ((l->width + chunk_of<LANES> - 1) / chunk_of<LANES>), per = 256 / LANES;
@@ -737,7 +756,7 @@ extern "C" int c6_logits_process(const c6_logits *l, const int32_t *history, int
     else if (history) C6_LAUNCH(LANES, true, false);   \
     else if (bias) C6_LAUNCH(LANES, false, true);      \
     else C6_LAUNCH(LANES, false, false)
-    switch (lanes_of(l)) {
+    switch (lanes_of(l, history ? MANY_HISTORIES : MANY)) {
     case 16: C6_LAUNCH_LANES(16); break;
     case 64: C6_LAUNCH_LANES(64); break;
     default: C6_LAUNCH_LANES(256);

@@ -98,6 +98,30 @@ def test_process(i, shape, kind):
         assert torch.equal(w.nan_to_num(nan=99.0), y.nan_to_num(nan=99.0))
 
 
+# Many narrow rows: from 4096 rows (8192 with a history) of up to 384 entries on, 16 lanes take a row; a case on each side of each border.  The history's
+# room: too small for one 16-byte load, just enough, ragged, longer than what the lanes of a row read at once.
+@pytest.mark.parametrize("rows,width,kind,mask,cap", [
+    (4095, 361, "f32", "rows", 3), (4096, 361, "f32", "soa", 4), (8191, 225, "bf16", "rows", 63), (8192, 225, "bf16", "soa", 64), (8193, 361, "f16", "shared", 65),
+    (8192, 384, "f32", "none", 200), (8192, 385, "f32", "rows", 200), (9001, 81, "f32", "soa", 50), (8200, 3, "bf16", "rows", 7), (8192, 7, "f16", "rows", 1),
+    (10001, 8, "f32", "shared", 5), (8197, 361, "bf16", "rows", 700), (8192, 1, "f32", "rows", 2), (8200, 383, "f32", "soa", 3)], ids=str)
+def test_process_of_many_rows(rows, width, kind, mask, cap):
+    torch, ops, _ = setup()
+    rng = np.random.default_rng(rows + width + cap)
+    x, vals, m, packed = make(rows, width, kind, width, mask, pad=width % 4, lead=cap % 3)
+    hist = rng.integers(-1, width + 1, (rows, cap)).astype(np.int32)
+    lens = rng.integers(-1, cap + 2, rows).astype(np.int32)
+    pen = np.stack([rng.uniform(0.5, 2, rows), rng.uniform(-0.5, 0.5, rows), rng.uniform(0, 1, rows)], 1).astype(np.float32)
+    bias = rng.normal(0, 2, (rows, width)).astype(np.float32)
+    for case in ({}, {"bias": bias[0]}, {"history": hist, "history_len": lens, "penalties": pen}, {"history": hist, "penalties": pen[0], "bias": bias}):
+        want, tol = po.process(vals, packed, **case)
+        dev = {k: torch.tensor(v, device="cuda") for k, v in case.items()}
+        y = ops.logits_process(x, mask=m, **dev)
+        po.near(host(y), want, tol, kind, ("process", rows, width, kind, list(case)))
+        buf = torch.full((rows, width + 3), 7.0, dtype=x.dtype, device="cuda")
+        z = ops.logits_process(x, mask=m, out=buf[:, 1:width + 1], **dev)
+        assert torch.equal(z.nan_to_num(nan=99.0), y.nan_to_num(nan=99.0)) and bool((buf[:, 0] == 7).all()) and bool((buf[:, width + 1:] == 7).all())
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("target", ["index32", "index64", "weights"])
 @pytest.mark.parametrize("i,shape", list(enumerate(SHAPES)), ids=lambda s: str(s))
