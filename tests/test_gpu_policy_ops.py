@@ -181,6 +181,8 @@ WAYS = [(4096, 81, "f32", "index32", "rows"), (4097, 225, "bf16", "weights", "so
         (300, 8193, "f32", "weights", "rows"), (600, 16385, "f32", "index32", "none"), (520, 40001, "bf16", "weights", "shared"), (300, 65536, "bf16", "weights", "none"),
         (300, 65537, "bf16", "weights", "rows"), (300, 65537, "bf16", "index32", "rows"), (129, 65536, "f32", "index64", "rows"), (130, 65537, "f32", "index32", "none"),
         (128, 32769, "f32", "index32", "rows"), (129, 32769, "f32", "index32", "rows"), (257, 131072, "f16", "index32", "none"), (2, 1000003, "bf16", "weights", "rows"),
+        (257, 99001, "bf16", "index64", "rows"), (300, 50001, "f32", "index32", "soa"), (320, 98313, "f16", "index64", "shared"), (321, 98313, "f16", "index32", "rows"),
+        (256, 50001, "f32", "index32", "rows"), (513, 49157, "f32", "index32", "rows"),
         (2, 9000001, "f32", "index32", "rows"), (1, 9000001, "f16", "weights", "none")]      # (more chunks than workgroups a row)
 
 
