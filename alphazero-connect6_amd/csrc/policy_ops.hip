@@ -738,6 +738,7 @@ extern "C" int c6_logits_process(const c6_logits *l, const int32_t *history, int
     if (int rc = check_written(l, out, out_stride, "c6_logits_process: out is NULL")) return rc;
     if (history) {
         if (history_cap < 0 || history_stride < 0 || penalties_stride < 0) return bad("c6_logits_process: negative size or stride of the history");
+        if (history_cap > 1 << 30) return bad("c6_logits_process: a row of the history has at most 2^30 ids");      // (the kernel's index steps past its end)
         if (!penalties) return bad("c6_logits_process: a history needs penalties");
         if (!c6_aligned(history, 4) || !c6_aligned(penalties, 4) || !c6_aligned(history_len, 4)) return bad("c6_logits_process: a history, its lengths and penalties are aligned to 4 bytes");
         if (!fits(l->rows, history_stride, history_cap, 4) || !fits(l->rows, penalties_stride, 3, 4)) return bad("c6_logits_process: the history exceeds the address space");

@@ -53,6 +53,8 @@ def _logits(x, mask):
     if device < 0 or len(shape) != 2:
         raise C6Error("logits must be a [rows, width] tensor of float32, float16 or bfloat16 on the GPU")
     rows, width = shape
+    if rows > 0x7fffffff or width > 1 << 30:      # (the C struct's fields would take the low 32 bits)
+        raise C6Error("logits must have at most 2^31 - 1 rows of at most 2^30 entries")
     stride, step = x.stride()
     if step != 1 and width > 1:
         raise C6Error("the entries of a row of logits must lie next to each other")
@@ -120,6 +122,8 @@ def logits_process(logits, mask=None, bias=None, history=None, history_len=None,
         if not isinstance(history, _Tensor) or history.dim() not in (1, 2) or penalties is None:
             raise C6Error("history must be an int32 tensor [rows, cap] or [cap], and needs penalties")
         cap = history.shape[-1]
+        if cap > 1 << 30:
+            raise C6Error("a row of the history has at most 2^30 ids")
         h, hs = _rows_by(history, _I32, dev, rows, cap, "history")
         p, ps = _rows_by(penalties, _F32, dev, rows, 3, "penalties")
         if history_len is not None:

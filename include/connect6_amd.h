@@ -594,8 +594,8 @@ typedef struct c6_logits {
  * (repetition, frequency, presence) = penalties[r * penalties_stride + 0 .. 2], in 32 bits:
  *     y = x;   if c > 0:  y = (x > 0 ? x / repetition : x * repetition) - (frequency * c + presence);
  *     y += bias[r * bias_stride + v];      an entry that is not legal: y = -infinity, whatever x is
- * and out = y rounded once to the type.  history (int32) NULL: no penalties; a row of it is history_cap ids of readable memory, of which those
- * behind history_len[r] hold anything; history_len NULL: every row has history_cap ids; bias NULL:
+ * and out = y rounded once to the type.  history (int32) NULL: no penalties; a row of it is history_cap (<= 2^30) ids of readable memory, of which
+ * those behind history_len[r] hold anything; history_len NULL: every row has history_cap ids; bias NULL:
  * none.  Strides in elements, >= 0 (0: shared by the rows).  out may be x itself (same pointer and stride) and overlaps nothing else. */
 int c6_logits_process(const c6_logits *l, const int32_t *history, int64_t history_stride, const int32_t *history_len, int history_cap,
                       const float *penalties, int64_t penalties_stride, const float *bias, int64_t bias_stride, void *out, int64_t out_stride,

@@ -382,6 +382,20 @@ def test_python_refusals():
         c.norm()
 
 
+def test_sizes_beyond_32_bits_are_refused():
+    """their low 32 bits would be sizes that can be worked on"""
+    torch, ops, _ = setup()
+    one = torch.zeros(1, 1, device="cuda")
+    for rows, width in ((1 << 31, 1), ((1 << 32) + 2, 1), (1, (1 << 30) + 1), (1, (1 << 32) + 5)):
+        x = one.expand(rows, width)
+        for call in (lambda: ops.logits_process(x, out=x), lambda: ops.policy_loss(x, torch.zeros(1, dtype=torch.int32, device="cuda"))):
+            with pytest.raises(pkg.C6Error, match="2\\^30"):
+                call()
+    ids = torch.zeros(1, dtype=torch.int32, device="cuda").expand((1 << 32) + 3)
+    with pytest.raises(pkg.C6Error, match="2\\^30"):
+        ops.logits_process(one, history=ids, penalties=torch.ones(3, device="cuda"))
+
+
 # ---- clipping -------------------------------------------------------------------------------------------------------------
 def clip_case(torch, dts, sizes, kinds, seed, spread=4, lead=1):
     """tensors of `sizes` at odd addresses, scales apart by orders of magnitude"""

@@ -44,7 +44,7 @@ def test_null_logits():
 @pytest.mark.parametrize("kw", [dict(out=None), dict(out=4 * A + 2), dict(os=9), dict(os=-10), dict(os=1 << 62), dict(out=A, os=11), dict(out=A + 4), dict(out=A + 4 * 35),
                                 dict(history=A), dict(history=A, cap=-1, pen=A), dict(history=A, cap=3, pen=A, hs=-3), dict(history=A, cap=3, pen=A, ps=-3),
                                 dict(history=A + 1, cap=3, pen=A), dict(history=A, cap=3, pen=A + 2), dict(history=A, cap=3, pen=A, n=A + 1),
-                                dict(history=A, cap=3, pen=A, hs=1 << 62), dict(bias=A, bs=-1), dict(bias=A + 3), dict(bias=A, bs=1 << 62)])
+                                dict(history=A, cap=3, pen=A, hs=1 << 62), dict(history=A, cap=(1 << 30) + 1, pen=A), dict(bias=A, bs=-1), dict(bias=A + 3), dict(bias=A, bs=1 << 62)])
 def test_bad_process_arguments(kw):
     assert process(logits(), **kw) == BAD
 
