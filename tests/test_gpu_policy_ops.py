@@ -183,6 +183,9 @@ WAYS = [(4096, 81, "f32", "index32", "rows"), (4097, 225, "bf16", "weights", "so
         (128, 32769, "f32", "index32", "rows"), (129, 32769, "f32", "index32", "rows"), (257, 131072, "f16", "index32", "none"), (2, 1000003, "bf16", "weights", "rows"),
         (257, 99001, "bf16", "index64", "rows"), (300, 50001, "f32", "index32", "soa"), (320, 98313, "f16", "index64", "shared"), (321, 98313, "f16", "index32", "rows"),
         (256, 50001, "f32", "index32", "rows"), (513, 49157, "f32", "index32", "rows"),
+        (300, 12288, "f32", "weights", "rows"), (300, 12289, "f32", "weights", "rows"), (300, 24576, "bf16", "index32", "soa"), (300, 24577, "bf16", "weights", "none"),
+        (300, 24576, "f32", "index64", "rows"), (300, 24577, "f32", "weights", "rows"), (300, 49153, "f16", "index32", "none"), (300, 49152, "bf16", "weights", "rows"),
+        (300, 49152, "f32", "index32", "rows"), (300, 98305, "bf16", "index64", "none"), (300, 57344, "f32", "index64", "none"), (300, 114689, "f16", "index32", "rows"),
         (2, 9000001, "f32", "index32", "rows"), (1, 9000001, "f16", "weights", "none")]      # (more chunks than workgroups a row)
 
 
