@@ -465,10 +465,10 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void c6_policy_loss_kern
         int lane = threadIdx.x % LANES;
         asm volatile("" : "+v"(lane));      // (what follows from it is computed in every turn, not kept in registers across them)
         const T *x = (const T *)l.x + r * l.x_stride;
-        // what is beside a row is fetched with it where there are registers to hold it (2048 x 16001 f32 against weights: 84 instead of 119 us), else as it is
-        // needed
+        // what is beside a row is fetched with it where there are registers to hold it (2048 x 16001 f32 against weights: 84 instead of 119 us;
+        // 2049 x 100003 bf16 with masks, against the move: 203 instead of 241), else as it is needed
         auto at = [&] {
-            if constexpr (LANES <= 64 || (WEIGHTS && (LANES < 1024 || NV * V::N <= 32))) return Fetched<T, LANES, NV, WEIGHTS>(beside<WEIGHTS>(l, t, r, 0), h, lane);
+            if constexpr (!WEIGHTS || LANES < 1024 || NV * V::N <= 32) return Fetched<T, LANES, NV, WEIGHTS>(beside<WEIGHTS>(l, t, r, 0), h, lane);
             else return beside<WEIGHTS>(l, t, r, 0);
         }();
         int index = -1;
@@ -497,7 +497,8 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void c6_policy_loss_kern
 }
 
 // The same in two launches, for rows that do not fit or are too few to fill the card: every chunk's Part into the workspace, then each chunk joins its
-// row's and writes its piece of the gradient.  3 x 131072 f32: 3.2 + 4.6 us; without a gradient 2048 x 100003 bf16 77 us (5.3 TB/s).
+// row's and writes its piece of the gradient.  3 x 131072 f32: 3.2 + 4.6 us; without a gradient 2048 x 100003 bf16 77 us (5.3 TB/s) and 7; with
+// masks both together 101, where masks read only as they are needed made it 114.
 constexpr int SPLIT_NV = 4, JOIN_MOST = 1024;
 template <typename T>
 constexpr int split_chunk = 256 * SPLIT_NV * C6Vec<T>::N;
@@ -513,7 +514,7 @@ __global__ __launch_bounds__(256) void c6_policy_loss_part_kernel(Rows l, Target
         const T *x = (const T *)l.x + r * l.x_stride;
         Held<T, 256, SPLIT_NV> h(min(l.width - v0, split_chunk<T>));
         h.request(x + v0, lane);
-        Beside here = beside<WEIGHTS>(l, t, r, v0);
+        Fetched<T, 256, SPLIT_NV, WEIGHTS> here(beside<WEIGHTS>(l, t, r, v0), h, lane);
         const Part p = block_part<256>(part_of<T, 256, SPLIT_NV, WEIGHTS>(h, here, lane), WEIGHTS, space);
         if (lane == 0) parts[item] = p;
         if (!WEIGHTS && lane == 0) {      // (the gradient may go where x is: the second launch does not read the entry again)
@@ -560,7 +561,7 @@ __global__ __launch_bounds__(256) void c6_policy_loss_join_kernel(Rows l, Target
                 h = Held<T, 256, SPLIT_NV>(min(l.width - v0, split_chunk<T>));
                 h.request(x + v0, lane);
             }
-            Beside here = beside<WEIGHTS>(l, t, r, v0);
+            Fetched<T, 256, SPLIT_NV, WEIGHTS> here(beside<WEIGHTS>(l, t, r, v0), h, lane);
             T *g = grad + r * grad_stride + v0;
             const int at_index = index < 0 ? -1 : index - v0;      // (of another chunk: outside this one's columns)
             here.settle(h, lane);
