@@ -448,7 +448,7 @@ __device__ __forceinline__ void gradient(float x, const At &at, const Done &k, i
 // One pass over rows that fit the registers of LANES lanes: read once, the gradient written once.  A lane takes the maximum of its own entries, the sums
 // relative to that, and one reduction over the lanes joins them.  As a piece's gradient leaves, the same piece of the workgroup's next row is requested
 // into its registers: loads and stores overlap, and the sums of a row begin as its first pieces arrive.
-// Measured, loss and gradient: 2049 x 100003 bf16 187 us (4.4 TB/s; 1020 in three passes over each row).  There a workgroup has a CU to itself (97 registers
+// Measured, loss and gradient: 2049 x 100003 bf16 187 us (4.4 TB/s; 1020 in three passes over each row).  There a workgroup has a CU to itself (up to 122 registers
 // a lane, 16 waves) and the vector unit is busy for half the time, two exponentials an element of it: what is left over the 149 us of a copy is the part of
 // that work which one row's loads do not cover, a row address aligned to two bytes (3 us), and the 2049th row.  2048 x 16000 f32 45 us (5.8 TB/s),
 // 16384 x 361 bf16 against weights 12 us, 2048 x 225 f32 4 us.
