@@ -18,17 +18,13 @@
 //         position (position-outer order: 2 + 8 accumulator tiles per wave instead of 32), epilogue = bias + residual + ReLU +
 //         16-byte NHWC stores of the 2x2 pixels of every tile.
 //         Schedule = the f32n one: persistent workgroups; wave w owns output channels [32w, 32w + 32) for all 64 tiles of the
-//         block, so its transformed weights are private and stream L2 -> VGPR three 8-channel groups ahead (no weight staging
+//         block, so its transformed weights are private and stream L2 -> VGPR seven 8-channel groups ahead (no weight staging
 //         in LDS); V_p (64 x (C + 4) floats) lands in LDS by LDS-DMA as a linear copy one position ahead, double-buffered;
 //         ONE barrier per position.
 //         Weights are the MFMA A operand (D = U x V): a lane's accumulators are 16-byte NHWC runs of one tile.
 // MFMA operand mapping (as in conv_f32n.hip): one ds_read_b128 gives lane (tile j, h) channels 8u + 4h .. + 3 of group u; MFMA r
 // of the group contracts the channel pair (8u + r, 8u + 4 + r); weight lane (cout i, h) holds U_p[i][8u + 4h + r].
-#include "c6_device.h"
-#include "c6_engine.h"
-
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
+#include "c6_wino.h"
 
 #define WINO_BT 64      // tiles per block
 #define WINO_PF 7       // weight groups in flight ahead of the one being multiplied (ring of 8)
@@ -167,18 +163,8 @@ __global__ void c6_wino_tail_kernel(float *__restrict__ V, long total_tiles) {
 }
 
 // ---- GEMM + output transform ---------------------------------------------------------------------------------------
-// Every vector-memory operation of the main loop is issued by hand (inline asm) because vmcnt retires IN ORDER: a weight load
-// issued behind the slab DMAs cannot be waited for without waiting for them.  With the compiler's own loads its s_waitcnt
-// counts do not see the DMAs and wait for far too much; here each wait names exactly the operations that are younger than
-// the group it needs: the WINO_PF weight groups behind it, plus the ND slab DMAs while those are younger too.
-// operations younger than the weights of group i when they are waited for, SPREAD schedule (see the kernel)
-constexpr int wino_wait(int i, int nd) {
-    const int lo = i - WINO_PF > 0 ? i - WINO_PF : 0, hi = (nd - 1 < i - 1) ? nd - 1 : i - 1;
-    return WINO_PF + (hi >= lo ? hi - lo + 1 : 0);
-}
-#define WINO_ULOAD(dst, voff, base) asm volatile("global_load_dwordx4 %0, %1, %2" : "=v"(dst) : "v"(voff), "s"(base) : "memory")
-#define WINO_UWAIT(dst, n) asm volatile("s_waitcnt vmcnt(%1)" : "+v"(dst) : "n"(n) : "memory")
-
+// Weights: loads that the compiler sees, waits for and counts.  The slab's LDS-DMAs are asm (c6_stream.h) and retire in the same order: the compiler's waits,
+// which do not count them, make the DMAs of some groups ago land early, and the barrier waits for what is older than the WINO_PF youngest requests.
 template <int C, int N>
 __global__ __launch_bounds__(64 * (C / 32)) void c6_wino_gemm_kernel(const float *__restrict__ V, const float *__restrict__ U,
                                                                      const float *__restrict__ bias, const float *__restrict__ res,
@@ -189,6 +175,7 @@ __global__ __launch_bounds__(64 * (C / 32)) void c6_wino_gemm_kernel(const float
     constexpr int ND = (NCH + WAVES - 1) / WAVES;    // slab DMAs per wave and position (the same count in every wave)
     static_assert(PF == 7 && NG % 8 == 0, "ring of 8 weight groups, 7 in flight");
     constexpr bool SPREAD = NG >= 16 && ND <= 16;    // one slab DMA per group instead of all of them behind the barrier (C >= 128)
+    static_assert((SPREAD ? NG - ND : NG) >= PF, "c6_dma_barrier: that many requests follow a position's last DMA");
     extern __shared__ __attribute__((aligned(16))) float wsm[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int j = lane & 31, h = lane >> 5;
@@ -197,7 +184,7 @@ __global__ __launch_bounds__(64 * (C / 32)) void c6_wino_gemm_kernel(const float
     if (b >= nblocks) return;
 
     // this wave's transformed weights: [wave][pos][group][lane][4] floats, one linear 1-KiB-per-group stream per block
-    const float *ubase = U + (size_t)wave * NGT * 256;
+    const auto weights = c6_weights(U);
     const unsigned lane16 = (unsigned)lane * 16u;
 
     // LDS-DMA of one (block, position) slab: NCH linear 1-KiB chunks, chunk c by wave c mod WAVES; a wave whose last turn
@@ -208,7 +195,7 @@ __global__ __launch_bounds__(64 * (C / 32)) void c6_wino_gemm_kernel(const float
         c = c < NCH ? c : NCH - 1;
         const float *gp = src + (size_t)c * 256;
         const int lds_off = (buf * SLAB + c * 256) * 4;
-        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane16), "s"(gp), "s"(lds_off) : "memory");
+        c6_dma(gp, lane16, lds_off);
     };
     auto dma_slab = [&](const float *src, int buf) {
 #pragma unroll
@@ -218,7 +205,10 @@ __global__ __launch_bounds__(64 * (C / 32)) void c6_wino_gemm_kernel(const float
     dma_slab(V + (size_t)b * G::BLOCK_FLOATS, 0);
     f32x4 ring[8];
 #pragma unroll
-    for (int q = 0; q < PF; q++) WINO_ULOAD(ring[q], lane16 + (unsigned)q * 1024u, ubase);
+    for (int q = 0; q < PF; q++) {
+        int uoff = (wave * NGT + q) * 1024;
+        ring[q] = c6_request<f32x4>(weights, lane16, uoff);
+    }
     int gi = PF;                                     // next weight group to request, 0 .. NGT-1 (wraps: the next block's)
 
 #pragma unroll 1
@@ -268,13 +258,12 @@ __global__ __launch_bounds__(64 * (C / 32)) void c6_wino_gemm_kernel(const float
             }
         }
 
-        __builtin_amdgcn_s_waitcnt(0x0F70);          // vmcnt(0), as a builtin: the compiler's own wait bookkeeping sees the residual loads retired
+        __builtin_amdgcn_s_waitcnt(0x0F70);          // vmcnt(0): what is pending in front of the loop the compiler would wait for in every one of its turns
 #pragma unroll 1
         for (int p = 0; p < 16; p++) {
             // the slab of position p (issued one position ago) has landed: only the PF youngest operations -- weight
             // requests, all younger than those DMAs -- may still be in flight
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PF) : "memory");
-            __syncthreads();
+            c6_dma_barrier<PF>();
             const float *nsrc;
             {
                 int nb = p < 15 ? b : b + (int)gridDim.x;
@@ -290,13 +279,13 @@ __global__ __launch_bounds__(64 * (C / 32)) void c6_wino_gemm_kernel(const float
             // (SPREAD: issue one slab DMA in the shadow of the MFMAs), 2 x 4 MFMAs.
             // (u) + 1 == NG reads one group into the row padding / the next row: loaded, never used.
             f32x4 va0 = *reinterpret_cast<const f32x4 *>(vb), va1 = *reinterpret_cast<const f32x4 *>(vb + 32 * CP), vn0, vn1;
-#define WINO_GROUP(q, u, NWAIT, DMA)                                                                             \
+#define WINO_GROUP(q, u, DMA)                                                                                    \
             {                                                                                                    \
-                WINO_ULOAD(ring[((q) + PF) & 7], lane16 + (unsigned)gi * 1024u, ubase);                          \
+                int uoff = (wave * NGT + gi) * 1024;                                                             \
+                ring[((q) + PF) & 7] = c6_request<f32x4>(weights, lane16, uoff);                                          \
                 gi = gi + 1 == NGT ? 0 : gi + 1;                                                                 \
                 vn0 = *reinterpret_cast<const f32x4 *>(vb + 8 * ((u) + 1 < NG ? (u) + 1 : (u)));                 \
                 vn1 = *reinterpret_cast<const f32x4 *>(vb + 32 * CP + 8 * ((u) + 1 < NG ? (u) + 1 : (u)));       \
-                WINO_UWAIT(ring[(q)], NWAIT);                                                                    \
                 const f32x4 w = ring[(q)];                                                                       \
                 __builtin_amdgcn_sched_barrier(0);                                                               \
                 m0 = __builtin_amdgcn_mfma_f32_32x32x2f32(w[0], va0[0], m0, 0, 0, 0);                            \
@@ -310,24 +299,23 @@ __global__ __launch_bounds__(64 * (C / 32)) void c6_wino_gemm_kernel(const float
                 va0 = vn0; va1 = vn1;                                                                            \
             }
             if (SPREAD) {
-                // DMA k is issued in group k, behind that group's weight wait: younger than the weights of group i are its 7
-                // followers plus the DMAs k with max(0, i - 7) <= k <= min(ND - 1, i - 1)   (wino_wait)
-#define WG_(i) WINO_GROUP((i) & 7, (i), wino_wait((i), ND), (i))
+                // DMA k is issued in group k
+#define WG_(i) WINO_GROUP((i) & 7, (i), (i))
                 WG_(0) WG_(1) WG_(2) WG_(3) WG_(4) WG_(5) WG_(6) WG_(7) WG_(8) WG_(9) WG_(10) WG_(11) WG_(12) WG_(13) WG_(14) WG_(15)
 #undef WG_
 #pragma unroll 1
                 for (int u0 = 16; u0 < NG; u0 += 8) {
-                    WINO_GROUP(0, u0, PF, -1) WINO_GROUP(1, u0 + 1, PF, -1) WINO_GROUP(2, u0 + 2, PF, -1) WINO_GROUP(3, u0 + 3, PF, -1)
-                    WINO_GROUP(4, u0 + 4, PF, -1) WINO_GROUP(5, u0 + 5, PF, -1) WINO_GROUP(6, u0 + 6, PF, -1) WINO_GROUP(7, u0 + 7, PF, -1)
+                    WINO_GROUP(0, u0, -1) WINO_GROUP(1, u0 + 1, -1) WINO_GROUP(2, u0 + 2, -1) WINO_GROUP(3, u0 + 3, -1)
+                    WINO_GROUP(4, u0 + 4, -1) WINO_GROUP(5, u0 + 5, -1) WINO_GROUP(6, u0 + 6, -1) WINO_GROUP(7, u0 + 7, -1)
                 }
             } else {
-                // all ND DMAs went out before group 0; groups 0..6 were requested before them: those DMAs are younger too
-                WINO_GROUP(0, 0, PF + ND, -1) WINO_GROUP(1, 1, PF + ND, -1) WINO_GROUP(2, 2, PF + ND, -1) WINO_GROUP(3, 3, PF + ND, -1)
-                WINO_GROUP(4, 4, PF + ND, -1) WINO_GROUP(5, 5, PF + ND, -1) WINO_GROUP(6, 6, PF + ND, -1) WINO_GROUP(7, 7, PF, -1)
+                // all ND DMAs went out before group 0
+                WINO_GROUP(0, 0, -1) WINO_GROUP(1, 1, -1) WINO_GROUP(2, 2, -1) WINO_GROUP(3, 3, -1)
+                WINO_GROUP(4, 4, -1) WINO_GROUP(5, 5, -1) WINO_GROUP(6, 6, -1) WINO_GROUP(7, 7, -1)
 #pragma unroll 1
                 for (int u0 = 8; u0 < NG; u0 += 8) {
-                    WINO_GROUP(0, u0, PF, -1) WINO_GROUP(1, u0 + 1, PF, -1) WINO_GROUP(2, u0 + 2, PF, -1) WINO_GROUP(3, u0 + 3, PF, -1)
-                    WINO_GROUP(4, u0 + 4, PF, -1) WINO_GROUP(5, u0 + 5, PF, -1) WINO_GROUP(6, u0 + 6, PF, -1) WINO_GROUP(7, u0 + 7, PF, -1)
+                    WINO_GROUP(0, u0, -1) WINO_GROUP(1, u0 + 1, -1) WINO_GROUP(2, u0 + 2, -1) WINO_GROUP(3, u0 + 3, -1)
+                    WINO_GROUP(4, u0 + 4, -1) WINO_GROUP(5, u0 + 5, -1) WINO_GROUP(6, u0 + 6, -1) WINO_GROUP(7, u0 + 7, -1)
                 }
             }
 #undef WINO_GROUP

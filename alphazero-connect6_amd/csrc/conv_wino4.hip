@@ -10,7 +10,7 @@
 //   c6_wino4_gemm_kernel  Z[block][tile][row i][b][cout] = sum_j A^T[b][j] sum_cin U_ij[cout][cin] V[block][tile][ij][cin]:
 //                         conv_wino.hip's schedule (persistent workgroups, wave w owns couts [32w, 32w+32) x 64 tiles, weights L2 ->
 //                         VGPR through a ring of 8 groups, V slabs by LDS-DMA one position ahead, one barrier per position); positions
-//                         j = 0 and j = 5 of a row accumulate straight into Z, j = 1 .. 4 aside + a few packed vector instructions;
+//                         j = 0 and j = 5 of a row accumulate straight into Z, j = 1 .. 4 aside + a few vector instructions;
 //                         a row's Z is stored while the next row accumulates.  MFMA bound, at the part's power limit
 //   c6_wino4_in_kernel    activations NHWC -> V[block][tile 64][pos 36][C]      HBM bound: reads 1x, writes 36/16 x the activations
 //   c6_wino4_out_kernel   A^T Z + bias (+ residual), ReLU -> activations NHWC   HBM bound: reads 24/16 x + 1x, writes 1x;
@@ -309,10 +309,9 @@ static bool w4_has_tail(int nboards) {
 // persistent workgroups of 8 waves; wave w owns couts [32w, 32w + 32) x 64 tiles, so its transformed weights are private and stream
 // L2 -> VGPR as one linear 1-KiB-per-group sequence 7 groups ahead (ring of 8; 16 changed nothing); V_p (64 tile rows of 1 KiB) lands in
 // LDS by LDS-DMA one position ahead, double-buffered, rows padded to C + 4 floats (conflict-free ds_read_b128); one barrier per position.
-//  * Vector-memory operations retire IN ORDER on one counter (loads, LDS-DMAs and stores alike), and the compiler's own s_waitcnt
-//    counts do not see inline-asm operations: all of the loop's are issued by hand and every wait names exactly the operations younger
-//    than the weight group it needs (w4_wait): the 7 groups behind it, the slab DMAs (group k < 8 issues DMA k of the next position) and
-//    the result stores issued since (one per group, groups 8 .. 23 of the positions that store).
+//  * Weights, DMAs and results: c6_stream.h.  The compiler's wait for a weight group counts the requests and result stores behind it (one store per group,
+//    groups 8 .. 23 of the positions that store), not the slab DMAs (group k < 8 issues DMA k of the next position): behind those it is up to eight operations
+//    too early, about half of the 7 groups ahead.
 //  * The FP32 matrix instructions run on the lanes of the vector ALU (their peak IS the vector FP32 peak; a kernel of plain vector
 //    instructions beside this one on another stream makes no progress at all): every vector instruction in the loop is matrix time
 //    lost.  The weight stream advances a SCALAR pointer, the tile fragments alternate between two register sets instead of being
@@ -322,11 +321,14 @@ static bool w4_has_tail(int nboards) {
 //    accumulated in registers -- one row at a time, 4 x 32 registers -- and 24 instead of 36 values per (tile, cout) go to memory: a third
 //    less for this kernel to write and for the boundary kernel behind it to read.  A^T = [1 1 1 1 1 0; 0 1 -1 2 -2 0; 0 1 1 4 4 0;
 //    0 1 -1 8 -8 1]: position j = 0 accumulates straight into Z_0 and j = 5 straight into Z_3 (the MFMA's own accumulate); j = 1 .. 4
-//    accumulate aside and cost 40 packed vector instructions per position on average -- the one exception to the rule above: +1.5 % on
+//    accumulate aside and cost 80 vector instructions per position on average -- the one exception to the rule above: +1.5 % on
 //    this kernel, -19 % on the boundary kernels (same box, in the engine: 248.4 -> 236.8 ms per round).  Stores: Z_0, Z_1 during position
 //    j = 5 of their row, Z_2, Z_3 during j = 0 of the next.  Result: Zo[block][tile 64][row i 6][b 4][C].
+// The vector-memory operations younger than group i's weights when they are multiplied: the requests of the W4_PF groups behind it, the slab DMAs (nd a wave and
+// position; eight waves: 8, the four-wave jobs: 16) and the result stores issued since.  The kernel asserts from these that a position's DMAs have landed
+// by its end and that a split job leaves no request behind.
 constexpr int w4_store_group(int k) { return 8 + k; }      // store k (0 .. 15) of a storing position goes out in group 8 + k
-constexpr int w4_wait(int i, bool stores, int nd = 8) {      // nd: slab DMAs per wave and position (8 waves: 8; the four-wave jobs of the tiniest batches: 16)
+constexpr int w4_wait(int i, bool stores, int nd = 8) {
     const int lo = i - W4_PF > 0 ? i - W4_PF : 0, hi = (nd - 1 < i - 1) ? nd - 1 : i - 1;
     const int dmas = hi >= lo ? hi - lo + 1 : 0;
     int st = 0;
@@ -336,8 +338,7 @@ constexpr int w4_wait(int i, bool stores, int nd = 8) {      // nd: slab DMAs pe
     return W4_PF + dmas + st;
 }
 static_assert(w4_store_group(15) < 32 - W4_PF, "a position's stores are older than every request that is waited for in the next one");
-// the LAST position of a split job (SPLIT below, r5): the weight stream ends with the row and no next position is fetched -- younger than group i's
-// request are only the groups i + 1 .. 31 and the result stores issued since
+// ... in the last position of a split job: its weight stream ends with the row and no next position is fetched
 constexpr int w4_wait_last(int i) {
     int st = 0;
     for (int k = 0; k < 16; k++)
@@ -350,13 +351,15 @@ constexpr int w4_wait_last(int i) {
 // position, bit-identical sums; every job has its own prologue, its last position requests nothing beyond the row (LP).  For small batches.
 // HW (split form only): half-width jobs of FOUR waves (128 of the 256 output channels, blockIdx.z) for the tiniest batches, as conv_wino6.hip's.
 template <int N, bool SPLIT, bool HW = false>
-__global__ __launch_bounds__(HW ? 256 : 64 * (W4_C / 32)) void c6_wino4_gemm_kernel(const float *__restrict__ V, const float *__restrict__ U,
+__global__ __launch_bounds__(HW ? 256 : 64 * (W4_C / 32), 2) void c6_wino4_gemm_kernel(const float *__restrict__ V, const float *__restrict__ U,
                                                                                     float *__restrict__ Zo, int nblocks, int blkB, int blkBP) {
     using G = W4Geom<N>;
     static_assert(!HW || SPLIT, "half-width jobs exist in the split form only");
     constexpr int C = G::C, CP = G::CP, SLAB = G::SLAB, WAVES = HW ? 4 : G::WAVES, NG = G::NG, PF = W4_PF;
     constexpr int ND = W4_BT / WAVES;
     static_assert(PF == 7 && NG == 32 && (ND == 8 || ND == 16), "ring of 8 weight groups; 8 (four waves: 16) DMAs per wave and position");
+    static_assert(NG - ND >= PF && w4_wait(NG - 1, true, ND) == PF, "c6_dma_barrier: that many requests, and nothing else, are younger than a position's last DMA at its end");
+    static_assert(w4_wait_last(NG - 1) == 0, "a split job leaves nothing in flight but its last stores");
     constexpr int RM = PF;
     constexpr int ZTILE = 24 * C;                    // floats of a tile in Zo
     constexpr size_t ZBLOCK = (size_t)W4_BT * ZTILE;
@@ -373,43 +376,26 @@ __global__ __launch_bounds__(HW ? 256 : 64 * (W4_C / 32)) void c6_wino4_gemm_ker
     // weight sets at 36 C^2 and 66 C^2); a set is packed [wave][position][group][lane][4]
     auto rows_of = [&](int blk) { return blk < blkB ? 6 : 5; };
     auto wbase_of = [&](int blk) {
-        return blk < blkB ? U + (size_t)cw * (W4_NP * NG * 256)
-                          : U + (size_t)(blk < blkBP ? W4_NP : W4_NP + W4_NP_EDGE) * C * C + (size_t)cw * (W4_NP_EDGE * NG * 256);
+        return 4 * (blk < blkB ? cw * (W4_NP * NG * 256) : (blk < blkBP ? W4_NP : W4_NP + W4_NP_EDGE) * C * C + cw * (W4_NP_EDGE * NG * 256));      // byte
     };
     const unsigned lane16 = (unsigned)lane * 16u;
-    const unsigned zoff0 = (unsigned)(((size_t)j * ZTILE + n4) * 4), zoff1 = zoff0 + (unsigned)((size_t)32 * ZTILE * 4);
+    const unsigned zoff = (unsigned)(j * ZTILE + n4) * 4u;
 
     auto dma_chunk = [&](const float *src, int buf, int c0) {
         const int c = c0 * WAVES + wave;
         const float *gp = src + (size_t)c * G::TILE_STRIDE;
         const int lds_off = (buf * SLAB + c * CP) * 4;
-        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane16), "s"(gp), "s"(lds_off) : "memory");
+        c6_dma(gp, lane16, lds_off);
     };
     f32x4 ring[PF + 1];
-    int ub = b, ungt = rows_of(b) * 6 * NG;      // the weight stream runs ahead of the multiplications: its own block and group counters
-    const float *uptr = wbase_of(b);
-    int gi = 0;
-#define W4_UNEXT()                                                       \
-    {                                                                    \
-        uptr += 256;                                                     \
-        if (!SPLIT) {                                                    \
-            gi += 1;                                                     \
-            if (gi == ungt) {                                            \
-                gi = 0;                                                  \
-                ub = ub + (int)gridDim.x < nblocks ? ub + (int)gridDim.x : ub; \
-                ungt = rows_of(ub) * 6 * NG;                             \
-                uptr = wbase_of(ub);                                     \
-            }                                                            \
-        }                                                                \
-    }
-    // the first position's V rows into slab 0, the first seven weight groups into the ring (SPLIT: per job; the empty asm keeps the job's group
-    // addresses from being hoisted out of the block loop into scalar registers)
+    const auto weights = c6_weights(U);
+    int uoff = wbase_of(b);      // the next group of the weight stream, seven ahead of the multiplications
+    // the first position's V rows into slab 0, the first seven weight groups into the ring (SPLIT: per job)
 #define W4_PROLOGUE(ROW)                                                                                         \
     {                                                                                                            \
         _Pragma("unroll") for (int c0 = 0; c0 < ND; c0++) dma_chunk(V + (size_t)b * G::BLOCK_FLOATS + (size_t)(6 * (ROW)) * G::POS_STRIDE, 0, c0); \
-        uptr = wbase_of(b) + (size_t)(6 * (ROW)) * (NG * 256);                                                   \
-        if (SPLIT) asm volatile("" : "+s"(uptr));                                                                \
-        _Pragma("unroll") for (int q = 0; q < PF; q++) { W4_ULOAD(ring[q], lane16, uptr); W4_UNEXT() }           \
+        uoff = wbase_of(b) + 6 * (ROW) * (NG * 1024);                                                            \
+        _Pragma("unroll") for (int q = 0; q < PF; q++) { ring[q] = c6_request<f32x4>(weights, lane16, uoff); uoff += 1024; }           \
     }
     if (!SPLIT) W4_PROLOGUE(0)
 
@@ -425,13 +411,7 @@ __global__ __launch_bounds__(HW ? 256 : 64 * (W4_C / 32)) void c6_wino4_gemm_ker
     {                                                                                                            \
         const f32x16 &sv = ((k) & 4) ? SET1 : SET0;                                                              \
         const f32x4 a = {sv[4 * ((k) & 3)], sv[4 * ((k) & 3) + 1], sv[4 * ((k) & 3) + 2], sv[4 * ((k) & 3) + 3]}; \
-        /* SPLIT: the second tile half's offset rides in the scalar base (one vector register less) */         \
-        const float *d_ = (DST) + (size_t)(BIDX) * C + (SPLIT && ((k) & 4) ? (size_t)32 * ZTILE : (size_t)0);   \
-        const unsigned zo_ = SPLIT ? zoff0 : ((k) & 4) ? zoff1 : zoff0;                                          \
-        if (((k) & 3) == 0) W4_STORE(zo_, a, d_, 0);                                                             \
-        else if (((k) & 3) == 1) W4_STORE(zo_, a, d_, 32);                                                       \
-        else if (((k) & 3) == 2) W4_STORE(zo_, a, d_, 64);                                                       \
-        else W4_STORE(zo_, a, d_, 96);                                                                           \
+        c6_put16(c6_buffer(DST, ZBLOCK * 4), zoff, (((k) & 4) * 8 * ZTILE + (BIDX) * C + 8 * ((k) & 3)) * 4, a);  \
     }
 #define W4Z_LAST_ROW()                                                                                           \
     {                                                                                                            \
@@ -439,17 +419,20 @@ __global__ __launch_bounds__(HW ? 256 : 64 * (W4_C / 32)) void c6_wino4_gemm_ker
         _Pragma("unroll") for (int k = 0; k < 8; k++) W4Z_STORE1(z30, z31, 3, zprev, k)                           \
     }
     // JJ = position's column j: 0 accumulates into z0 from zero, 5 into z3 on top of it, 1 .. 4 into m from zero
-#define W4Z_GROUP(q, u, NWAIT, DMA, JJ, BUF, LP)                                                                 \
+// Products and row sums stand where they are written: values pass through volatile asm, and such statements keep their order.  Without it only the compiler's
+// habit keeps the 256 products of a position between its loads and barriers (one form had them behind all its loads, and 39 registers spilled).
+#define W4Z_PIN(Z) asm volatile("" : "+v"(Z));
+#define W4Z_GROUP(q, u, DMA, JJ, BUF, LP)                                                                        \
             {                                                                                                    \
-                if (!(LP) || (u) + PF < NG) {      /* (LP: a request nobody waits for lands in registers the compiler has given to something else) */ \
-                    W4_ULOAD(ring[((q) + PF) & RM], lane16, uptr);                                               \
-                    W4_UNEXT()                                                                                   \
+                if (!(LP) || (u) + PF < NG) {      /* (LP: the job's last position requests nothing beyond its row) */ \
+                    if ((u) + PF == NG) uoff = last ? next_w : uoff;      /* (the next position's first group) */ \
+                    ring[((q) + PF) & RM] = c6_request<f32x4>(weights, lane16, uoff);                                     \
+                    uoff += 1024;                                                                                \
                 }                                                                                                \
                 if ((u) + 1 < NG) {                                                                              \
                     va[((u) + 1) & 1][0] = *reinterpret_cast<const f32x4 *>(vb + 8 * ((u) + 1));                 \
                     va[((u) + 1) & 1][1] = *reinterpret_cast<const f32x4 *>(vb + 32 * CP + 8 * ((u) + 1));       \
                 }                                                                                                \
-                W4_UWAIT(ring[(q)], NWAIT);                                                                      \
                 const f32x4 w = ring[(q)];                                                                       \
                 __builtin_amdgcn_sched_barrier(0);                                                               \
                 if ((JJ) == 0) {                                                                                 \
@@ -483,24 +466,19 @@ __global__ __launch_bounds__(HW ? 256 : 64 * (W4_C / 32)) void c6_wino4_gemm_ker
                         m1 = __builtin_amdgcn_mfma_f32_32x32x2f32(w[r], va[(u) & 1][1][r], m1, 0, 0, 0);         \
                     }                                                                                            \
                 }                                                                                                \
+                if ((JJ) == 0) { W4Z_PIN(z00) W4Z_PIN(z01) }                                                      \
+                else if ((JJ) == 5) { W4Z_PIN(z30) W4Z_PIN(z31) }                                                 \
+                else { W4Z_PIN(m0) W4Z_PIN(m1) }                                                                  \
                 __builtin_amdgcn_sched_barrier(0);                                                               \
             }
-#define WGZ_(i, JJ, BUF) W4Z_GROUP((i) & RM, (i), (SPLIT && (JJ) == 5) ? w4_wait_last((i)) : w4_wait((i), (!SPLIT && (JJ) == 0) || (JJ) == 5, ND), (i), JJ, BUF, SPLIT && (JJ) == 5)
+#define WGZ_(i, JJ, BUF) W4Z_GROUP((i) & RM, (i), (i), JJ, BUF, SPLIT && (JJ) == 5)
     // one position (row i_, column JJ): slab in LDS buffer JJ & 1
 #define W4Z_POSITION(i_, JJ)                                                                                     \
         {                                                                                                        \
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PF) : "memory");                                            \
-            __builtin_amdgcn_s_barrier();                                                                        \
-            const float *nsrc;                                                                                   \
-            {                                                                                                    \
-                const int pp = 6 * (i_) + (JJ);                                                                  \
-                if (SPLIT) nsrc = V + (size_t)b * G::BLOCK_FLOATS + (size_t)(pp + 1) * G::POS_STRIDE;      /* (not used by the job's last position) */ \
-                else {                                                                                           \
-                    int nb = pp < 6 * R - 1 ? b : b + (int)gridDim.x;                                            \
-                    nb = nb < nblocks ? nb : b;                                                                  \
-                    nsrc = V + (size_t)nb * G::BLOCK_FLOATS + (size_t)(pp < 6 * R - 1 ? pp + 1 : 0) * G::POS_STRIDE; \
-                }                                                                                                \
-            }                                                                                                    \
+            c6_dma_barrier<PF>();                                                                               \
+            const int pp = 6 * (i_) + (JJ);                                                                      \
+            const bool last = !SPLIT && (JJ) == 5 && pp == 6 * R - 1;      /* the block's last position: the next one is the next block's first */ \
+            const float *here = V + (size_t)b * G::BLOCK_FLOATS + (size_t)(pp + 1) * G::POS_STRIDE, *nsrc = last ? next_v : here; \
             const float *vb = wsm + ((JJ) & 1) * SLAB + j * CP + 4 * h;                                          \
             f32x4 va[2][2];                                                                                      \
             va[0][0] = *reinterpret_cast<const f32x4 *>(vb);                                                     \
@@ -515,26 +493,36 @@ __global__ __launch_bounds__(HW ? 256 : 64 * (W4_C / 32)) void c6_wino4_gemm_ker
             WGZ_(28, JJ, (JJ) & 1) WGZ_(29, JJ, (JJ) & 1) WGZ_(30, JJ, (JJ) & 1) WGZ_(31, JJ, (JJ) & 1)                 \
         }
     // the vector part: Z_b += A^T[b][JJ] * M for the columns that accumulate aside (A^T[.][1..4] = (1,1,1,1), (1,-1,1,-1), (1,2,4,8), (1,-2,4,-8))
+// One register set after the other, each in place, nothing scheduled across: with the 16 values of all eight sets interleaved old and new sets were alive side by
+// side and the block form spilled 37 registers.
+#define W4Z_ALL(Z, EXPR) { _Pragma("unroll") for (int v = 0; v < 16; v++) Z[v] = (EXPR); __builtin_amdgcn_sched_barrier(0); }
 #define W4Z_UPDATE(JJ)                                                                                           \
-        _Pragma("unroll") for (int v = 0; v < 16; v++) {                                                         \
-            z00[v] += m0[v]; z01[v] += m1[v];                                                                    \
-            if ((JJ) == 1) { z10[v] = m0[v]; z11[v] = m1[v]; z20[v] = m0[v]; z21[v] = m1[v]; z30[v] = m0[v]; z31[v] = m1[v]; } \
-            if ((JJ) == 2) { z10[v] -= m0[v]; z11[v] -= m1[v]; z20[v] += m0[v]; z21[v] += m1[v]; z30[v] -= m0[v]; z31[v] -= m1[v]; } \
-            if ((JJ) == 3) {                                                                                     \
-                z10[v] = __builtin_fmaf(2.f, m0[v], z10[v]); z11[v] = __builtin_fmaf(2.f, m1[v], z11[v]);        \
-                z20[v] = __builtin_fmaf(4.f, m0[v], z20[v]); z21[v] = __builtin_fmaf(4.f, m1[v], z21[v]);        \
-                z30[v] = __builtin_fmaf(8.f, m0[v], z30[v]); z31[v] = __builtin_fmaf(8.f, m1[v], z31[v]);        \
-            }                                                                                                    \
-            if ((JJ) == 4) {                                                                                     \
-                z10[v] = __builtin_fmaf(-2.f, m0[v], z10[v]); z11[v] = __builtin_fmaf(-2.f, m1[v], z11[v]);      \
-                z20[v] = __builtin_fmaf(4.f, m0[v], z20[v]); z21[v] = __builtin_fmaf(4.f, m1[v], z21[v]);        \
-                z30[v] = __builtin_fmaf(-8.f, m0[v], z30[v]); z31[v] = __builtin_fmaf(-8.f, m1[v], z31[v]);      \
-            }                                                                                                    \
+        W4Z_ALL(z00, z00[v] + m0[v]) W4Z_ALL(z01, z01[v] + m1[v])                                                \
+        if ((JJ) == 1) { z10 = m0; z11 = m1; z20 = m0; z21 = m1; z30 = m0; z31 = m1; }                           \
+        if ((JJ) == 2) {                                                                                         \
+            W4Z_ALL(z30, z30[v] - m0[v]) W4Z_ALL(z31, z31[v] - m1[v])                                            \
+            W4Z_ALL(z20, z20[v] + m0[v]) W4Z_ALL(z21, z21[v] + m1[v])                                            \
+            z10 = z30; z11 = z31;                                                                                \
+        }                                                                                                        \
+        if ((JJ) == 3) {                                                                                         \
+            W4Z_ALL(z10, __builtin_fmaf(2.f, m0[v], z10[v])) W4Z_ALL(z11, __builtin_fmaf(2.f, m1[v], z11[v]))    \
+            W4Z_ALL(z20, __builtin_fmaf(4.f, m0[v], z20[v])) W4Z_ALL(z21, __builtin_fmaf(4.f, m1[v], z21[v]))    \
+            W4Z_ALL(z30, __builtin_fmaf(8.f, m0[v], z30[v])) W4Z_ALL(z31, __builtin_fmaf(8.f, m1[v], z31[v]))    \
+        }                                                                                                        \
+        if ((JJ) == 4) {                                                                                         \
+            W4Z_ALL(z10, __builtin_fmaf(-2.f, m0[v], z10[v])) W4Z_ALL(z11, __builtin_fmaf(-2.f, m1[v], z11[v]))  \
+            W4Z_ALL(z20, __builtin_fmaf(4.f, m0[v], z20[v])) W4Z_ALL(z21, __builtin_fmaf(4.f, m1[v], z21[v]))    \
+            W4Z_ALL(z30, __builtin_fmaf(-8.f, m0[v], z30[v])) W4Z_ALL(z31, __builtin_fmaf(-8.f, m1[v], z31[v]))  \
+            W4Z_PIN(z00) W4Z_PIN(z01) W4Z_PIN(z10) W4Z_PIN(z11) W4Z_PIN(z20) W4Z_PIN(z21) W4Z_PIN(z30) W4Z_PIN(z31) \
         }
 
 #pragma unroll 1
     for (; b < nblocks; b += gridDim.x) {
         const int R = rows_of(b);
+        // what follows the block's last position (behind the last block: its own first, which nobody multiplies)
+        const int next = SPLIT ? b : b + (int)gridDim.x < nblocks ? b + (int)gridDim.x : b;
+        const float *next_v = V + (size_t)next * G::BLOCK_FLOATS;
+        const int next_w = wbase_of(next);
         if (SPLIT) {
             if (row0 >= R) continue;      // (an edge class has five rows: uniform over the workgroup)
             W4_PROLOGUE(row0)             // (what the previous job left in flight -- its last Z stores -- is older than these requests and retires before them)
@@ -552,19 +540,17 @@ __global__ __launch_bounds__(HW ? 256 : 64 * (W4_C / 32)) void c6_wino4_gemm_ker
         }
         if (SPLIT) W4Z_LAST_ROW()
     }
-    // the last row's Z_2, Z_3 (first the weight stream's last seven requests land: nobody waits for them -- conv_wino6.hip, r5)
-    if (!SPLIT) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        W4Z_LAST_ROW()
-    }
+    // the last row's Z_2, Z_3
+    if (!SPLIT) W4Z_LAST_ROW()
 #undef W4Z_LAST_ROW
 #undef W4_PROLOGUE
 #undef W4Z_UPDATE
+#undef W4Z_ALL
+#undef W4Z_PIN
 #undef W4Z_POSITION
 #undef WGZ_
 #undef W4Z_GROUP
 #undef W4Z_STORE1
-#undef W4_UNEXT
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
@@ -1116,8 +1102,8 @@ __global__ __launch_bounds__(512) void c6_wino4_wgrad_kernel(const float *__rest
             const size_t src = (size_t)blk * G::BLOCK_FLOATS + (size_t)(half * W4G_ROWS + row) * G::TILE_STRIDE + (size_t)pos * C;
             const float *gd = D + src, *gv = V + src;
             const int ld = ((buf * 2 + 0) * STG + row * CP) * 4, lv = ((buf * 2 + 1) * STG + row * CP) * 4;
-            asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane16), "s"(gd), "s"(ld) : "memory");
-            asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane16), "s"(gv), "s"(lv) : "memory");
+            c6_dma(gd, lane16, ld);
+            c6_dma(gv, lane16, lv);
         }
     };
     f32x16 acc[8];
@@ -1129,7 +1115,7 @@ __global__ __launch_bounds__(512) void c6_wino4_wgrad_kernel(const float *__rest
     dma(0);
 #pragma unroll 1
     for (int st = 0; st < nst; st++) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        c6_dma_wait<0>();
         __syncthreads();                                             // stage st has landed; everyone is done with the other buffer
         if (st + 1 < nst) dma(st + 1);
         const float *dl = wsm + ((st & 1) * 2 + 0) * STG + kk * CP + wave * 32 + i;

@@ -275,9 +275,12 @@ template <int N> static bool w6_has_tail(int nboards) {
 
 // ---- the GEMMs of a block, with the column half of the output transform ("Z rows"): conv_wino4.hip's c6_wino4_gemm_kernel ----------
 // over four classes: rows of positions 6 / 5 / 5 / 8, weight sets at 0 / 36 / 66 / 96 C^2, tile slots of 48 positions in V and 32 row
-// sums in Z.  The schedule, the hand-issued memory operations and their wait counts are the original's (see there).
-constexpr int w6_store_group(int k) { return 8 + k; }
-constexpr int w6_wait(int i, bool stores, int nd = 8) {      // nd: slab DMAs per wave and position (8 waves: 8; the 4-wave jobs of tiny batches: 16)
+// sums in Z.  The schedule is the original's (see there).
+// The vector-memory operations younger than group i's weights when they are multiplied: the requests of the W6_PF groups behind it, the slab DMAs (nd a wave and
+// position; eight waves: 8, the four-wave jobs: 16) and the result stores issued since.  The kernel asserts from these that a position's DMAs have landed
+// by its end and that a split job leaves no request behind.
+constexpr int w6_store_group(int k) { return 8 + k; }      // store k (0 .. 15) of a storing position goes out in group 8 + k
+constexpr int w6_wait(int i, bool stores, int nd = 8) {
     const int lo = i - W6_PF > 0 ? i - W6_PF : 0, hi = (nd - 1 < i - 1) ? nd - 1 : i - 1;
     const int dmas = hi >= lo ? hi - lo + 1 : 0;
     int st = 0;
@@ -287,8 +290,7 @@ constexpr int w6_wait(int i, bool stores, int nd = 8) {      // nd: slab DMAs pe
     return W6_PF + dmas + st;
 }
 static_assert(w6_store_group(15) < 32 - W6_PF, "a position's stores are older than every request that is waited for in the next one");
-// the LAST position of a split job (below): the weight stream ends with the row and no next position is fetched -- younger than group i's request are
-// only the groups i + 1 .. 31 and the result stores issued since
+// ... in the last position of a split job: its weight stream ends with the row and no next position is fetched
 constexpr int w6_wait_last(int i) {
     int st = 0;
     for (int k = 0; k < 16; k++)
@@ -301,13 +303,13 @@ constexpr int w6_wait_last(int i) {
 //
 // SPLIT (r5): the unit of work is a ROW of positions instead of a block (a row's four row sums depend on nothing but its own six -- D': two rows' ten --
 // positions).  A block on one CU is a chain of 48 positions x 13.7 us, whatever the batch: one game's eight boards took 0.66 ms per layer on 4 of the
-// 256 CUs.  Split, its 28 rows run on 28 CUs at once.  Same instruction stream per position (same waits), only the addresses of the V rows, of the
+// 256 CUs.  Split, its 28 rows run on 28 CUs at once.  Same instruction stream per position, only the addresses of the V rows, of the
 // weight groups and of Z differ; the launcher takes this form while the blocks do not fill the chip a few times over (c6_w6_dispatch).
 // HW (r5, split form only): half-width jobs for the tiniest batches -- a workgroup of FOUR waves multiplies a row for 128 of the 256 output channels
 // (blockIdx.z picks the half), one wave per SIMD instead of two: a position takes 6.8 instead of 13.7 us, twice as many jobs.  Each wave fetches 16 of the
-// slab's 64 rows (ND = 16: the wait counts take the DMA count as a parameter).  Same per-wave instruction stream: bit-identical sums.
+// slab's 64 rows (ND = 16).  Same per-wave instruction stream: bit-identical sums.
 template <bool DP, bool SPLIT, bool HW = false>
-__global__ __launch_bounds__(HW ? 256 : 64 * (W6_C / 32)) void c6_w6_gemm_kernel(const float *__restrict__ V, const float *__restrict__ U, float *__restrict__ Zo,
+__global__ __launch_bounds__(HW ? 256 : 64 * (W6_C / 32), 2) void c6_w6_gemm_kernel(const float *__restrict__ V, const float *__restrict__ U, float *__restrict__ Zo,
                                                                                  int first, int nblocks, int blkB, int blkBP, int blkD) {
 #define W6_BX ((int)blockIdx.x)
 #define W6_GX ((int)gridDim.x)
@@ -327,8 +329,8 @@ __device__ __forceinline__ void c6_w6_gemm_body(const float *__restrict__ V, con
 // The half-width jobs of BOTH row forms in one launch (r5): at a handful of games a layer's two GEMM launches took 50 and 42 us side by side on two streams,
 // and the fork / join between the streams cost as much again (12 .. 27 us before and after, profiles/r05_kernel_stats_1game.csv).  The first g6 workgroups
 // along x run the rows of six, the rest the rows of five of class D' -- two inlined bodies behind a branch that is uniform over the workgroup, each with
-// its own instruction stream and wait counts (four waves per workgroup: the register file has room for the larger of the two).
-__global__ __launch_bounds__(256) void c6_w6_gemm_half_pair_kernel(const float *__restrict__ V, const float *__restrict__ U, float *__restrict__ Zo, int n6, int nblocks,
+// its own instruction stream (four waves per workgroup: the register file has room for the larger of the two).
+__global__ __launch_bounds__(256, 2) void c6_w6_gemm_half_pair_kernel(const float *__restrict__ V, const float *__restrict__ U, float *__restrict__ Zo, int n6, int nblocks,
                                                                     int blkB, int blkBP, int blkD, int g6) {
     if ((int)blockIdx.x < g6) c6_w6_gemm_body<false, true, true>(V, U, Zo, 0, n6, blkB, blkBP, blkD, (int)blockIdx.x, g6);
     else c6_w6_gemm_body<true, true, true>(V, U, Zo, n6, nblocks, blkB, blkBP, blkD, (int)blockIdx.x - g6, (int)gridDim.x - g6);
