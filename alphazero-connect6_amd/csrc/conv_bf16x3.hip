@@ -19,6 +19,7 @@
 // A/B partners in round 1 and are gone; their numbers are in DESIGN.md 5.)
 #include "c6_device.h"
 #include "c6_engine.h"
+#include "c6_stream.h"
 
 #include <cstring>
 
@@ -105,8 +106,15 @@ __global__ __launch_bounds__(64 * (C / 32)) void c6_conv3x3_b3s_kernel(const flo
     float *stg = reinterpret_cast<float *>(smem16 + 2 * G::IN_UNITS) + (size_t)wave * IPS * 256;
 
     // weights of this wave: [stage = ks*9 + tap][wave][ct][plane][lane][8]
-    auto wptr = [&](int stage, int ct, int plane) -> const bf16x8 * {
-        return reinterpret_cast<const bf16x8 *>(wp + ((((size_t)stage * WAVES + wave) * 2 + ct) * 2 + plane) * 512) + lane;
+    const auto weights = c6_weights(wp);
+    const unsigned wlane = (unsigned)(wave * 4096 + lane * 16);
+    auto load_w = [&](int stage, bf16x8 (&hi)[2], bf16x8 (&mid)[2]) {
+        int at = stage * WAVES * 4096;
+#pragma unroll
+        for (int ct = 0; ct < 2; ct++) {
+            hi[ct] = c6_request<bf16x8>(weights, wlane + ct * 2048, at);
+            mid[ct] = SPLIT ? c6_request<bf16x8>(weights, wlane + ct * 2048 + 1024, at) : hi[ct];
+        }
     };
 
     if (total == 0) return;
@@ -114,8 +122,7 @@ __global__ __launch_bounds__(64 * (C / 32)) void c6_conv3x3_b3s_kernel(const flo
 #pragma unroll 1
     for (int k = 0; k < NITEM; k++) item_store(lds0, k, item_load(in + (size_t)b0 * (size_t)(CELLS * C), k));   // very first slice
     bf16x8 whi[2], wmid[2];
-#pragma unroll
-    for (int ct = 0; ct < 2; ct++) { whi[ct] = *wptr(0, ct, 0); wmid[ct] = SPLIT ? *wptr(0, ct, 1) : whi[ct]; }
+    load_w(0, whi, wmid);
 
 #pragma unroll 1
     for (int lb = 0; lb < nlocal; lb++) {
@@ -160,15 +167,14 @@ __global__ __launch_bounds__(64 * (C / 32)) void c6_conv3x3_b3s_kernel(const flo
                 int ntap = tap + 1, nks = ks;
                 if (ntap == 9) { ntap = 0; nks++; }
                 if (nks == KS) nks = 0;      // wraps to the next board's first stage (one harmless extra load at the very end)
-#pragma unroll
-                for (int ct = 0; ct < 2; ct++) { nhi[ct] = *wptr(nks * 9 + ntap, ct, 0); nmid[ct] = SPLIT ? *wptr(nks * 9 + ntap, ct, 1) : nhi[ct]; }
+                load_w(nks * 9 + ntap, nhi, nmid);
             }
 #pragma unroll
             for (int half = 0; half < 2; half++) {
                 // the next input slice trickles in: item group k leaves global memory at sub-stage 3k by LDS-DMA
                 // (global_load_lds_dwordx4: per-lane gather, no VGPRs -- a register-held copy was being spilled across the
                 // MFMAs, and that scratch traffic showed up as +30 % HBM bytes) and is split + written to its slots at 3k + 2.
-                // vmcnt completes in order: exactly the four weight loads of one step are younger than the DMA by then.
+                // By then the weights of one step more have been requested behind the DMA (four loads, two without the mid planes): c6_dma_wait.
                 if (more) {
                     const int sidx = tap * 2 + half, k = sidx / 3, ph = sidx % 3;
                     if (ph == 0) {
@@ -177,18 +183,15 @@ __global__ __launch_bounds__(64 * (C / 32)) void c6_conv3x3_b3s_kernel(const flo
                             if (k * IPS + q < NITEM) {
                                 int item = tid + (k * IPS + q) * THREADS;
                                 item = item < CELLS * 8 ? item : CELLS * 8 - 1;
-                                // Written as asm: through the builtin hipcc treats every later ds_read as a possible reader of
-                                // the DMA's LDS bytes and puts s_waitcnt vmcnt(0) in front of the next pixel-fragment reads --
-                                // the "asynchronous" copy was waited for on the spot (HBM latency, 6 times per slice).  The
-                                // landing area is read only at ph == 2, behind the explicit vmcnt wait below.
+                                // (Through the builtin the "asynchronous" copy was waited for by the next pixel-fragment reads: HBM latency,
+                                // 6 times per slice.)  The landing area is read only at ph == 2, behind the wait below.
                                 const float *gp = nslice + (size_t)(item >> 3) * C + (item & 7) * 4;
                                 // LDS byte address of this wave's landing slot (the dynamic segment starts at 0: no static LDS here)
                                 const int lds_off = __builtin_amdgcn_readfirstlane((int)((2 * G::IN_UNITS) * 2 + (wave * IPS + q) * 1024));
-                                asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(gp), "s"(lds_off) : "memory", "m0");
+                                c6_dma(gp, lds_off);
                             }
                     } else if (ph == 2) {
-                        if (SPLIT) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");      // four weight loads per step are younger ...
-                        else asm volatile("s_waitcnt vmcnt(2)" ::: "memory");             // ... two without the mid planes
+                        c6_dma_wait<SPLIT ? 4 : 2>();
 #pragma unroll
                         for (int q = 0; q < IPS; q++)
                             if (k * IPS + q < NITEM) item_store(lds_nx, k * IPS + q, *reinterpret_cast<const f32x4 *>(stg + q * 256 + lane * 4));

@@ -14,6 +14,7 @@
 // of the group contracts the channel pair (8u + r, 8u + 4 + r), and weight lane (cout i, h) holds W[i][8u + 4h + r].
 #include "c6_device.h"
 #include "c6_engine.h"
+#include "c6_stream.h"
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -55,8 +56,12 @@ __global__ __launch_bounds__(64 * (C / 32)) void c6_conv3x3_f32n_kernel(const fl
         return ((p / N + 1) * W + (p % N + 1)) * F3N_SLOT + q * 4;
     };
     // weights of this wave: [stage = ks*9 + tap][wave][u][lane][4]
-    auto wptr = [&](int stage, int u) -> const f32x4 * {
-        return reinterpret_cast<const f32x4 *>(wp + (((size_t)stage * WAVES + wave) * 4 + u) * 256) + lane;
+    const auto weights = c6_weights(wp);
+    const unsigned wlane = (unsigned)(wave * 4096 + lane * 16);
+    auto load_w = [&](int stage, f32x4 (&w)[4]) {
+        int at = stage * WAVES * 4096;
+#pragma unroll
+        for (int u = 0; u < 4; u++) w[u] = c6_request<f32x4>(weights, wlane + u * 1024, at);
     };
 
     if (total == 0) return;
@@ -69,8 +74,7 @@ __global__ __launch_bounds__(64 * (C / 32)) void c6_conv3x3_f32n_kernel(const fl
                 *reinterpret_cast<const f32x4 *>(in + (size_t)b0 * (size_t)(CELLS * C) + (size_t)(item >> 3) * C + (item & 7) * 4);
     }
     f32x4 wc[4];
-#pragma unroll
-    for (int u = 0; u < 4; u++) wc[u] = *wptr(0, u);
+    load_w(0, wc);
 
 #pragma unroll 1
     for (int lb = 0; lb < nlocal; lb++) {
@@ -119,13 +123,12 @@ __global__ __launch_bounds__(64 * (C / 32)) void c6_conv3x3_f32n_kernel(const fl
                     int ntap = tap + 1, nks = ks;
                     if (ntap == 9) { ntap = 0; nks++; }
                     if (nks == KS) nks = 0;
-#pragma unroll
-                    for (int u = 0; u < 4; u++) wn[u] = *wptr(nks * 9 + ntap, u);
+                    load_w(nks * 9 + ntap, wn);
                 }
 #pragma unroll
                 for (int half = 0; half < 2; half++) {
                     // trickle: item group k leaves HBM at sub-stage 3k (LDS-DMA, no VGPRs) and moves to its slots at 3k + 2;
-                    // exactly the four weight loads of one step are younger than the DMA by then (vmcnt completes in order)
+                    // the four weights of one step more have been requested behind the DMA by then (c6_dma_wait)
                     if (more) {
                         const int sidx = tap * 2 + half, k = sidx / 3, ph = sidx % 3;
                         if (ph == 0) {
@@ -136,10 +139,10 @@ __global__ __launch_bounds__(64 * (C / 32)) void c6_conv3x3_f32n_kernel(const fl
                                     item = item < CELLS * 8 ? item : CELLS * 8 - 1;
                                     const float *gp = nslice + (size_t)(item >> 3) * C + (item & 7) * 4;
                                     const int lds_off = __builtin_amdgcn_readfirstlane((int)(2 * G::IN_FLOATS * 4 + (wave * IPS + q) * 1024));
-                                    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(gp), "s"(lds_off) : "memory", "m0");
+                                    c6_dma(gp, lds_off);
                                 }
                         } else if (ph == 2) {
-                            asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+                            c6_dma_wait<4>();
 #pragma unroll
                             for (int q = 0; q < IPS; q++) {
                                 const int item = tid + (k * IPS + q) * THREADS;

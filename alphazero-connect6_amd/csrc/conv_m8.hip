@@ -27,6 +27,7 @@
 // (the planes are shifted so that one scale pair fits both: see M8_XH_SHIFT below).
 #include "c6_device.h"
 #include "c6_engine.h"
+#include "c6_stream.h"
 
 #include "../../include/connect6_amd.h"
 
@@ -135,6 +136,7 @@ __global__ __launch_bounds__(64 * (C / 32)) void c6_conv3x3_m8_kernel(const floa
     // weights of this wave: fp16 planes [stage = ks*9 + tap][wave][ct][lane][8 halfs], then fp8 planes
     // [ks*5 + pair][wave][ct][lane][32 bytes]
     constexpr size_t W16_BYTES = (size_t)KS * 10 * WAVES * 2 * 64 * 16;      // 10 stages per slice: tap 9 is all zeros
+    const auto weights = c6_weights(wp_);
     auto w16ptr = [&](int stage, int ct) -> const f16x8 * {
         return reinterpret_cast<const f16x8 *>(wp + ((((size_t)stage * WAVES + wave) * 2 + ct) * 64) * 16) + lane;
     };
@@ -252,8 +254,7 @@ __global__ __launch_bounds__(64 * (C / 32)) void c6_conv3x3_m8_kernel(const floa
             for (int ct = 0; ct < 2; ct++) w8[ct] = load_w8(ks * 5 + p, ct);
 #pragma unroll
             for (int ct = 0; ct < 2; ct++) b16[ct] = *w16ptr(ks * 10 + 2 * p + 1, ct);
-            // trickle group p leaves global memory by LDS-DMA (per-lane gather into the wave's landing area, no VGPRs;
-            // issued as asm: through the builtin hipcc puts s_waitcnt vmcnt(0) in front of every later ds_read) ...
+            // trickle group p leaves global memory by LDS-DMA (per-lane gather into the wave's landing area, no VGPRs) ...
             if (more) {
 #pragma unroll
                 for (int q = 0; q < IPS; q++)
@@ -262,7 +263,7 @@ __global__ __launch_bounds__(64 * (C / 32)) void c6_conv3x3_m8_kernel(const floa
                         item = item < CELLS * 8 ? item : CELLS * 8 - 1;
                         const float *gp = nslice + (size_t)(item >> 3) * C + (item & 7) * 4;
                         const int lds_off = __builtin_amdgcn_readfirstlane((int)((2 * G::IN_UNITS) * 2 + (wave * IPS + q) * 1024));
-                        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(gp), "s"(lds_off) : "memory", "m0");
+                        c6_dma(gp, lds_off);
                     }
             }
             run16(a16, off0, H0);
@@ -274,13 +275,13 @@ __global__ __launch_bounds__(64 * (C / 32)) void c6_conv3x3_m8_kernel(const floa
             {   // A of the next pair: tap 2p+2, the next slice's (or board's) tap 0 after the last pair
                 const int nks = ks + 1 < KS ? ks + 1 : 0;      // wraps to the next board's first stage (harmless at the very end)
                 const int sa = p < 4 ? ks * 10 + t0 + 2 : nks * 10;
+                int at = M8_HEADER + sa * WAVES * 2048;
 #pragma unroll
-                for (int ct = 0; ct < 2; ct++) a16[ct] = *w16ptr(sa, ct);
+                for (int ct = 0; ct < 2; ct++) a16[ct] = c6_request<f16x8>(weights, (unsigned)(wave * 2048 + ct * 1024 + lane * 16), at);
             }
-            // ... and is split and written to its slots: vmcnt completes in order and exactly the two fp16 weight loads above
-            // are younger than the DMA (the loads at the top of the pair are older)
+            // ... and is split and written to its slots: the two requests above stand behind the DMA (c6_dma_wait)
             if (more && p * IPS < NITEM) {
-                asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
+                c6_dma_wait<2>();
 #pragma unroll
                 for (int q = 0; q < IPS; q++)
                     if (p * IPS + q < NITEM) item_store(lds_nx, p * IPS + q, *reinterpret_cast<const f32x4 *>(stg + q * 256 + lane * 4));
