@@ -52,14 +52,12 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 #define M8_XH_MAX 3584.0f   // 448 * 2^3
 #define M8_HEADER 16        // bytes in front of the weight planes: int32 d
 
-// The MFMAs are issued as inline asm with the accumulator TIED (dst = src C).  Through the builtins hipcc picks the three-address
-// form, renames accumulator tiles from one MFMA to the next and, at 256 VGPRs, ends up moving and spilling whole tiles inside
-// the K loop (20 tile moves + 13 tile spills per tap pair in one instantiation, none in another: chaotic).  A tied tile is one
-// read-modify-write live range.  The hazards hipcc would cover with s_nop are covered by hand: the accumulators are first read
-// by VALU / stores after the K loop, behind M8_MFMA_DRAIN.
-#define M8_MFMA16(ACC, A, B) asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+v"(ACC) : "v"(A), "v"(B))
-#define M8_MFMA8(ACC, A, B, SA, SB) asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]" : "+v"(ACC) : "v"(A), "v"(B), "v"(SA), "v"(SB))
-#define M8_MFMA_DRAIN() asm volatile("s_nop 15\n\ts_nop 15" ::: "memory")
+// The accumulator passes through an empty asm behind its MFMA: tied there, it stays in its registers.  Left alone hipcc renames accumulator tiles from one MFMA
+// to the next and, at 256 VGPRs, ends up moving and spilling whole tiles inside the K loop (20 tile moves + 13 tile spills per tap pair in one
+// instantiation, none in another: chaotic).  (Not MFMAs in asm: their wait states before and behind them would be nobody's.)
+#define M8_PIN(ACC) asm volatile("" : "+v"(ACC))
+#define M8_MFMA16(ACC, A, B) do { ACC = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, B, ACC, 0, 0, 0); M8_PIN(ACC); } while (0)
+#define M8_MFMA8(ACC, A, B, SA, SB) do { ACC = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, ACC, 0, 0, 0, SA, 0, SB); M8_PIN(ACC); } while (0)
 
 template <int C, int N>
 struct M8Geom {
@@ -76,7 +74,7 @@ struct M8Geom {
 };
 
 template <int C, int N, bool HEAD = false>
-__global__ __launch_bounds__(64 * (C / 32)) void c6_conv3x3_m8_kernel(const float *__restrict__ in, const unsigned char *__restrict__ wp_,
+__global__ __launch_bounds__(64 * (C / 32), 2) void c6_conv3x3_m8_kernel(const float *__restrict__ in, const unsigned char *__restrict__ wp_,
                                                                       const float *__restrict__ bias, const float *__restrict__ res,
                                                                       float *__restrict__ out, int nboards, int relu,
                                                                       const float *__restrict__ head_w, unsigned int *__restrict__ range_flag,
@@ -153,7 +151,7 @@ __global__ __launch_bounds__(64 * (C / 32)) void c6_conv3x3_m8_kernel(const floa
     const int wshift = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const int *>(wp));      // the layer's weight shift d
     wp += M8_HEADER;
     const int scale_x = 127 - 4, scale_w = 127 - (wshift + M8_XL_SHIFT - 4);
-    int vscale_w = scale_w, vscale_x = scale_x;      // the asm form takes the scales from VGPRs
+    int vscale_w = scale_w, vscale_x = scale_x;      // in VGPRs, once
     asm volatile("" : "+v"(vscale_w), "+v"(vscale_x));
 
     if (total == 0) return;
@@ -214,7 +212,7 @@ __global__ __launch_bounds__(64 * (C / 32)) void c6_conv3x3_m8_kernel(const floa
                 if (pt + 1 < p_hi) px[sl ^ 1] = *reinterpret_cast<const f16x8 *>(ap + ((pt + 1) * 16) * M8_SLOT);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int ct = 0; ct < 2; ct++)      // accumulator tied (dst = src C): see M8_MFMA16
+                for (int ct = 0; ct < 2; ct++)      // (tied: see M8_PIN)
                     M8_MFMA16(acc[ct][pt], wv[ct], px[sl]);
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -291,11 +289,6 @@ __global__ __launch_bounds__(64 * (C / 32)) void c6_conv3x3_m8_kernel(const floa
         }
     }   // ks
 
-        M8_MFMA_DRAIN();      // MFMA results -> VALU / store reads
-        // (r5: every accumulator tile passes through an empty asm BEHIND the drain -- volatile statements keep their order, so no read of a tile can be
-        //  scheduled between the last MFMA and the wait states; without it only the statement order, not a dependence, stood between them)
-#pragma unroll
-        for (int pt = 0; pt < PT; pt++) { asm volatile("" : "+v"(acc[0][pt])); asm volatile("" : "+v"(acc[1][pt])); }
         // epilogue: + bias, ReLU, 16-byte stores straight from the accumulators (rows with x == N are junk); the stores
         // drain behind the next board's first slice
         float *outb = out + b * (size_t)CELLS * C;

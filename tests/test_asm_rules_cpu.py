@@ -1,7 +1,7 @@
 """What inline assembly in the kernels may do.  The compiler takes an asm statement's outputs as written once it has been issued and does not see what it reads later:
 a load whose wait stands in another statement leaves a register that may be copied, spilled or given away while the load is in flight; a store written in asm may
 read a register after it has been overwritten, or a matrix product before it is there.  So: no loads into registers without their wait in the same statement, no
-stores, and M0 named as clobbered where it is written."""
+stores, no matrix instructions, and M0 named as clobbered where it is written."""
 import glob
 import os
 import re
@@ -43,6 +43,8 @@ def faults(code, whole):
                 out.append("a load whose wait is not in the statement: " + x.strip())
         if STORE.search(x):
             out.append("a store: " + x.strip())
+        if "mfma" in x:
+            out.append("a matrix instruction, whose wait states nobody counts: " + x.strip())
     if re.search(r"\bs_mov_b32 m0\b", code) and '"m0"' not in whole:
         out.append("M0 is written and not named as clobbered")
     return out
@@ -57,7 +59,8 @@ def test_inline_assembly(path):
 def test_the_rules_see_what_they_are_for():
     bad = ['asm volatile("global_load_dwordx4 %0, %1, %2" : "=v"(d) : "v"(o), "s"(b) : "memory")',
            'asm volatile("global_store_dwordx4 %0, %1, %2 offset:" #imm "\\n\\ts_nop 1" ::"v"(o), "v"(d), "s"(b) : "memory")',
-           'asm volatile("s_mov_b32 m0, %2\\n\\ts_nop 0\\n\\tglobal_load_lds_dwordx4 %0, %1" ::"v"(l), "s"(g), "s"(o) : "memory")']
+           'asm volatile("s_mov_b32 m0, %2\\n\\ts_nop 0\\n\\tglobal_load_lds_dwordx4 %0, %1" ::"v"(l), "s"(g), "s"(o) : "memory")',
+           'asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+v"(ACC) : "v"(A), "v"(B))']
     good = ['asm volatile("global_load_dwordx4 %0, %1, %2\\n\\ts_waitcnt vmcnt(0)" : "=&v"(d) : "v"(o), "s"(b) : "memory")',
             'asm volatile("s_mov_b32 m0, %2\\n\\ts_nop 0\\n\\tglobal_load_lds_dwordx4 %0, %1" ::"v"(l), "s"(g), "s"(o) : "memory", "m0")',
             'asm volatile("" : "+v"(d))']
