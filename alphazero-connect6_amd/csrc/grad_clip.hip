@@ -79,8 +79,8 @@ __global__ __launch_bounds__(256) void c6_clip_finish_kernel(const double *parti
     if (threadIdx.x == 0) *norm = (float)n;
 }
 
-template <typename T>
-__device__ __forceinline__ void chunk_scale(const T *x, T *y, uint32_t n, float f) {
+template <typename T, typename F>
+__device__ __forceinline__ void chunk_scale(const T *x, T *y, uint32_t n, F f) {
     typedef C6Vec<T> V;
     constexpr int U = CHUNK / (256 * V::N);
     c6_u32x4 raw[U];
@@ -98,7 +98,7 @@ __device__ __forceinline__ void chunk_scale(const T *x, T *y, uint32_t n, float 
         if (whole) V::get(raw[u], g);
         else V::get_some(x + c, n - c, 0.f, g);
 #pragma unroll
-        for (int i = 0; i < V::N; i++) g[i] *= f;
+        for (int i = 0; i < V::N; i++) g[i] = (float)(g[i] * f);
         if (whole) V::store_past(y + c, V::put(g));
         else V::put_some(y + c, n - c, g);
     }
@@ -113,10 +113,12 @@ __global__ __launch_bounds__(256) void c6_clip_apply_kernel(const Chunk *table, 
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
     const double q = (double)max_norm / (n + 1e-6);
     const float f = q > 1.0 ? 1.f : (float)q;       // a NaN norm makes f NaN
+    const bool far = q < 0x1p-126;                  // f has lost bits or is 0 where a gradient times q is neither: multiplied in 64 bits
     for (int c = (int)blockIdx.x + (chunks - 1 - (int)blockIdx.x) / (int)gridDim.x * (int)gridDim.x; c >= 0; c -= gridDim.x) {
         const Chunk k = table[c];
         if (f == 1.f && k.src == k.dst) continue;   // g * 1 is g
-        C6_BY_TYPE(k.type, T, chunk_scale((const T *)k.src, (T *)k.dst, k.n, f));
+        if (far) C6_BY_TYPE(k.type, T, chunk_scale((const T *)k.src, (T *)k.dst, k.n, q));
+        else C6_BY_TYPE(k.type, T, chunk_scale((const T *)k.src, (T *)k.dst, k.n, f));
     }
 }
 
