@@ -6,8 +6,9 @@ move is chosen, the loss they are trained on, and the clipping of the gradients 
     norm = GradClip(grads).clip(1.0)
 
 Everything runs on torch's current stream of the tensors' device without synchronising, and can be captured into a graph.  Arguments
-that do not fit raise C6Error before anything runs.  Nothing here is recorded by autograd: logits that require a gradient are refused
-(pass them detached; policy_loss returns the gradient, policy_loss_grad takes the upstream one).
+that do not fit raise C6Error before anything runs.  Nothing here is recorded by autograd: while it records (not under no_grad), logits, biases,
+penalties, weights or upstream gradients that require a gradient are refused, and so are forward-mode duals (pass them detached; policy_loss returns
+the gradient, policy_loss_grad takes the upstream one).
 
 `import torch` comes before the first use of the library in a process that wants both on the GPU: whichever is first brings the HIP runtime
 that the other then shares (torch does not start on another's)."""
@@ -16,6 +17,7 @@ import functools
 import sys
 
 import torch
+import torch.autograd.forward_ad as _forward
 
 import alphazero_connect6_amd as _pkg
 
@@ -45,6 +47,14 @@ def _loss_workspace(rows, width):
 # The checks below cost a call less than its launch: messages are made when they are needed, and attributes are read once.
 
 
+def _followed(t, what):
+    """refuses what autograd would have to follow: the result has no record of it"""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise C6Error(f"{what} requires a gradient: autograd does not see this operator, pass a detached tensor")
+    if getattr(_forward, "_current_level", 0) >= 0 and _forward.unpack_dual(t).tangent is not None:
+        raise C6Error(f"{what} carries a forward-mode tangent: autograd does not see this operator")
+
+
 def _logits(x, mask):
     """-> (c6_logits, rows, width)"""
     kind = _TYPE.get(x.dtype) if isinstance(x, _Tensor) else None
@@ -58,8 +68,7 @@ def _logits(x, mask):
     stride, step = x.stride()
     if step != 1 and width > 1:
         raise C6Error("the entries of a row of logits must lie next to each other")
-    if x.requires_grad:
-        raise C6Error("logits that require a gradient: autograd does not see this operator, pass logits.detach()")
+    _followed(x, "the logits tensor")
     if mask is None:
         return Logits(rows, width, kind, device, x.data_ptr(), stride, None, 0, 0), rows, width
     if not isinstance(mask, _Tensor) or mask.dtype is not _U8 or mask.get_device() != device:
@@ -79,6 +88,7 @@ def _written(out, x, what):
         raise C6Error(f"{what} must have the logits' shape, type and device")
     if out.requires_grad:
         raise C6Error(f"{what} must not require a gradient")
+    _followed(out, what)
     if out.stride(1) != 1 and x.shape[1] > 1:
         raise C6Error(f"the entries of a row of {what} must lie next to each other")
     return out
@@ -88,6 +98,7 @@ def _rows_by(t, dtype, device, rows, width, what):
     """(pointer, row stride) of a [rows, width] / [1, width] / [width] tensor"""
     if not isinstance(t, _Tensor) or t.dtype is not dtype or t.get_device() != device:
         raise C6Error(f"{what} must be a {dtype} tensor on the logits' device")
+    _followed(t, what)
     shape, stride = t.shape, t.stride()
     dim = len(shape)
     if (dim != 2 and dim != 1) or shape[-1] != width or (dim == 2 and shape[0] != rows and shape[0] != 1):
@@ -100,6 +111,7 @@ def _rows_by(t, dtype, device, rows, width, what):
 def _per_row(t, dtype, device, rows, what):
     if not isinstance(t, _Tensor) or t.dtype is not dtype or t.get_device() != device or t.shape != (rows,) or (rows > 1 and not t.is_contiguous()):
         raise C6Error(f"{what} must be a contiguous {dtype} tensor [{rows}] on the logits' device")
+    _followed(t, what)
     return t.data_ptr()
 
 
@@ -145,6 +157,7 @@ def _target(targets, device, rows, width):
         return _per_row(targets, targets.dtype, device, rows, "targets of indices"), kind, 0
     if targets.dtype is not _F32 or targets.dim() != 2 or targets.shape[0] != rows or targets.shape[1] != width:
         raise C6Error(f"targets must be int32 or int64 indices [{rows}], or float32 weights [{rows}, {width}]")
+    _followed(targets, "targets")
     stride, step = targets.stride()
     if step != 1 and width > 1:
         raise C6Error("the weights of a row must lie next to each other")

@@ -40,3 +40,35 @@ def test_clip_factor_below_the_smallest_normal(value, max_norm, kind):
     inside = ops.GradClip([g])
     inside.clip(max_norm)
     assert torch.equal(g, out)
+
+
+def differentiable_calls(ops, x, t, w, b, p, d):
+    lse = total = torch.zeros(4, device="cuda")
+    ids = torch.zeros(4, 3, dtype=torch.int32, device="cuda")
+    return {"logits": lambda v: ops.logits_process(v), "loss logits": lambda v: ops.policy_loss(v, t), "bias": lambda v: ops.logits_process(x, bias=v), "penalties": lambda v: ops.logits_process(x, history=ids, penalties=v),
+            "weights": lambda v: ops.policy_loss(x, v, grad_scale=1.0), "grad weights": lambda v: ops.policy_loss_grad(x, v, lse, total, d), "dloss": lambda v: ops.policy_loss_grad(x, t, lse, total, v),
+            "lse": lambda v: ops.policy_loss_grad(x, t, v, total, d), "total": lambda v: ops.policy_loss_grad(x, t, lse, v, d)}
+
+
+def test_what_autograd_would_follow_is_refused():
+    ops = ops_()
+    x = torch.randn(4, 10, device="cuda")
+    given = {"logits": x, "loss logits": x, "bias": torch.randn(4, 10, device="cuda"), "penalties": torch.ones(3, device="cuda"), "weights": torch.rand(4, 10, device="cuda"),
+             "grad weights": torch.rand(4, 10, device="cuda"), "dloss": torch.ones(4, device="cuda"), "lse": torch.zeros(4, device="cuda"), "total": torch.ones(4, device="cuda")}
+    calls = differentiable_calls(ops, x, torch.zeros(4, dtype=torch.int32, device="cuda"), None, None, None, torch.ones(4, device="cuda"))
+    for name, call in calls.items():
+        v = given[name]
+        first = lambda r: r if isinstance(r, torch.Tensor) else r[0]  # noqa: E731
+        want = first(call(v))
+        leaf = v.clone().requires_grad_()
+        for asks in (leaf, leaf * 1):
+            with pytest.raises(pkg.C6Error, match="requires a gradient"):
+                call(asks)
+            with torch.no_grad():      # nothing is recorded: nothing is lost
+                assert torch.equal(first(call(asks)), want), name
+            assert torch.equal(first(call(asks.detach())), want), name
+        with torch.autograd.forward_ad.dual_level():
+            dual = torch.autograd.forward_ad.make_dual(v.clone(), torch.ones_like(v))
+            with pytest.raises(pkg.C6Error, match="tangent"):
+                call(dual)
+            assert torch.equal(first(call(v)), want), name
