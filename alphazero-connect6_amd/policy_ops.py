@@ -30,6 +30,7 @@ _TYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _INDEX = {torch.int32: 0, torch.int64: 1}
 _WEIGHTS = 2
 _Tensor, _F32, _I32, _U8 = torch.Tensor, torch.float32, torch.int32, torch.uint8
+_written_to = torch.autograd.graph.increment_version      # tensors of the caller's that a call wrote: autograd notices where it had saved them for a backward pass
 
 
 def _raw_stream(device):
@@ -127,7 +128,7 @@ def logits_process(logits, mask=None, bias=None, history=None, history_len=None,
     out: a tensor like logits, possibly logits itself.  Returns out."""
     l, rows, width = _logits(logits, mask)
     dev = l.device
-    out = _written(out, logits, "out")
+    given, out = out, _written(out, logits, "out")
     h = n = p = b = None
     hs = ps = bs = cap = 0
     if history is not None:
@@ -145,6 +146,8 @@ def logits_process(logits, mask=None, bias=None, history=None, history_len=None,
     if bias is not None:
         b, bs = _rows_by(bias, _F32, dev, rows, width, "bias")
     _chk(lib().c6_logits_process(l, h, hs, n, cap, p, ps, b, bs, out.data_ptr(), out.stride(0), _stream(dev)))
+    if given is not None:
+        _written_to(out)
     return out
 
 
@@ -174,7 +177,7 @@ def policy_loss(logits, targets, mask=None, grad_scale=None, grad=None):
     l, rows, width = _logits(logits, mask)
     dev = l.device
     t, kind, ts = _target(targets, dev, rows, width)
-    g, gs = None, 0
+    g, gs, given = None, 0, grad
     if grad_scale is not None:
         grad = _written(grad, logits, "grad")
         g, gs = grad.data_ptr(), grad.stride(0)
@@ -187,6 +190,8 @@ def policy_loss(logits, targets, mask=None, grad_scale=None, grad=None):
         keep = torch.empty_strided((nbytes,), (1,), dtype=_U8, device=logits.device)
         space = keep.data_ptr()
     _chk(lib().c6_policy_loss(l, t, kind, ts, at, at + 4 * rows, at + 8 * rows, g, gs, grad_scale or 0.0, space, nbytes, _stream(dev)))
+    if given is not None:
+        _written_to(grad)
     loss, lse, total = stats.unbind(0)
     return (loss, lse, total) if grad is None else (loss, lse, total, grad)
 
@@ -197,11 +202,13 @@ def policy_loss_grad(logits, targets, lse, total, dloss, mask=None, out=None):
     l, rows, width = _logits(logits, mask)
     dev = l.device
     t, kind, ts = _target(targets, dev, rows, width)
-    out = _written(out, logits, "out")
+    given, out = out, _written(out, logits, "out")
     one = rows != 1 and isinstance(dloss, _Tensor) and dloss.dim() == 1 and dloss.shape[0] == 1
     d = _per_row(dloss, _F32, dev, 1 if one else rows, "dloss")
     _chk(lib().c6_policy_loss_grad(l, t, kind, ts, _per_row(lse, _F32, dev, rows, "lse"), _per_row(total, _F32, dev, rows, "total"), d, 0 if one else 1,
                                    out.data_ptr(), out.stride(0), _stream(dev)))
+    if given is not None:
+        _written_to(out)
     return out
 
 
@@ -235,6 +242,8 @@ class GradClip:
                                   self.device.index, C.byref(h)))
         self.h = h
         self._keep = grads, outs
+        # (views of one buffer share its version)
+        self._bases = list({id(b): b for b in (t if t._base is None else t._base for t in (grads if outs is None else outs))}.values())
         self._bytes = lib().c6_clip_workspace(h)
 
     def close(self):
@@ -246,7 +255,7 @@ class GradClip:
             while GradClip._late:
                 lib().c6_clip_destroy(GradClip._late.pop())
             lib().c6_clip_destroy(self.h)
-            self.h = self._keep = None
+            self.h = self._keep = self._bases = None
 
     def __del__(self, _ending=sys.is_finalizing):
         if _ending() or not getattr(self, "h", None):
@@ -263,16 +272,23 @@ class GradClip:
             norm = torch.empty_strided((1,), (1,), dtype=_F32, device=self.device)
         elif not isinstance(norm, _Tensor) or norm.dtype is not _F32 or norm.shape != (1,) or norm.device != self.device:
             raise C6Error("norm must be a float32 tensor [1] on the gradients' device")
+        else:
+            _followed(norm, "norm")
         return norm, torch.empty_strided((self._bytes,), (1,), dtype=_U8, device=self.device)
 
     def norm(self, norm=None):
         """the global norm, a float32 tensor [1]; the gradients stay as they are"""
-        norm, space = self._call(norm)
+        given, (norm, space) = norm, self._call(norm)
         _chk(lib().c6_clip_norm(self.h, norm.data_ptr(), space.data_ptr(), self._bytes, _stream(self.device.index)))
+        if given is not None:
+            _written_to(norm)
         return norm
 
     def clip(self, max_norm, norm=None):
         """scales the gradients; returns their norm before that, a float32 tensor [1]"""
-        norm, space = self._call(norm)
+        given, (norm, space) = norm, self._call(norm)
         _chk(lib().c6_clip_apply(self.h, max_norm, norm.data_ptr(), space.data_ptr(), self._bytes, _stream(self.device.index)))
+        _written_to(self._bases)
+        if given is not None:
+            _written_to(norm)
         return norm

@@ -72,3 +72,36 @@ def test_what_autograd_would_follow_is_refused():
             with pytest.raises(pkg.C6Error, match="tangent"):
                 call(dual)
             assert torch.equal(first(call(v)), want), name
+
+
+def test_writing_in_place_is_seen_by_autograd():
+    """a tensor that autograd saved and one of the calls overwrites: the backward pass says so instead of using the new values"""
+    ops = ops_()
+    i = torch.zeros(3, dtype=torch.int32, device="cuda")
+    lse = total = torch.zeros(3, device="cuda")
+    up = torch.ones(3, device="cuda")
+
+    def clip(t):
+        ops.GradClip([t[:1], t[1:]]).clip(0.1)
+
+    def clip_into(t):
+        ops.GradClip([torch.ones_like(t)], [t]).clip(0.1)
+
+    writes = [lambda t: ops.logits_process(t, out=t), lambda t: ops.logits_process(torch.ones_like(t), out=t), lambda t: ops.policy_loss(t, i, grad_scale=1.0, grad=t),
+              lambda t: ops.policy_loss_grad(t, i, lse, total, up, out=t), clip, clip_into]
+    for k, write in enumerate(writes):
+        w = torch.ones(3, 7, device="cuda", requires_grad=True)
+        saved = torch.randn(3, 7, device="cuda")
+        y = (w * saved).sum()
+        version = saved._version
+        write(saved)
+        assert saved._version > version, k
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    c, n = ops.GradClip([saved]), torch.zeros(1, device="cuda")
+    before = n._version, saved._version
+    c.norm(n)
+    assert n._version > before[0] and saved._version == before[1]      # (only read)
+    x = torch.randn(3, 7, device="cuda")
+    ops.logits_process(x), ops.policy_loss(x, i, grad_scale=1.0), ops.policy_loss_grad(x, i, lse, total, up)
+    assert x._version == 0
