@@ -131,6 +131,18 @@ struct c6_clip {
     Chunk *table = nullptr;
 };
 
+// Memory is allocated, filled and freed beside a stream that another thread is capturing into a graph: in a thread's default mode the runtime would refuse
+// these calls and end that capture.
+struct AnyCapture {
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    AnyCapture() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+    ~AnyCapture() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+};
+// on the thread's own stream: the default one would wait for, or be refused beside, blocking streams
+static bool upload(void *to, const void *from, size_t bytes) {
+    return hipMemcpyAsync(to, from, bytes, hipMemcpyHostToDevice, hipStreamPerThread) == hipSuccess && hipStreamSynchronize(hipStreamPerThread) == hipSuccess;
+}
+
 static int clip_create(int count, const void *const *grads, void *const *outs, const size_t *sizes, const int *types, int device, c6_clip **out) {
     struct Span { uintptr_t a, b; bool written; };
     std::vector<Chunk> table;
@@ -166,12 +178,12 @@ static int clip_create(int count, const void *const *grads, void *const *outs, c
     if (int rc = c6_check_device(device)) return rc;
     C6DeviceScope scope(device);
     if (!scope.ok) return c6_set_error(C6_ERR_HIP, "c6_clip_create: hipSetDevice");
+    AnyCapture beside;
     c6_clip *c = new c6_clip();
     c->device = device;
     c->chunks = (int)table.size();
     c->parts = std::min(c->chunks, MAXPART);
-    if (c->chunks && (hipMalloc(&c->table, table.size() * sizeof(Chunk)) != hipSuccess ||
-                      hipMemcpy(c->table, table.data(), table.size() * sizeof(Chunk), hipMemcpyHostToDevice) != hipSuccess)) {
+    if (c->chunks && (hipMalloc(&c->table, table.size() * sizeof(Chunk)) != hipSuccess || !upload(c->table, table.data(), table.size() * sizeof(Chunk)))) {
         hipFree(c->table);
         delete c;
         return c6_set_error(C6_ERR_HIP, "c6_clip_create: no memory for the table");
@@ -194,6 +206,7 @@ extern "C" int c6_clip_create(int count, const void *const *grads, void *const *
 extern "C" void c6_clip_destroy(c6_clip *c) {
     if (!c) return;
     C6DeviceScope scope(c->device);
+    AnyCapture beside;
     hipFree(c->table);
     delete c;
 }

@@ -218,7 +218,7 @@ class GradClip:
     Made once for buffers that stay where they are (it keeps them alive): contiguous float32 / float16 / bfloat16 tensors of one device, of any
     number and size.  outs: tensors like grads to write to; None: in place.  A graph that captured a call needs the object for as long as it is
     replayed."""
-    _late = []       # tables of objects that were collected during a capture, where memory cannot be freed
+    _late = []       # tables of objects that were collected: freed when the next one is made or closed, not by the collector, whose moment nobody chooses
 
     def __init__(self, grads, outs=None):
         grads = list(grads)
@@ -233,10 +233,13 @@ class GradClip:
             raise C6Error("GradClip needs tensors")
         if outs is not None and (len(outs) != len(grads) or any(o.shape != g.shape or o.dtype is not g.dtype for o, g in zip(outs, grads))):
             raise C6Error("outs must be tensors like grads")
+        if torch.cuda.is_current_stream_capturing():
+            raise C6Error("GradClip cannot be made during a capture")
         self.device = grads[0].device
         k = len(grads)
         ptrs = (C.c_void_p * k)(*[t.data_ptr() for t in grads])
         optrs = None if outs is None else (C.c_void_p * k)(*[t.data_ptr() for t in outs])
+        self._free_late()
         h = C.c_void_p()
         _chk(lib().c6_clip_create(k, ptrs, optrs, (C.c_size_t * k)(*[t.numel() for t in grads]), (C.c_int * k)(*[_TYPE[t.dtype] for t in grads]),
                                   self.device.index, C.byref(h)))
@@ -246,24 +249,28 @@ class GradClip:
         self._bases = list({id(b): b for b in (t if t._base is None else t._base for t in (grads if outs is None else outs))}.values())
         self._bytes = lib().c6_clip_workspace(h)
 
+    @staticmethod
+    def _free_late():
+        while GradClip._late:
+            try:
+                h = GradClip._late.pop()
+            except IndexError:      # (another thread's)
+                break
+            lib().c6_clip_destroy(h)      # (hipFree waits for what the device still has to do)
+
     def close(self):
         """frees the table once nothing that uses it runs any more"""
         if self.h:
             if torch.cuda.is_current_stream_capturing():
                 raise C6Error("GradClip cannot be closed during a capture")
-            torch.cuda.synchronize(self.device)
-            while GradClip._late:
-                lib().c6_clip_destroy(GradClip._late.pop())
-            lib().c6_clip_destroy(self.h)
-            self.h = self._keep = self._bases = None
+            self._free_late()
+            h, self.h = self.h, None
+            lib().c6_clip_destroy(h)
+            self._keep = self._bases = None
 
     def __del__(self, _ending=sys.is_finalizing):
-        if _ending() or not getattr(self, "h", None):
-            return
-        if torch.cuda.is_current_stream_capturing():
+        if not _ending() and getattr(self, "h", None):
             GradClip._late.append(self.h)
-        else:
-            self.close()
 
     def _call(self, norm):
         if not self.h:

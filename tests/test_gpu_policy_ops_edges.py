@@ -105,3 +105,70 @@ def test_writing_in_place_is_seen_by_autograd():
     x = torch.randn(3, 7, device="cuda")
     ops.logits_process(x), ops.policy_loss(x, i, grad_scale=1.0), ops.policy_loss_grad(x, i, lse, total, up)
     assert x._version == 0
+
+
+def test_clip_handles_beside_a_capture():
+    """one thread captures; another makes, uses and drops handles, and the collector takes some: the capture stays whole, and so does what it captured"""
+    ops = ops_()
+    x = torch.randn(5000, device="cuda")
+    y = torch.randn(300, device="cuda")
+    made, ready, done = [], threading.Event(), threading.Event()
+    errors = []
+
+    def other():
+        try:
+            torch.cuda.set_device(0)
+            ready.wait(60)
+            for k in range(3):
+                c = ops.GradClip([y])
+                made.append(c.h is not None)
+                if k == 1:
+                    c.close()
+                del c
+            gc.collect()
+        except BaseException as e:      # noqa: BLE001
+            errors.append(e)
+        finally:
+            done.set()
+
+    thread = threading.Thread(target=other)
+    thread.start()
+    kept, dropped = ops.GradClip([x]), ops.GradClip([y])
+    stream = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    out = torch.zeros(1, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        kept.norm(out)
+        with pytest.raises(pkg.C6Error, match="capture"):
+            kept.close()
+        with pytest.raises(pkg.C6Error, match="capture"):
+            ops.GradClip([y])
+        del dropped
+        gc.collect()
+        ready.set()
+        assert done.wait(60)
+    thread.join(60)
+    assert not errors, errors
+    assert made == [True] * 3
+    for _ in range(3):
+        x.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert abs(float(out) - float(x.double().norm())) <= 1e-6 * float(out)
+    ops.GradClip([y]).close()
+    assert not ops.GradClip._late
+
+
+def test_collected_clips_do_not_wait_for_the_device():
+    ops = ops_()
+    x = torch.randn(1000, device="cuda")
+    c = ops.GradClip([x])
+    n = c.norm()
+    h = c.h
+    del c
+    gc.collect()
+    assert h in ops.GradClip._late
+    assert abs(float(n) - float(x.double().norm())) <= 1e-6 * float(n)
+    d = ops.GradClip([x])
+    assert not ops.GradClip._late and torch.equal(d.norm(), n)
