@@ -129,6 +129,17 @@ struct C6DeviceScope {
     }
 };
 
+// Launches and says whether that worked, by the launch's own answer: hipGetLastError() would give an older error of the thread's for this call's.
+template <typename T>
+struct C6As { typedef T type; };
+template <typename... P>
+static inline bool c6_launch(void (*kernel)(P...), unsigned grid, unsigned block, hipStream_t s, typename C6As<P>::type... args) {
+    void *at[] = {const_cast<void *>(static_cast<const void *>(&args))...};
+    const bool ok = hipLaunchKernel(reinterpret_cast<const void *>(kernel), dim3(grid), dim3(block), at, 0, s) == hipSuccess;
+    if (!ok) (void)hipGetLastError();      // (reported by the caller: not left behind for somebody else's)
+    return ok;
+}
+
 static inline size_t c6_type_bytes(int type) { return type == C6_TYPE_F32 ? 4 : 2; }
 static inline bool c6_type_ok(int type) { return type == C6_TYPE_F32 || type == C6_TYPE_F16 || type == C6_TYPE_BF16; }
 static inline bool c6_aligned(const void *p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }

@@ -185,6 +185,7 @@ static int clip_create(int count, const void *const *grads, void *const *outs, c
     c->parts = std::min(c->chunks, MAXPART);
     if (c->chunks && (hipMalloc(&c->table, table.size() * sizeof(Chunk)) != hipSuccess || !upload(c->table, table.data(), table.size() * sizeof(Chunk)))) {
         hipFree(c->table);
+        (void)hipGetLastError();      // (reported here: not left behind for somebody else's call)
         delete c;
         return c6_set_error(C6_ERR_HIP, "c6_clip_create: no memory for the table");
     }
@@ -223,12 +224,10 @@ static int check_call(c6_clip *c, const float *norm, bool norm_needed, const voi
 static int enqueue(c6_clip *c, bool apply, float max_norm, float *norm, double *partial, hipStream_t s) {
     C6DeviceScope scope(c->device);
     if (!scope.ok) return c6_set_error(C6_ERR_HIP, "c6_clip: hipSetDevice");
-    if (c->chunks) hipLaunchKernelGGL(c6_clip_norm_kernel, dim3(c->parts), dim3(256), 0, s, c->table, c->chunks, partial);
-    if (apply)
-        hipLaunchKernelGGL(c6_clip_apply_kernel, dim3(std::max(c->parts, 1)), dim3(256), 0, s, c->table, c->chunks, partial, c->parts, max_norm, norm);
-    else
-        hipLaunchKernelGGL(c6_clip_finish_kernel, dim3(1), dim3(256), 0, s, partial, c->parts, norm);
-    return hipGetLastError() == hipSuccess ? C6_OK : c6_set_error(C6_ERR_HIP, "c6_clip: launch failed");
+    const bool ok = (!c->chunks || c6_launch(c6_clip_norm_kernel, c->parts, 256, s, c->table, c->chunks, partial)) &&
+                    (apply ? c6_launch(c6_clip_apply_kernel, std::max(c->parts, 1), 256, s, c->table, c->chunks, partial, c->parts, max_norm, norm)
+                           : c6_launch(c6_clip_finish_kernel, 1, 256, s, partial, c->parts, norm));
+    return ok ? C6_OK : c6_set_error(C6_ERR_HIP, "c6_clip: launch failed");
 }
 
 extern "C" int c6_clip_norm(c6_clip *c, float *norm, void *workspace, size_t workspace_bytes, void *stream) {

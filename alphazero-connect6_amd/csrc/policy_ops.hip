@@ -728,7 +728,7 @@ int cus() {
 
 Rows rows_of(const c6_logits *l) { return Rows{l->x, l->mask, l->x_stride, l->mask_row, l->mask_byte, l->rows, l->width}; }
 
-int launched() { return hipGetLastError() == hipSuccess ? C6_OK : c6_set_error(C6_ERR_HIP, "logits: launch failed"); }
+int launched(bool ok) { return ok ? C6_OK : c6_set_error(C6_ERR_HIP, "logits: launch failed"); }
 
 }   // namespace
 
@@ -750,9 +750,10 @@ extern "C" int c6_logits_process(const c6_logits *l, const int32_t *history, int
     C6DeviceScope scope(l->device);
     if (!scope.ok) return c6_set_error(C6_ERR_HIP, "c6_logits_process: hipSetDevice");
     const Repeats h{history, history_len, penalties, history_stride, penalties_stride, history_cap};
+    bool ok = false;
 #define C6_LAUNCH(LANES, HIST, BIAS)                                                                                                                        \
-    C6_BY_TYPE(l->type, T, hipLaunchKernelGGL((c6_logits_process_kernel<T, LANES, HIST, BIAS>), dim3(grid_of<LANES>(l)), dim3(256), 0, (hipStream_t)stream, rows_of(l), \
-                                              h, bias, bias_stride, (T *)out, out_stride))
+    C6_BY_TYPE(l->type, T, ok = c6_launch(c6_logits_process_kernel<T, LANES, HIST, BIAS>, grid_of<LANES>(l), 256, (hipStream_t)stream, rows_of(l), h, bias, bias_stride, \
+                                          (T *)out, out_stride))
 #define C6_LAUNCH_LANES(LANES)                         \
     if (history && bias) C6_LAUNCH(LANES, true, true); \
     else if (history) C6_LAUNCH(LANES, true, false);   \
@@ -765,7 +766,7 @@ extern "C" int c6_logits_process(const c6_logits *l, const int32_t *history, int
     }
 #undef C6_LAUNCH_LANES
 #undef C6_LAUNCH
-    return launched();
+    return launched(ok);
 }
 
 // Which way the loss goes, by the pieces of N entries (16 bytes) in a row.  The registers of 64, 256 or 1024 lanes hold up to 16384 (against weights, which
@@ -790,7 +791,7 @@ extern "C" size_t c6_policy_loss_workspace(int rows, int width) {
 }
 
 template <typename T, bool WEIGHTS>
-static void loss_launch(const c6_logits *l, const Target &t, float *loss, float *lse, float *total, T *grad, int64_t grad_stride, float scale, void *workspace, hipStream_t s) {
+static bool loss_launch(const c6_logits *l, const Target &t, float *loss, float *lse, float *total, T *grad, int64_t grad_stride, float scale, void *workspace, hipStream_t s) {
     constexpr int N = C6Vec<T>::N;
     const Rows rows = rows_of(l);
     if (splits(l->rows, l->width, N, WEIGHTS, grad != nullptr)) {
@@ -798,15 +799,12 @@ static void loss_launch(const c6_logits *l, const Target &t, float *loss, float 
         Part *parts = (Part *)workspace;
         float *at = (float *)(parts + items);
         const unsigned grid = (unsigned)std::min<int64_t>(items, 1 << 22), join = (unsigned)std::min<int64_t>(l->rows * (grad ? std::min<int64_t>(chunks, JOIN_MOST) : 1), 1 << 22);
-        hipLaunchKernelGGL((c6_policy_loss_part_kernel<T, WEIGHTS>), dim3(grid), dim3(256), 0, s, rows, t, parts, at);
-        hipLaunchKernelGGL((c6_policy_loss_join_kernel<T, WEIGHTS>), dim3(join), dim3(256), 0, s, rows, t, parts, at, loss, lse,
-                           total, grad, grad_stride, scale);
-        return;
+        return c6_launch(c6_policy_loss_part_kernel<T, WEIGHTS>, grid, 256, s, rows, t, parts, at) &&
+               c6_launch(c6_policy_loss_join_kernel<T, WEIGHTS>, join, 256, s, rows, t, parts, at, loss, lse, total, grad, grad_stride, scale);
     }
 #define C6_LAUNCH(LANES, NV, RESIDENT)                                                                                                                                       \
-    hipLaunchKernelGGL((c6_policy_loss_kernel<T, LANES, NV, WEIGHTS>),                                                                                                       \
-                       dim3((unsigned)std::min<int64_t>(LANES < 256 ? ((int64_t)l->rows * LANES + 255) / 256 : l->rows, (int64_t)cus() * RESIDENT)), dim3(LANES < 256 ? 256 : LANES), 0, s, \
-                       rows, t, loss, lse, total, grad, grad_stride, scale)
+    return c6_launch(c6_policy_loss_kernel<T, LANES, NV, WEIGHTS>, (unsigned)std::min<int64_t>(LANES < 256 ? ((int64_t)l->rows * LANES + 255) / 256 : l->rows, (int64_t)cus() * RESIDENT), \
+                     LANES < 256 ? 256 : LANES, s, rows, t, loss, lse, total, grad, grad_stride, scale)
     // The pieces that a lane may hold come in steps of a third or less: those beyond the row take part in its sums all the same (in steps of two 300 x 80001
     // bf16 took 37.1 us instead of 33.3, 2048 x 20000 f32 85.7 instead of 80.3, 2048 x 24000 bf16 against weights 92.0 instead of 85.5; skipped by a branch
     // they cost 2048 x 128000 bf16, where there are none, 8 %)
@@ -852,9 +850,10 @@ extern "C" int c6_policy_loss(const c6_logits *l, const void *target, int target
     C6DeviceScope scope(l->device);
     if (!scope.ok) return c6_set_error(C6_ERR_HIP, "c6_policy_loss: hipSetDevice");
     const Target t{target, target_stride, target_kind};
-    C6_BY_TYPE(l->type, T, if (target_kind == C6_TARGET_WEIGHTS) loss_launch<T, true>(l, t, loss, lse, total, (T *)grad, grad_stride, grad_scale, workspace, (hipStream_t)stream);
-               else loss_launch<T, false>(l, t, loss, lse, total, (T *)grad, grad_stride, grad_scale, workspace, (hipStream_t)stream));
-    return launched();
+    bool ok = false;
+    C6_BY_TYPE(l->type, T, const auto launch = target_kind == C6_TARGET_WEIGHTS ? loss_launch<T, true> : loss_launch<T, false>;
+               ok = launch(l, t, loss, lse, total, (T *)grad, grad_stride, grad_scale, workspace, (hipStream_t)stream));
+    return launched(ok);
 }
 
 extern "C" int c6_policy_loss_grad(const c6_logits *l, const void *target, int target_kind, int64_t target_stride, const float *lse, const float *total,
@@ -871,16 +870,17 @@ extern "C" int c6_policy_loss_grad(const c6_logits *l, const void *target, int t
     if (!scope.ok) return c6_set_error(C6_ERR_HIP, "c6_policy_loss_grad: hipSetDevice");
     const Target t{target, target_stride, target_kind};
 #define C6_LAUNCH(LANES, WEIGHTS)                                                                                                                          \
-    C6_BY_TYPE(l->type, T, hipLaunchKernelGGL((c6_policy_loss_grad_kernel<T, LANES, WEIGHTS>), dim3(grid_of<LANES>(l)), dim3(256), 0, (hipStream_t)stream, rows_of(l), t, \
-                                              lse, total, dloss, dloss_stride, (T *)grad, grad_stride))
+    C6_BY_TYPE(l->type, T, ok = c6_launch(c6_policy_loss_grad_kernel<T, LANES, WEIGHTS>, grid_of<LANES>(l), 256, (hipStream_t)stream, rows_of(l), t, lse, total, dloss, \
+                                          dloss_stride, (T *)grad, grad_stride))
     const bool weights = target_kind == C6_TARGET_WEIGHTS;
+    bool ok = false;
     switch (lanes_of(l)) {
     case 16: if (weights) C6_LAUNCH(16, true); else C6_LAUNCH(16, false); break;
     case 64: if (weights) C6_LAUNCH(64, true); else C6_LAUNCH(64, false); break;
     default: if (weights) C6_LAUNCH(256, true); else C6_LAUNCH(256, false);
     }
 #undef C6_LAUNCH
-    return launched();
+    return launched(ok);
 }
 
 // The trainer's batch in the operator's terms; a wave a position.

@@ -172,3 +172,28 @@ def test_collected_clips_do_not_wait_for_the_device():
     assert abs(float(n) - float(x.double().norm())) <= 1e-6 * float(n)
     d = ops.GradClip([x])
     assert not ops.GradClip._late and torch.equal(d.norm(), n)
+
+
+def test_errors_of_other_calls_are_not_taken_for_ones_own():
+    """an error that an earlier HIP call of the thread left behind: the operators' launches work and say so"""
+    ops = ops_()
+    x = torch.randn(5, 99, device="cuda")
+    i = torch.zeros(5, dtype=torch.int32, device="cuda")
+    long = torch.randn(2, 200003, device="cuda")      # (two launches)
+    clip = ops.GradClip([x.clone()])
+    want = [ops.logits_process(x), *ops.policy_loss(x, i, grad_scale=1.0), *ops.policy_loss(long, i[:2], grad_scale=1.0), clip.norm()]
+    lse, total = want[2], want[3]
+    want.append(ops.policy_loss_grad(x, i, lse, total, want[1]))
+    torch.cuda.synchronize()
+    hip = pkg.lib()
+    calls = [lambda: [ops.logits_process(x)], lambda: list(ops.policy_loss(x, i, grad_scale=1.0)), lambda: list(ops.policy_loss(long, i[:2], grad_scale=1.0)), lambda: [clip.norm()],
+             lambda: [ops.policy_loss_grad(x, i, lse, total, want[1])]]
+    got = []
+    try:
+        for call in calls:
+            assert hip.hipSetDevice(12345) != 0
+            got += call()
+    finally:
+        hip.hipGetLastError()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
