@@ -4,6 +4,7 @@
 #include "c6_train.h"
 
 #include <algorithm>
+#include <initializer_list>
 
 namespace {
 
@@ -670,6 +671,31 @@ int check_logits(const c6_logits *l) {
     return C6_OK;
 }
 
+// `rows` pieces of memory, `stride` bytes apart, of `width` bytes each
+struct Span {
+    const void *p;
+    int64_t stride, width;
+};
+// nothing of the one is part of the other: apart as a whole, or rows of both interleave in one buffer
+bool apart(const Span &w, const Span &o, int64_t rows) {
+    if (!w.p || !o.p || rows <= 0 || w.width <= 0 || o.width <= 0) return true;
+    const int64_t a = (int64_t)(uintptr_t)w.p, b = (int64_t)(uintptr_t)o.p;
+    if (a + (rows - 1) * w.stride + w.width <= b || b + (rows - 1) * o.stride + o.width <= a) return true;
+    if (rows < 2 || w.stride < 1 || o.stride % w.stride) return false;
+    int64_t off = (b - a) % w.stride;      // every row of the other lies here between two of the one
+    if (off < 0) off += w.stride;
+    return off >= w.width && w.stride - off >= o.width;
+}
+// what a call writes overlaps none of what it reads beside x
+int check_apart(const c6_logits *l, const Span &out, std::initializer_list<Span> read) {
+    const int64_t rows = l->rows, bytes = (l->width + 7) / 8;
+    if (!out.p || !rows || !l->width) return C6_OK;
+    bool ok = l->mask_byte == 1 ? apart(out, Span{l->mask, l->mask_row, bytes}, rows)
+                                : apart(Span{out.p, 0, (rows - 1) * out.stride + out.width}, Span{l->mask, 0, (rows - 1) * l->mask_row + (bytes - 1) * l->mask_byte + 1}, 1);
+    for (const Span &o : read) ok = ok && apart(out, o, rows);
+    return ok ? C6_OK : bad("logits: the output overlaps another argument");
+}
+
 // a written matrix: its rows do not overlap one another, and it is x itself or leaves x alone (rows of both may interleave in one buffer)
 int check_written(const c6_logits *l, const void *out, int64_t stride, const char *null_msg) {
     const int64_t es = (int64_t)c6_type_bytes(l->type);
@@ -680,15 +706,7 @@ int check_written(const c6_logits *l, const void *out, int64_t stride, const cha
     if (!fits(l->rows, stride, l->width, es)) return bad("logits: the output exceeds the address space");
     if (l->rows > 1 && out == l->x && stride != l->x_stride) return bad("logits: in place needs the same stride");
     if (out == l->x) return C6_OK;
-    const int64_t a = (int64_t)(uintptr_t)l->x, b = (int64_t)(uintptr_t)out;
-    const int64_t a1 = a + ((l->rows - 1) * l->x_stride + l->width) * es, b1 = b + ((l->rows - 1) * stride + l->width) * es;
-    if (a1 <= b || b1 <= a) return C6_OK;
-    if (l->rows > 1 && stride == l->x_stride) {      // interleaved: row r of the output lies between rows of x
-        int64_t off = (b - a) % (stride * es);
-        if (off < 0) off += stride * es;
-        if (off >= l->width * es && stride * es - off >= l->width * es) return C6_OK;
-    }
-    return bad("logits: the output overlaps x without being x");
+    return apart(Span{out, stride * es, l->width * es}, Span{l->x, l->x_stride * es, l->width * es}, l->rows) ? C6_OK : bad("logits: the output overlaps x without being x");
 }
 
 int check_target(const c6_logits *l, const void *target, int kind, int64_t stride) {
@@ -698,6 +716,12 @@ int check_target(const c6_logits *l, const void *target, int kind, int64_t strid
     if (!c6_aligned(target, kind == C6_TARGET_INDEX64 ? 8 : 4)) return bad("policy loss: target is not aligned to its type");
     if (kind == C6_TARGET_WEIGHTS && (stride < 0 || !fits(l->rows, stride, l->width, 4))) return bad("policy loss: bad stride of the weights");
     return C6_OK;
+}
+
+Span target_span(const c6_logits *l, const void *target, int kind, int64_t stride) {
+    if (kind == C6_TARGET_WEIGHTS) return Span{target, stride * 4, (int64_t)l->width * 4};
+    const int64_t bytes = kind == C6_TARGET_INDEX64 ? 8 : 4;
+    return Span{target, bytes, bytes};
 }
 
 // Four rows a wave once that still leaves every SIMD one; 16 lanes count a history for longer, and take twice the rows for it.  Four rows a wave against
@@ -745,6 +769,9 @@ extern "C" int c6_logits_process(const c6_logits *l, const int32_t *history, int
         if (!fits(l->rows, history_stride, history_cap, 4) || !fits(l->rows, penalties_stride, 3, 4)) return bad("c6_logits_process: the history exceeds the address space");
     }
     if (bias && (bias_stride < 0 || !c6_aligned(bias, 4) || !fits(l->rows, bias_stride, l->width, 4))) return bad("c6_logits_process: bad bias");
+    const int64_t es = (int64_t)c6_type_bytes(l->type);
+    if (int rc = check_apart(l, Span{out, out_stride * es, l->width * es}, {Span{bias, bias_stride * 4, (int64_t)l->width * 4}, Span{history, history_stride * 4, (int64_t)history_cap * 4},
+                                                                          Span{history ? history_len : nullptr, 4, 4}, Span{history ? penalties : nullptr, penalties_stride * 4, 12}})) return rc;
     if (int rc = c6_check_device(l->device)) return rc;
     if (!l->rows || !l->width) return C6_OK;
     C6DeviceScope scope(l->device);
@@ -842,6 +869,11 @@ extern "C" int c6_policy_loss(const c6_logits *l, const void *target, int target
         if (int rc = check_written(l, grad, grad_stride, "")) return rc;
     if (l->rows && (!loss || !lse || !total)) return bad("c6_policy_loss: loss, lse or total is NULL");
     if (!c6_aligned(loss, 4) || !c6_aligned(lse, 4) || !c6_aligned(total, 4)) return bad("c6_policy_loss: loss, lse and total are aligned to 4 bytes");
+    const int64_t es = (int64_t)c6_type_bytes(l->type);
+    const Span t_span = target_span(l, target, target_kind, target_stride);
+    if (int rc = check_apart(l, Span{grad, grad_stride * es, l->width * es}, {t_span, Span{loss, 4, 4}, Span{lse, 4, 4}, Span{total, 4, 4}})) return rc;
+    for (const float *stat : {loss, lse, total})
+        if (int rc = check_apart(l, Span{stat, 4, 4}, {t_span, Span{l->x, l->x_stride * es, l->width * es}})) return rc;
     const int n = l->type == C6_TYPE_F32 ? 4 : 8;
     if (l->rows && splits(l->rows, l->width, n, target_kind == C6_TARGET_WEIGHTS, grad != nullptr) && (!workspace || workspace_bytes < split_bytes(l->rows, l->width, n) || !c6_aligned(workspace, alignof(Part))))
         return bad("c6_policy_loss: the workspace is NULL, smaller than c6_policy_loss_workspace() or not aligned to 16 bytes");
@@ -864,6 +896,8 @@ extern "C" int c6_policy_loss_grad(const c6_logits *l, const void *target, int t
     if (l->rows && (!lse || !total || !dloss)) return bad("c6_policy_loss_grad: lse, total or dloss is NULL");
     if (!c6_aligned(lse, 4) || !c6_aligned(total, 4) || !c6_aligned(dloss, 4)) return bad("c6_policy_loss_grad: lse, total and dloss are aligned to 4 bytes");
     if (dloss_stride < 0) return bad("c6_policy_loss_grad: negative stride");
+    const int64_t es = (int64_t)c6_type_bytes(l->type);
+    if (int rc = check_apart(l, Span{grad, grad_stride * es, l->width * es}, {target_span(l, target, target_kind, target_stride), Span{lse, 4, 4}, Span{total, 4, 4}, Span{dloss, dloss_stride * 4, 4}})) return rc;
     if (int rc = c6_check_device(l->device)) return rc;
     if (!l->rows || !l->width) return C6_OK;
     C6DeviceScope scope(l->device);

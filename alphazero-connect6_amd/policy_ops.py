@@ -125,7 +125,7 @@ def logits_process(logits, mask=None, bias=None, history=None, history_len=None,
     mask: uint8 [rows, ceil(width / 8)], any strides (a transposed view of legal_mask's layout too), or one for all rows; set bits are legal.
     bias: float32 [width] or [rows, width].  history: int32 [rows, cap] ids (or one for all rows), of which the first history_len[r] count (int32
     [rows]; None: all); ids outside the row, such as -1, count for nothing.  penalties: float32 [3] or [rows, 3] = repetition, frequency, presence.
-    out: a tensor like logits, possibly logits itself.  Returns out."""
+    out: a tensor like logits, possibly logits itself; it overlaps no other argument.  Returns out."""
     l, rows, width = _logits(logits, mask)
     dev = l.device
     given, out = out, _written(out, logits, "out")
@@ -173,7 +173,7 @@ def policy_loss(logits, targets, mask=None, grad_scale=None, grad=None):
 
     targets: int32 / int64 [rows] -- the entry played; outside the row or illegal: the row adds nothing -- or float32 [rows, width] weights >= 0
     (visit counts, a teacher's distribution).  loss = sum t (lse - x), total = sum t.  mask as in logits_process.  grad: where the gradient goes,
-    possibly logits itself.  A row with no legal entry above -infinity has loss 0, lse -infinity and gradient 0."""
+    possibly logits itself; it overlaps no other argument.  A row with no legal entry above -infinity has loss 0, lse -infinity and gradient 0."""
     l, rows, width = _logits(logits, mask)
     dev = l.device
     t, kind, ts = _target(targets, dev, rows, width)
@@ -198,7 +198,7 @@ def policy_loss(logits, targets, mask=None, grad_scale=None, grad=None):
 
 def policy_loss_grad(logits, targets, lse, total, dloss, mask=None, out=None):
     """The gradient by the logits from the lse and total of policy_loss and the upstream gradient dloss, float32 [rows] or [1] (c6_policy_loss_grad).
-    out: where it goes, possibly logits itself."""
+    out: where it goes, possibly logits itself; it overlaps no other argument."""
     l, rows, width = _logits(logits, mask)
     dev = l.device
     t, kind, ts = _target(targets, dev, rows, width)

@@ -596,7 +596,7 @@ typedef struct c6_logits {
  *     y += bias[r * bias_stride + v];      an entry that is not legal: y = -infinity, whatever x is
  * and out = y rounded once to the type.  history (int32) NULL: no penalties; a row of it is history_cap (<= 2^30) ids of readable memory, of which
  * those behind history_len[r] hold anything; history_len NULL: every row has history_cap ids; bias NULL:
- * none.  Strides in elements, >= 0 (0: shared by the rows).  out may be x itself (same pointer and stride) and overlaps nothing else. */
+ * none.  Strides in elements, >= 0 (0: shared by the rows).  out may be x itself (same pointer and stride); it overlaps no other argument (refused). */
 int c6_logits_process(const c6_logits *l, const int32_t *history, int64_t history_stride, const int32_t *history_len, int history_cap,
                       const float *penalties, int64_t penalties_stride, const float *bias, int64_t bias_stride, void *out, int64_t out_stride,
                       void *stream);
@@ -614,7 +614,8 @@ enum {
 /* bytes of workspace (aligned to 16) that c6_policy_loss needs for so many rows and entries, of any type (may be 0) */
 size_t c6_policy_loss_workspace(int rows, int width);
 /* loss, lse, total: float [rows], written.  grad (type of x, stride in elements) may be NULL: no gradient; else the gradient at
- * scale = grad_scale for every row (1 / rows: the mean's).  grad may be x itself (same pointer and stride) and overlaps nothing else. */
+ * scale = grad_scale for every row (1 / rows: the mean's).  grad may be x itself (same pointer and stride); it and the statistics overlap no other
+ * argument (refused). */
 int c6_policy_loss(const c6_logits *l, const void *target, int target_kind, int64_t target_stride, float *loss, float *lse, float *total, void *grad,
                    int64_t grad_stride, float grad_scale, void *workspace, size_t workspace_bytes, void *stream);
 /* the gradient alone, from the lse and total that c6_policy_loss left: scale = dloss[r * dloss_stride] (dloss_stride 0: one for all rows) */
