@@ -917,12 +917,13 @@ extern "C" int c6_policy_loss_grad(const c6_logits *l, const void *target, int t
     return launched(ok);
 }
 
-// The trainer's batch in the operator's terms; a wave a position.
+// The trainer's batch in the operator's terms; a wave a position.  Visits are summed and divided in 64 bits: finite ones of any size have a finite sum (with sums
+// below 2^24 and whole visits the same bits as in 32: one rounding of the same quotient).
 __global__ __launch_bounds__(256) void c6t_policy_targets_kernel(int B, int cells, const float *boards, const float *poses, const float *visits, uint8_t *mask, int *index,
                                                                  float *weights) {
     const int lane = threadIdx.x & 63, b = blockIdx.x * 4 + (threadIdx.x >> 6), bytes = (cells + 7) / 8;
     if (b >= B) return;
-    float sum = 0.f;
+    double sum = 0;
     for (int v0 = 0; v0 < cells; v0 += 64) {
         const int v = v0 + lane;
         const bool empty = v < cells && boards[(size_t)b * cells + v] == 0.f;
@@ -935,7 +936,7 @@ __global__ __launch_bounds__(256) void c6t_policy_targets_kernel(int B, int cell
         return;
     }
     sum = c6_wave_sum(sum);
-    for (int v = lane; v < cells; v += 64) weights[(size_t)b * cells + v] = sum > 0.f ? visits[(size_t)b * cells + v] / sum : 0.f;
+    for (int v = lane; v < cells; v += 64) weights[(size_t)b * cells + v] = sum > 0 ? (float)(visits[(size_t)b * cells + v] / sum) : 0.f;
 }
 void c6t_policy_targets(int B, int cells, const float *boards, const float *poses, const float *visits, unsigned char *mask, int *index, float *weights, hipStream_t s) {
     hipLaunchKernelGGL(c6t_policy_targets_kernel, dim3((B + 3) / 4), dim3(256), 0, s, B, cells, boards, poses, visits, mask, index, weights);
