@@ -197,3 +197,40 @@ def test_errors_of_other_calls_are_not_taken_for_ones_own():
         hip.hipGetLastError()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("width", [7, 361, 5001, 40001, 70001])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_weights_at_illegal_entries_count_for_nothing(width, kind):
+    """... whatever stands there: NaN, infinities; in every way a loss against weights goes, and in the backward pass alone"""
+    ops = ops_()
+    rng = np.random.default_rng(width)
+    rows = 5000 if width == 7 else 6
+    x = torch.tensor(rng.normal(0, 3, (rows, width)), device="cuda").to({"f32": torch.float32, "bf16": torch.bfloat16}[kind])
+    keep = rng.random((rows, width)) < 0.5
+    keep[1] = False
+    keep[2] = False
+    keep[2, width - 1] = True
+    t = (rng.random((rows, width)) * keep).astype(np.float32)
+    junk = np.where(keep, t, rng.choice(np.array([np.nan, np.inf, -np.inf, 3e38], np.float32), (rows, width))).astype(np.float32)
+    m, clean, dirty = torch.tensor(po.pack(keep), device="cuda"), torch.tensor(t, device="cuda"), torch.tensor(junk, device="cuda")
+    a, b = ops.policy_loss(x, clean, mask=m, grad_scale=0.5), ops.policy_loss(x, dirty, mask=m, grad_scale=0.5)
+    assert all(torch.equal(p, q) for p, q in zip(a, b)) and all(bool(v[0 if k == 1 else slice(None)].isfinite().all()) for k, v in enumerate(a))
+    assert all(torch.equal(p, q) for p, q in zip(ops.policy_loss(x, clean, mask=m), ops.policy_loss(x, dirty, mask=m)))
+    up = torch.full((1,), 0.5, device="cuda")
+    assert torch.equal(ops.policy_loss_grad(x, clean, a[1], a[2], up, mask=m), ops.policy_loss_grad(x, dirty, a[1], a[2], up, mask=m))
+    want, tol = po.loss(host(x)[:6], t[:6], po.pack(keep)[:6], 0.5)
+    po.near(host(a[3])[:6], want["grad"], tol["grad"], kind, "grad")
+
+
+def test_outputs_that_overlap_an_argument_are_refused():
+    ops = ops_()
+    x, w = torch.randn(4, 10, device="cuda"), torch.rand(4, 10, device="cuda")
+    lse, total, up = torch.zeros(4, device="cuda"), torch.ones(4, device="cuda"), torch.ones(4, device="cuda")
+    wide = torch.randn(4, 30, device="cuda")
+    for call in (lambda: ops.policy_loss(x, w, grad_scale=1.0, grad=w), lambda: ops.policy_loss_grad(x, w, lse, total, up, out=w), lambda: ops.logits_process(x, bias=w, out=w),
+                 lambda: ops.logits_process(wide[:, :10], bias=wide[:, 5:15], out=wide[:, 10:20])):
+        with pytest.raises(pkg.C6Error, match="overlaps"):
+            call()
+    want = ops.logits_process(wide[:, :10].clone(), bias=wide[:, 10:20].clone())
+    assert torch.equal(ops.logits_process(wide[:, :10], bias=wide[:, 10:20], out=wide[:, 20:]), want)      # columns of one buffer
