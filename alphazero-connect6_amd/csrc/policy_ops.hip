@@ -664,6 +664,8 @@ int check_logits(const c6_logits *l) {
     if (l->x_stride < 0 || l->mask_row < 0 || l->mask_byte < 0) return bad("logits: negative stride");
     const int64_t es = (int64_t)c6_type_bytes(l->type);
     if (!fits(l->rows, l->x_stride, l->width, es)) return bad("logits: the matrix exceeds the address space");
+    int64_t bytes;      // of a row of the mask, from its first to its last
+    if (l->mask && (__builtin_mul_overflow((int64_t)((l->width + 7) / 8), l->mask_byte, &bytes) || !fits(l->rows, l->mask_row, bytes, 1))) return bad("logits: the mask exceeds the address space");
     if (l->rows && l->width) {
         if (!l->x) return bad("logits: x is NULL");
         if (!c6_aligned(l->x, es)) return bad("logits: x is not aligned to its type");
@@ -671,10 +673,14 @@ int check_logits(const c6_logits *l) {
     return C6_OK;
 }
 
-// `rows` pieces of memory, `stride` bytes apart, of `width` bytes each
+// `rows` pieces of memory, `stride` elements apart, of `width` elements each (in bytes; sizes have passed fits())
 struct Span {
-    const void *p;
-    int64_t stride, width;
+    const void *p = nullptr;
+    int64_t stride = 0, width = 0;
+    Span(const void *p_, int64_t stride_, int64_t width_, int64_t bytes) {
+        if (!p_) return;
+        p = p_; stride = stride_ * bytes; width = width_ * bytes;
+    }
 };
 // nothing of the one is part of the other: apart as a whole, or rows of both interleave in one buffer
 bool apart(const Span &w, const Span &o, int64_t rows) {
@@ -690,8 +696,8 @@ bool apart(const Span &w, const Span &o, int64_t rows) {
 int check_apart(const c6_logits *l, const Span &out, std::initializer_list<Span> read) {
     const int64_t rows = l->rows, bytes = (l->width + 7) / 8;
     if (!out.p || !rows || !l->width) return C6_OK;
-    bool ok = l->mask_byte == 1 ? apart(out, Span{l->mask, l->mask_row, bytes}, rows)
-                                : apart(Span{out.p, 0, (rows - 1) * out.stride + out.width}, Span{l->mask, 0, (rows - 1) * l->mask_row + (bytes - 1) * l->mask_byte + 1}, 1);
+    bool ok = l->mask_byte == 1 ? apart(out, Span(l->mask, l->mask_row, bytes, 1), rows)
+                                : apart(Span(out.p, 0, (rows - 1) * out.stride + out.width, 1), Span(l->mask, 0, (rows - 1) * l->mask_row + (bytes - 1) * l->mask_byte + 1, 1), 1);
     for (const Span &o : read) ok = ok && apart(out, o, rows);
     return ok ? C6_OK : bad("logits: the output overlaps another argument");
 }
@@ -706,7 +712,7 @@ int check_written(const c6_logits *l, const void *out, int64_t stride, const cha
     if (!fits(l->rows, stride, l->width, es)) return bad("logits: the output exceeds the address space");
     if (l->rows > 1 && out == l->x && stride != l->x_stride) return bad("logits: in place needs the same stride");
     if (out == l->x) return C6_OK;
-    return apart(Span{out, stride * es, l->width * es}, Span{l->x, l->x_stride * es, l->width * es}, l->rows) ? C6_OK : bad("logits: the output overlaps x without being x");
+    return apart(Span(out, stride, l->width, es), Span(l->x, l->x_stride, l->width, es), l->rows) ? C6_OK : bad("logits: the output overlaps x without being x");
 }
 
 int check_target(const c6_logits *l, const void *target, int kind, int64_t stride) {
@@ -719,9 +725,7 @@ int check_target(const c6_logits *l, const void *target, int kind, int64_t strid
 }
 
 Span target_span(const c6_logits *l, const void *target, int kind, int64_t stride) {
-    if (kind == C6_TARGET_WEIGHTS) return Span{target, stride * 4, (int64_t)l->width * 4};
-    const int64_t bytes = kind == C6_TARGET_INDEX64 ? 8 : 4;
-    return Span{target, bytes, bytes};
+    return kind == C6_TARGET_WEIGHTS ? Span(target, stride, l->width, 4) : Span(target, 1, 1, kind == C6_TARGET_INDEX64 ? 8 : 4);
 }
 
 // Four rows a wave once that still leaves every SIMD one; 16 lanes count a history for longer, and take twice the rows for it.  Four rows a wave against
@@ -770,8 +774,8 @@ extern "C" int c6_logits_process(const c6_logits *l, const int32_t *history, int
     }
     if (bias && (bias_stride < 0 || !c6_aligned(bias, 4) || !fits(l->rows, bias_stride, l->width, 4))) return bad("c6_logits_process: bad bias");
     const int64_t es = (int64_t)c6_type_bytes(l->type);
-    if (int rc = check_apart(l, Span{out, out_stride * es, l->width * es}, {Span{bias, bias_stride * 4, (int64_t)l->width * 4}, Span{history, history_stride * 4, (int64_t)history_cap * 4},
-                                                                          Span{history ? history_len : nullptr, 4, 4}, Span{history ? penalties : nullptr, penalties_stride * 4, 12}})) return rc;
+    if (int rc = check_apart(l, Span(out, out_stride, l->width, es), {Span(bias, bias_stride, l->width, 4), Span(history, history_stride, history_cap, 4),
+                                                                    Span(history ? history_len : nullptr, 1, 1, 4), Span(history ? penalties : nullptr, penalties_stride, 3, 4)})) return rc;
     if (int rc = c6_check_device(l->device)) return rc;
     if (!l->rows || !l->width) return C6_OK;
     C6DeviceScope scope(l->device);
@@ -871,9 +875,9 @@ extern "C" int c6_policy_loss(const c6_logits *l, const void *target, int target
     if (!c6_aligned(loss, 4) || !c6_aligned(lse, 4) || !c6_aligned(total, 4)) return bad("c6_policy_loss: loss, lse and total are aligned to 4 bytes");
     const int64_t es = (int64_t)c6_type_bytes(l->type);
     const Span t_span = target_span(l, target, target_kind, target_stride);
-    if (int rc = check_apart(l, Span{grad, grad_stride * es, l->width * es}, {t_span, Span{loss, 4, 4}, Span{lse, 4, 4}, Span{total, 4, 4}})) return rc;
+    if (int rc = check_apart(l, Span(grad, grad_stride, l->width, es), {t_span, Span(loss, 1, 1, 4), Span(lse, 1, 1, 4), Span(total, 1, 1, 4)})) return rc;
     for (const float *stat : {loss, lse, total})
-        if (int rc = check_apart(l, Span{stat, 4, 4}, {t_span, Span{l->x, l->x_stride * es, l->width * es}})) return rc;
+        if (int rc = check_apart(l, Span(stat, 1, 1, 4), {t_span, Span(l->x, l->x_stride, l->width, es)})) return rc;
     const int n = l->type == C6_TYPE_F32 ? 4 : 8;
     if (l->rows && splits(l->rows, l->width, n, target_kind == C6_TARGET_WEIGHTS, grad != nullptr) && (!workspace || workspace_bytes < split_bytes(l->rows, l->width, n) || !c6_aligned(workspace, alignof(Part))))
         return bad("c6_policy_loss: the workspace is NULL, smaller than c6_policy_loss_workspace() or not aligned to 16 bytes");
@@ -895,9 +899,10 @@ extern "C" int c6_policy_loss_grad(const c6_logits *l, const void *target, int t
     if (int rc = check_written(l, grad, grad_stride, "c6_policy_loss_grad: grad is NULL")) return rc;
     if (l->rows && (!lse || !total || !dloss)) return bad("c6_policy_loss_grad: lse, total or dloss is NULL");
     if (!c6_aligned(lse, 4) || !c6_aligned(total, 4) || !c6_aligned(dloss, 4)) return bad("c6_policy_loss_grad: lse, total and dloss are aligned to 4 bytes");
-    if (dloss_stride < 0) return bad("c6_policy_loss_grad: negative stride");
+    if (dloss_stride < 0 || !fits(l->rows, dloss_stride, 1, 4)) return bad("c6_policy_loss_grad: bad stride of dloss");
     const int64_t es = (int64_t)c6_type_bytes(l->type);
-    if (int rc = check_apart(l, Span{grad, grad_stride * es, l->width * es}, {target_span(l, target, target_kind, target_stride), Span{lse, 4, 4}, Span{total, 4, 4}, Span{dloss, dloss_stride * 4, 4}})) return rc;
+    if (int rc = check_apart(l, Span(grad, grad_stride, l->width, es), {target_span(l, target, target_kind, target_stride), Span(lse, 1, 1, 4), Span(total, 1, 1, 4), Span(dloss, dloss_stride, 1, 4)}))
+        return rc;
     if (int rc = c6_check_device(l->device)) return rc;
     if (!l->rows || !l->width) return C6_OK;
     C6DeviceScope scope(l->device);

@@ -91,7 +91,7 @@ def net_flops_per_board(n, C, blocks):
     return 2 * 9 * 2 * C * n2 + (blocks - 1) * 2 * (2 * 9 * C * C * n2) + heads
 
 
-CONV_SOURCES = ("conv_wino6.hip", "conv_wino6_gemm.inc", "c6_wino.h", "net_kernels.hip")      # what the FP32 tower's kernels (the ones the PMC summary describes) are compiled from
+CONV_SOURCES = ("conv_wino6.hip", "conv_wino6_gemm.inc", "c6_wino.h", "c6_stream.h", "net_kernels.hip")      # what the FP32 tower's kernels (the ones the PMC summary describes) are compiled from
 
 
 def kernel_source_hash(names=None):

@@ -39,3 +39,14 @@ def test_neighbours_and_interleaved_rows_are_not_refused():
             (process, logits(mask=OUT - 8, mask_row=1, mask_byte=4), {}), (process, logits(mask=OUT + 160, mask_row=2, mask_byte=1), {})]
     for k, (call, l, kw) in enumerate(near):
         assert call(l, **kw) == NO_GPU, (k, pkg.lib().c6_last_error())
+
+
+@pytest.mark.parametrize("kw", [dict(mask=16 * A, mask_row=1 << 62, mask_byte=1), dict(mask=16 * A, mask_row=0, mask_byte=1 << 62), dict(mask=16 * A, mask_row=1 << 61, mask_byte=1 << 61)])
+def test_masks_beyond_the_address_space(kw):
+    assert process(logits(**kw)) == BAD and loss(logits(**kw)) == BAD and grad_of(logits(**kw)) == BAD
+
+
+def test_strides_beyond_the_address_space():
+    assert grad_of(logits(), ds=1 << 62) == BAD
+    if pkg.device_count() == 0:      # strides of what is not there are not looked at
+        assert process(logits(), hs=1 << 62, ps=1 << 62, bs=1 << 62) == NO_GPU and loss(logits(), gs=1 << 62) == NO_GPU
