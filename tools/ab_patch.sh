@@ -7,6 +7,6 @@ n=$1; f=$2; sedf=$3; shift 3
 cd "$(dirname "$0")/.." && mkdir -p tools/ab /tmp/ab_$n
 sed -f $sedf alphazero-connect6_amd/csrc/$f > /tmp/ab_$n/$f
 cmp -s /tmp/ab_$n/$f alphazero-connect6_amd/csrc/$f && { echo "the patch changed nothing"; exit 1; }
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wno-unused-value -Wno-unused-result -I alphazero-connect6_amd/csrc "$@" -x hip -c /tmp/ab_$n/$f -o /tmp/ab_$n/x.o || exit 1
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -fPIC -ffp-contract=off -Wno-unused-value -Wno-unused-result -I alphazero-connect6_amd/csrc "$@" -x hip -c /tmp/ab_$n/$f -o /tmp/ab_$n/x.o || exit 1
 objs=$(ls alphazero-connect6_amd/_build/*.o | grep -v "/$f.o")
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o tools/ab/lib$n.so /tmp/ab_$n/x.o $objs && echo built tools/ab/lib$n.so

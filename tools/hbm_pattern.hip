@@ -2,7 +2,7 @@
 //   pattern 0: SoA planes   addr = cell * G + 4 * lane_global            (the engine's board_soa layout)
 //   pattern 1: tiled AoSoA  addr = (tile * CELLS + cell) * TILE + 4 * lane_in_tile,  TILE = 1024 games (one workgroup)
 //   pattern 2: linear sweep (each wave reads CELLS consecutive 256-byte chunks: upper bound)
-// build: hipcc --offload-arch=gfx950 -O3 tools/hbm_pattern.hip -o /tmp/hbm_pattern ; run: /tmp/hbm_pattern [cells] [games]
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops tools/hbm_pattern.hip -o /tmp/hbm_pattern ; run: /tmp/hbm_pattern [cells] [games]
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

@@ -1,7 +1,7 @@
 """Where the spilled scalar registers' lane moves sit in a kernel's instruction stream: the loops of the gfx950 assembly (backward branches), innermost first,
 with their vector / scalar instruction counts and the v_readlane / v_writelane among them ("660 lane moves of 5 900 static vector
 instructions" of c6_search_kernel<2, 2> -- static counts say nothing about how often an instruction runs; the nesting does).
-    hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -x hip -c alphazero-connect6_amd/csrc/tree_kernels.hip -o /tmp/tree.o -save-temps=obj
+    hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -ffp-contract=off -x hip -c alphazero-connect6_amd/csrc/tree_kernels.hip -o /tmp/tree.o -save-temps=obj
     python tools/isa_loops.py /tmp/tree_kernels-hip-amdgcn-amd-amdhsa-gfx950.s _Z16c6_search_kernelILi2ELi2EEv5C6Devi [min_lines=60]"""
 import re
 import sys

@@ -1,5 +1,5 @@
 // mfma_calib.hip -- calibration of the FP32 and bf16 matrix-core ceilings on this MI355X in the shapes the conv kernels use.
-// Not part of the library.  hipcc --offload-arch=gfx950 -O3 mfma_calib.hip -o mfma_calib
+// Not part of the library.  hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops mfma_calib.hip -o mfma_calib
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

@@ -1,6 +1,6 @@
 // What a write-only / read-only / copy kernel reaches on this part (the yardsticks of conv_wino6.hip's boundary kernels: the first one only
 // writes V, the last one only reads Z and the residual, the ones between read and write):
-//   hipcc --offload-arch=gfx950 -O3 tools/probe/hbm_write.hip -o /tmp/hbm_write && /tmp/hbm_write
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops tools/probe/hbm_write.hip -o /tmp/hbm_write && /tmp/hbm_write
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

@@ -3,7 +3,7 @@
 // weights from a 9 MB L2-resident array (global_load_dwordx4), exactly the bytes per FLOP of c6_wino4_gemm_kernel, without its stores and DMA.
 //   A: v_mfma_f32_32x32x2_f32, wave tile 32 couts x 64 tiles = 2 accumulators of 16 registers (the kernel's form)
 //   B: v_mfma_f32_16x16x4_f32, the same wave tile = 8 accumulators of 4 registers
-// hipcc --offload-arch=gfx950 -O3 mfma_f32_gemmlike.hip -o mfma_f32_gemmlike && ./mfma_f32_gemmlike
+// hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops mfma_f32_gemmlike.hip -o mfma_f32_gemmlike && ./mfma_f32_gemmlike
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

@@ -2,7 +2,7 @@
 // One workgroup per CU (LDS request forces it): waves 0-7 issue v_mfma_f32_32x32x2_f32 (two independent accumulators, as the Winograd GEMM),
 // waves 8..8+X-1 run (A) packed-FMA chains, or (B) a float4 copy of a large buffer with a few packed FMAs per element (what a Winograd
 // boundary transform is: HBM bound, little arithmetic).  Times: MFMA waves alone, side waves alone, both.  both ~ max => they overlap;
-// both ~ sum => they share the pipe.      hipcc --offload-arch=gfx950 -O3 -o /tmp/coissue tools/probe/mfma_valu_coissue.hip && /tmp/coissue
+// both ~ sum => they share the pipe.      hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o /tmp/coissue tools/probe/mfma_valu_coissue.hip && /tmp/coissue
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

@@ -1,5 +1,5 @@
 // Probe (round 3): HIP virtual memory management on this pool -- reserve a large address range, map physical chunks into it as they are
-// needed (a record pool that grows without copying).   hipcc -O2 -o /tmp/vmm tools/probe/vmm_probe.hip && /tmp/vmm
+// needed (a record pool that grows without copying).   hipcc -O2 -Xclang -target-feature -Xclang -packed-fp32-ops -o /tmp/vmm tools/probe/vmm_probe.hip && /tmp/vmm
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #define CK(x) do { hipError_t e_ = (x); if (e_ != hipSuccess) { printf("FAIL %s: %s\n", #x, hipGetErrorString(e_)); return 1; } } while (0)

@@ -3,7 +3,7 @@
 //   O  = the tower's last output transform (c6_w6_out_kernel's body) compiled for <= 112 registers, 4 waves per workgroup, persistent grid
 // so that one workgroup of each fits on a CU together.  Times: G alone, O alone, O launched first (its waves are the OLDER ones) then G on
 // another stream, G first then O.  together ~ max => the boundary kernel's memory time hides under the matrix work; ~ sum => it does not.
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -o tools/probe/_w6_overlap tools/probe/w6_overlap.hip && tools/probe/_w6_overlap
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -ffp-contract=off -o tools/probe/_w6_overlap tools/probe/w6_overlap.hip && tools/probe/_w6_overlap
 #include "../../alphazero-connect6_amd/csrc/conv_wino6.hip"
 #include <chrono>
 #include <thread>

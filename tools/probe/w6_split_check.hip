@@ -1,5 +1,5 @@
 // Check (round 5): c6_w6_gemm_kernel's SPLIT form (rows as work items) against the block form on the same V / U: Z must be bit-identical
-// (the same instruction stream per position).   hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -o tools/probe/_w6_split_check tools/probe/w6_split_check.hip
+// (the same instruction stream per position).   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -ffp-contract=off -o tools/probe/_w6_split_check tools/probe/w6_split_check.hip
 #include "../../alphazero-connect6_amd/csrc/conv_wino6.hip"
 #include <cstdio>
 #include <vector>
