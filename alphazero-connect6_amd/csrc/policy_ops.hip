@@ -26,12 +26,14 @@ __device__ __forceinline__ uint32_t legal_bits(uint32_t byte, int c) { return by
 
 // ---- penalties, biases, masks -------------------------------------------------------------------------------------------
 // Bound by memory: every logit in and out once.  A row is cut into chunks; LANES threads take one chunk: of many rows of up to 384 entries 16 lanes each
-// (lanes_of()), a wave for rows of up to 1024, else a workgroup per 4096 (48 rows of 100003 bf16 with up to 2048 ids take 8.8 us so, 10.8 in chunks of
-// 8192: a larger chunk scans the history less often but leaves fewer waves).  The chunk's logits, mask and bias and the history's beginning are requested
+// (lanes_of()), a wave for rows of up to 1024, else a workgroup per 4096 (in chunks of 8192 48 rows of 100003 bf16 with up to 2048 ids took a
+// fifth longer: a larger chunk scans the history less often but leaves fewer waves).  The chunk's logits, mask and bias and the history's beginning are requested
 // first, 16 bytes a lane and all in flight, and wait in registers while the row's history is counted in LDS: each chunk reads the whole history and counts
 // the ids that fall into it (integer adds: the order does not matter).  Asking for the history's length only once the row had come cost 15 % of the time.
+// Every lane loads U pieces whether its row has them or not: 361 f32 entries on 64 lanes are 90 pieces of the 256 that are asked for (the surplus ones are the
+// last piece again, from the L1).
 // Measured, kernel alone: 512 x 131072 f32 96 us without mask and history (5.6 TB/s; a copy of that size 99), 104 us with both; 48 x 100003 bf16 with 2048
-// ids, mask and bias 9.2 us; 4096 x 361 f32 with 200 moves, legal masks and bias 7.2 us; one row of 361 2.0 us.
+// ids, mask and bias 9.1 us; 4096 x 361 f32 with 200 moves, legal masks and bias 7.4 us; one row of 361 2.0 us.
 struct Repeats {
     const int32_t *history, *len;
     const float *penalties;
@@ -189,7 +191,8 @@ struct alignas(16) Part {
     float m, s, w, d;
 };
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
-// exp(a) as 2^(a log2 e): half steps of |a| in the argument and of the result, where expf costs three times as many instructions
+// exp(a) as 2^(a log2 e): two half steps of |a| relative (1e-6 at |a| = 20, 5e-6 at 80) and the result's own, results below 2^-126 are 0; expf costs three times
+// as many instructions
 __device__ __forceinline__ float exp_of(float a) { return __builtin_amdgcn_exp2f(a * LOG2E); }
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
 
@@ -449,10 +452,11 @@ __device__ __forceinline__ void gradient(float x, const At &at, const Done &k, i
 // One pass over rows that fit the registers of LANES lanes: read once, the gradient written once.  A lane takes the maximum of its own entries, the sums
 // relative to that, and one reduction over the lanes joins them.  As a piece's gradient leaves, the same piece of the workgroup's next row is requested
 // into its registers: loads and stores overlap, and the sums of a row begin as its first pieces arrive.
-// Measured, loss and gradient: 2049 x 100003 bf16 187 us (4.4 TB/s; 1020 in three passes over each row).  There a workgroup has a CU to itself (up to 122 registers
+// Measured, loss and gradient: 2049 x 100003 bf16 187 us a launch among others (4.4 TB/s; 198 to 202 on its own; 1020 in three passes over each row).  There a workgroup has a CU to itself (up to 122 registers
 // a lane, 16 waves) and the vector unit is busy for half the time, two exponentials an element of it: what is left over the 149 us of a copy is the part of
 // that work which one row's loads do not cover, a row address aligned to two bytes (3 us), and the 2049th row.  2048 x 16000 f32 45 us (5.8 TB/s),
-// 16384 x 361 bf16 against weights 12 us, 2048 x 225 f32 4 us.
+// 16384 x 361 bf16 against weights 11 us, 2048 x 225 f32 4 us.  The loss alone, 32768 x 361 bf16: 8.8 us for 24 MB, the vector unit busy for 4.6 of them, the rest
+// the latency of one round of loads and of the reductions.  Against weights 16-bit rows of 1024 lanes and 8 pieces spill 3 registers (16 bytes of scratch).
 template <typename T, int LANES, int NV, bool WEIGHTS>
 __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void c6_policy_loss_kernel(Rows l, Target t, float *loss, float *lse, float *total, T *grad, int64_t grad_stride, float scale) {
     typedef C6Vec<T> V;
@@ -498,8 +502,9 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void c6_policy_loss_kern
 }
 
 // The same in two launches, for rows that do not fit or are too few to fill the card: every chunk's Part into the workspace, then each chunk joins its
-// row's and writes its piece of the gradient.  3 x 131072 f32: 3.2 + 4.6 us; without a gradient 2048 x 100003 bf16 77 us (5.3 TB/s) and 7; with
-// masks both together 101, where masks read only as they are needed made it 114.
+// row's and writes its piece of the gradient.  3 x 131072 f32: 3.6 + 4.9 us; without a gradient 2048 x 100003 bf16 77 us (5.3 TB/s) and 7; with
+// masks both together 101, where masks read only as they are needed made it 114.  With a gradient logits and weights are read twice (12 bytes an f32 entry
+// instead of 8): 512 x 131072 f32 155 us against the move, 241 against weights (3.4 TB/s of the bytes read and written once), 2048 x 152064 bf16 352 and 792 us.
 constexpr int SPLIT_NV = 4, JOIN_MOST = 1024;
 template <typename T>
 constexpr int split_chunk = 256 * SPLIT_NV * C6Vec<T>::N;
@@ -803,7 +808,9 @@ extern "C" int c6_logits_process(const c6_logits *l, const int32_t *history, int
 // Which way the loss goes, by the pieces of N entries (16 bytes) in a row.  The registers of 64, 256 or 1024 lanes hold up to 16384 (against weights, which
 // need registers of their own, 8192).  Split into chunks go
 //   longer rows;
-//   rows of over 8192 pieces that are too few for a workgroup each to fill the card (3 x 100003 bf16: 17.7 us in one workgroup a row);
+//   rows of over 8192 pieces that are too few for a workgroup each to fill the card (3 x 100003 bf16: 17.7 us in one workgroup a row).  The border of 128 rows
+//   is half of the CUs, not a measured one: from there to some 600 rows the last round of workgroups leaves much of the card idle (with a gradient, bf16, 80001
+//   wide: 129 rows 17 us, 257 28, 300 33, 512 36);
 //   without a gradient nothing need be held: from 2048 pieces on small workgroups are faster (2048 x 100003 bf16: 77 against 113 us; few rows: one launch is).
 static bool splits(int64_t rows, int64_t width, int n, bool weights, bool grad) {
     const int64_t pieces = (width + n - 1) / n;
@@ -836,9 +843,10 @@ static bool loss_launch(const c6_logits *l, const Target &t, float *loss, float 
 #define C6_LAUNCH(LANES, NV, RESIDENT)                                                                                                                                       \
     return c6_launch(c6_policy_loss_kernel<T, LANES, NV, WEIGHTS>, (unsigned)std::min<int64_t>(LANES < 256 ? ((int64_t)l->rows * LANES + 255) / 256 : l->rows, (int64_t)cus() * RESIDENT), \
                      LANES < 256 ? 256 : LANES, s, rows, t, loss, lse, total, grad, grad_stride, scale)
-    // The pieces that a lane may hold come in steps of a third or less: those beyond the row take part in its sums all the same (in steps of two 300 x 80001
-    // bf16 took 37.1 us instead of 33.3, 2048 x 20000 f32 85.7 instead of 80.3, 2048 x 24000 bf16 against weights 92.0 instead of 85.5; skipped by a branch
-    // they cost 2048 x 128000 bf16, where there are none, 8 %)
+    // Pieces beyond the row take part in its sums all the same.  From 2048 on the pieces held go up by a half or a third, below by two (four short rows a wave: by a
+    // half or a third): by two everywhere 300 x 80001 bf16 took 37.1 us instead of 33.3, 2048 x 20000 f32 85.7 instead of 80.3, 2048 x 24000 bf16 against weights
+    // 92.0 instead of 85.5.  14 pieces of 1024 lanes: rows of 12289 to 14336 pieces, among them a 16-bit vocabulary of 100 thousand (2049 x 100003 198 -> 194.5 us).
+    // (Skipped by a branch surplus pieces cost 2048 x 128000 bf16, where there are none, 8 %.)
     const int pieces = (l->width + N - 1) / N;
     const bool many = l->rows >= MANY;
     if (many && pieces <= 32) C6_LAUNCH(16, 2, 1 << 14);

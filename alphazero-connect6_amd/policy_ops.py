@@ -217,7 +217,10 @@ class GradClip:
 
     Made once for buffers that stay where they are (it keeps them alive): contiguous float32 / float16 / bfloat16 tensors of one device, of any
     number and size.  outs: tensors like grads to write to; None: in place.  A graph that captured a call needs the object for as long as it is
-    replayed."""
+    replayed.
+
+    An optimizer's zero_grad() drops the gradients by default, and the next backward pass makes new ones that the object does not know: keep them with
+    zero_grad(set_to_none=False)."""
     _late = []       # tables of objects that were collected: freed when the next one is made or closed, not by the collector, whose moment nobody chooses
 
     def __init__(self, grads, outs=None):

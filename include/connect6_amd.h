@@ -605,7 +605,8 @@ int c6_logits_process(const c6_logits *l, const int32_t *history, int64_t histor
  *     lse = log sum exp(x),   total = sum t,   loss = sum t (lse - x),   gradient = scale * (total * exp(x - lse) - t)
  * over the legal entries; the gradient of the others is 0.  A row without a legal entry above -infinity: loss = total = 0,
  * lse = -infinity, gradient 0.  NaN or +infinity at a legal entry makes the row NaN: its loss, lse and gradient (there at the legal entries for
- * certain, at the others either NaN or 0).  Statistics are held in 32 bits. */
+ * certain, at the others either NaN or 0).  Statistics are held in 32 bits; exponentials are off by some 2^-23 |x - lse| relative, and 0 below
+ * 2^-126. */
 enum {
     C6_TARGET_INDEX32 = 0,   /* target: int32 [rows], t = 1 at that entry; an index outside [0, width) or at an illegal entry: t = 0 everywhere */
     C6_TARGET_INDEX64 = 1,   /* ... int64 */
@@ -626,7 +627,7 @@ int c6_policy_loss_grad(const c6_logits *l, const void *target, int target_kind,
  *     norm = sqrt(sum of g^2 over every element of every tensor),   out = g * min(1, max_norm / (norm + 1e-6))
  * The sum is held in 64 bits (no overflow, nothing lost among many elements) in a fixed order: the same gradients give the same bits.
  * A c6_clip is the device-side table of the tensors' addresses, made once for buffers that stay where they are; it is only read
- * afterwards. */
+ * afterwards.  (Gradients that are allocated anew need a new one: the old one clips the old buffers.) */
 typedef struct c6_clip c6_clip;
 /* grads[i] / outs[i]: sizes[i] contiguous elements of types[i] (C6_TYPE_*), aligned to their type; a size may be 0.  outs NULL, or
  * outs[i] == grads[i]: in place.  Written memory may not overlap other memory of the table.  count 0: norm 0. */
