@@ -14,3 +14,10 @@ def test_no_packed_fp32_anywhere():
 
 def test_objects_depend_on_the_makefile():
     assert re.search(r"^\$\(OUT\)/%\.o:.*\bMakefile\b", MK, re.M)
+
+
+def test_build_compiles_every_time():
+    import inspect
+
+    import __graft_entry__ as g
+    assert '"make", "-B"' in inspect.getsource(g.build)
