@@ -52,10 +52,11 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 #define M8_XH_MAX 3584.0f   // 448 * 2^3
 #define M8_HEADER 16        // bytes in front of the weight planes: int32 d
 
-// The accumulator passes through an empty asm behind its MFMA: tied there, it stays in its registers.  Left alone hipcc renames accumulator tiles from one MFMA
-// to the next and, at 256 VGPRs, ends up moving and spilling whole tiles inside the K loop (20 tile moves + 13 tile spills per tap pair in one
-// instantiation, none in another: chaotic).  (Not MFMAs in asm: their wait states before and behind them would be nobody's.)
-#define M8_PIN(ACC) asm volatile("" : "+v"(ACC))
+// At 256 channels (two waves a SIMD, 256 registers each) the accumulator passes through an empty asm behind its MFMA: tied there, it stays in its registers.
+// Left alone hipcc renames accumulator tiles from one MFMA to the next and ends up moving and spilling whole tiles inside the K loop (20 tile moves + 13 tile
+// spills per tap pair in one instantiation, none in another: chaotic).  Smaller towers have the registers and keep their accumulators in AGPRs, which the empty
+// asm would move them out of.  (Not MFMAs in asm: their wait states before and behind them would be nobody's.)
+#define M8_PIN(ACC) do { if (C == 256) asm volatile("" : "+v"(ACC)); } while (0)
 #define M8_MFMA16(ACC, A, B) do { ACC = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, B, ACC, 0, 0, 0); M8_PIN(ACC); } while (0)
 #define M8_MFMA8(ACC, A, B, SA, SB) do { ACC = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, ACC, 0, 0, 0, SA, 0, SB); M8_PIN(ACC); } while (0)
 
@@ -74,7 +75,7 @@ struct M8Geom {
 };
 
 template <int C, int N, bool HEAD = false>
-__global__ __launch_bounds__(64 * (C / 32), 2) void c6_conv3x3_m8_kernel(const float *__restrict__ in, const unsigned char *__restrict__ wp_,
+__global__ __launch_bounds__(64 * (C / 32)) void c6_conv3x3_m8_kernel(const float *__restrict__ in, const unsigned char *__restrict__ wp_,
                                                                       const float *__restrict__ bias, const float *__restrict__ res,
                                                                       float *__restrict__ out, int nboards, int relu,
                                                                       const float *__restrict__ head_w, unsigned int *__restrict__ range_flag,
