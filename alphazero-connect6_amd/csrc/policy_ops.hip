@@ -684,7 +684,7 @@ struct Span {
     int64_t stride = 0, width = 0;
     Span(const void *p_, int64_t stride_, int64_t width_, int64_t bytes) {
         if (!p_) return;
-        p = p_; stride = stride_ * bytes; width = width_ * bytes;
+        p = p_; stride = (int64_t)((uint64_t)stride_ * (uint64_t)bytes); width = width_ * bytes;      // (a single row's stride may be anything)
     }
 };
 // nothing of the one is part of the other: apart as a whole, or rows of both interleave in one buffer
